@@ -277,7 +277,7 @@ def _write8(m, v, bits):
     y = [(m.abs().view(-1, BLOCK) / per[0][:, None]).view(-1), (v.view(-1, BLOCK) / per[1][:, None]).view(-1)]
     codes = []
     for x, half, r in ((y[0], 8, bits & 0xFFFF), (y[1], 16, bits >> 16)):
-        e = (torch.frexp(x)[1] - 1).clamp(min=-6)
+        e = (torch.frexp(x)[1] - 1).clamp(min=-6).masked_fill_(x == 0, -6)  # zero has no exponent: its code is 0
         q = torch.floor(x * half * torch.ldexp(torch.ones_like(x), -e) + (r.double() + 0.5) / 65536)
         codes.append((e + 6) * half + q.long())
     first = codes[0].clamp(max=127) + 128 * (m < 0)
