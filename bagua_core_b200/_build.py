@@ -36,6 +36,7 @@ SOURCES = [
     "comm/solo_transport.cc",
     "ops/ops.cc",
     "telemetry/telemetry.cc",
+    "trainer/adamw_plan.cc",
     "trainer/autograd_ops.cc",
     "trainer/gemm.cc",
     "trainer/grad_hooks.cc",
@@ -58,6 +59,8 @@ SOURCES = [
     "kernels/conv_wgrad.cu",
     "kernels/model_ops_cpu.cc",
     "kernels/encoder_ops.cu",
+    "kernels/adamw.cu",
+    "kernels/adamw_host.cc",
 ]
 
 

@@ -29,6 +29,7 @@
 #include "runtime/timeline.h"
 #include "telemetry/telemetry.h"
 #include "tensor/tensor.h"
+#include "trainer/adamw_plan.h"
 #include "trainer/autograd_ops.h"
 #include "trainer/grad_hooks.h"
 #include "trainer/sgd_plan.h"
@@ -1024,6 +1025,46 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
            },
            py::arg("groups"), py::arg("stream"))
       .def("zero_grad", &trainer::SgdPlan::zero_grad, py::arg("stream"));
+  // The numbers of a step are ints, or an int64 tensor on the device.
+  static auto step_numbers = [](const py::object& steps) {
+    trainer::StepNumbers n;
+    if (THPVariable_Check(steps.ptr()))
+      n.device = THPVariable_Unpack(steps.ptr());
+    else if (py::isinstance<py::int_>(steps))
+      n.host = {steps.cast<int64_t>()};
+    else
+      n.host = steps.cast<std::vector<int64_t>>();
+    return n;
+  };
+  py::class_<trainer::AdamWPlan>(m, "AdamWPlan")
+      .def(py::init([]() {
+        auto p = std::make_unique<trainer::AdamWPlan>();
+        p->keep = true;
+        return p;
+      }))
+      .def("add", &trainer::AdamWPlan::add, py::arg("param"), py::arg("grad"), py::arg("exp_avg"), py::arg("exp_avg_sq"), py::arg("scales"),
+           py::arg("bf16_shadow"), py::arg("group"))
+      .def("step",
+           [](trainer::AdamWPlan& p, const std::vector<std::tuple<double, double, double, double, double>>& groups, const py::object& step,
+              uint64_t seed) {
+             std::vector<adamw::GroupValues> gs;
+             for (auto& [lr, b1, b2, eps, wd] : groups) gs.push_back({lr, b1, b2, eps, wd});
+             return p.step(gs, step_numbers(step), seed);
+           },
+           py::arg("groups"), py::arg("step"), py::arg("seed"))
+      .def("zero_grad", &trainer::AdamWPlan::zero_grad, py::arg("stream"));
+  m.def(
+      "adamw_step",
+      [](const trainer::TensorList& p, const trainer::TensorList& g, const trainer::TensorList& ms, const trainer::TensorList& vs,
+         const std::optional<trainer::TensorList>& scales, const std::optional<trainer::TensorList>& copies, double lr, double b1, double b2,
+         double eps, double wd, const py::object& step, uint64_t seed, uint32_t first_index) {
+        return trainer::adamw_step(p, g, ms, vs, scales, copies, {lr, b1, b2, eps, wd}, step_numbers(step), seed, first_index);
+      },
+      py::arg("params"), py::arg("grads"), py::arg("exp_avgs"), py::arg("exp_avg_sqs"), py::arg("scales"), py::arg("copies"), py::arg("lr"),
+      py::arg("beta1"), py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"), py::arg("step"), py::arg("seed"), py::arg("first_index"));
+  m.def("adamw_read8", &trainer::adamw_read8, py::arg("exp_avgs"), py::arg("exp_avg_sqs"), py::arg("scales"), py::arg("exp_avgs_out"),
+        py::arg("exp_avg_sqs_out"));
+  m.attr("moment8_block") = adamw::kMoment8Block;
   py::class_<trainer::GradHooks, std::shared_ptr<trainer::GradHooks>>(m, "GradHooks")
       .def(py::init([](PyBackend& be, int device) { return std::make_shared<trainer::GradHooks>(be.inner, device); }),
            py::arg("backend"), py::arg("device"))

@@ -30,7 +30,7 @@ void SgdPlan::add(const at::Tensor& p, const at::Tensor& g, const at::Tensor& m,
   a.first = true;
   segs_.push_back(a);
   group_.push_back(group);
-  grad_buffer_.push_back(g.storage().data());
+  grads_.add(g);
   keep_.insert(keep_.end(), {p, g, m});
   if (shadow) keep_.push_back(*shadow);
 }
@@ -59,19 +59,24 @@ int SgdPlan::step(const std::vector<SgdGroup>& groups, uint64_t stream) {
   return launches;
 }
 
-void SgdPlan::zero_grad(uint64_t stream) {
+void GradBuffers::add(const at::Tensor& g) {
+  slices_.emplace_back((float*)g.data_ptr(), g.numel());
+  buffer_.push_back(g.storage().data());
+}
+
+void GradBuffers::zero(int device, uint64_t stream) const {
   std::vector<kernels::cuda::FillSegment> fill;
-  for (size_t k = 0; k < segs_.size();) {
+  for (size_t k = 0; k < slices_.size();) {
     // slices of one buffer follow each other: one segment for all of them (never over two buffers, which may lie next
     // to each other in separate allocations)
-    float* from = const_cast<float*>(segs_[k].g);
-    const void* buffer = grad_buffer_[k];
+    float* from = slices_[k].first;
+    const void* buffer = buffer_[k];
     int64_t n = 0;
-    for (; k < segs_.size() && grad_buffer_[k] == buffer && segs_[k].g == from + n; ++k) n += segs_[k].n;
+    for (; k < slices_.size() && buffer_[k] == buffer && slices_[k].first == from + n; ++k) n += slices_[k].second;
     if (n) fill.push_back({from, n});
   }
-  if (device_ >= 0) {
-    const c10::cuda::CUDAGuard on((c10::DeviceIndex)device_);  // memory can be set from any device, a kernel not
+  if (device >= 0) {
+    const c10::cuda::CUDAGuard on((c10::DeviceIndex)device);  // memory can be set from any device, a kernel not
     kernels::cuda::fill_zero(fill.data(), (int)fill.size(), (cudaStream_t)stream);
   } else {
     for (const auto& f : fill) std::memset(f.p, 0, (size_t)f.n * sizeof(float));

@@ -7,6 +7,7 @@
 #include <ATen/ATen.h>
 
 #include <optional>
+#include <utility>
 #include <vector>
 
 #include "../kernels/kernels.h"
@@ -19,6 +20,17 @@ struct SgdGroup {
   bool nesterov;
 };
 
+// The gradients of a plan, zeroed together.
+class GradBuffers {
+ public:
+  void add(const at::Tensor& g);
+  void zero(int device, uint64_t stream) const;
+
+ private:
+  std::vector<std::pair<float*, int64_t>> slices_;
+  std::vector<const void*> buffer_;  // of each slice: the storage it lies in
+};
+
 class SgdPlan {
  public:
   // One buffer (or a slice of one) whose parameters all belong to parameter group `group`.
@@ -26,14 +38,14 @@ class SgdPlan {
            int group);
   // Steps every buffer with its group's hyperparameters; returns the number of kernels launched.
   int step(const std::vector<SgdGroup>& groups, uint64_t stream);
-  void zero_grad(uint64_t stream);
+  void zero_grad(uint64_t stream) { grads_.zero(device_, stream); }
   bool empty() const { return segs_.empty(); }
 
  private:
   int device_ = -1;
   std::vector<kernels::SgdSegment> segs_;
   std::vector<int> group_;
-  std::vector<const void*> grad_buffer_;  // of each segment: the storage its gradient lies in
+  GradBuffers grads_;
   std::vector<at::Tensor> keep_;
 };
 

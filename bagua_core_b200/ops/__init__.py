@@ -10,6 +10,7 @@ import torch
 
 from .._native import C as _C
 from .. import BaguaTensorPy
+from .adamw import adamw_read8, adamw_state8, adamw_step  # noqa: F401
 
 
 def _s(t: torch.Tensor, stream=None) -> int:

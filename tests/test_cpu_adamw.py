@@ -1,0 +1,246 @@
+"""AdamW steps over lists of tensors (`ops.adamw_step`), moments in fp32 and in 8 bits, and the flat optimizer on them: on the
+host, against the definition in 64 bits.  The GPU runs the same checks (`test_gpu_adamw.py`)."""
+import copy
+
+import pytest
+import torch
+
+import adamw_plain as plain
+import bagua_core_b200.ops as ops
+import bagua_core_b200.parallel as P
+
+TYPES = [(torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.float32, torch.float16),
+         (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float16), (torch.float16, torch.float32)]
+SIZES = [1, 3, 255, 256, 257, 1024, 5000]
+HYPER = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
+U = 2.0 ** -24  # half a step of fp32
+
+
+def tensors(sizes, dtypes, device, seed=0):
+    """Parameters, gradients and moments whose sizes differ from block to block by orders of magnitude."""
+    g = torch.Generator().manual_seed(seed)
+    ps, gs, ms, vs = [], [], [], []
+    for n in sizes:
+        scale = torch.exp(2 * torch.randn((n + 255) // 256, generator=g) - 6).repeat_interleave(256)[:n]
+        ps.append(torch.randn(n, generator=g).to(dtypes[0]))
+        gs.append((torch.randn(n, generator=g) * scale).to(dtypes[1]))
+        ms.append(torch.randn(n, generator=g) * scale * 0.3)
+        vs.append((torch.randn(n, generator=g) * scale).square() + 0.1 * scale * scale)
+    return [[t.to(device) for t in x] for x in (ps, gs, ms, vs)]
+
+
+def close_param(got, want, old, dtype, lr):
+    """p is rounded to its type once; before that: three fp32 roundings of p's size, and of the update (at most 10 lr here, since the
+    moments of a test fit each other to within that) its division, its factors and both moments, 16 roundings at most."""
+    half = torch.finfo(dtype).eps / 2
+    bound = want.abs() * half + torch.finfo(dtype).smallest_normal * half + 3 * U * (old.double().abs() + want.abs()) + 10 * lr * 16 * U
+    assert ((got.cpu().double() - want).abs() <= bound).all()
+
+
+def check_step32(device, dtypes, t, copies=True, sizes=SIZES, hyper=HYPER):
+    ps, gs, ms, vs = tensors(sizes, dtypes, device)
+    old = [[t.cpu().clone() for t in x] for x in (ps, gs, ms, vs)]
+    cs = [torch.zeros_like(p, dtype=torch.bfloat16) for p in ps] if copies else None
+    ops.adamw_step(ps, gs, ms, vs, step=t, copies=cs, **hyper)
+    b1, b2 = hyper["betas"]
+    for k in range(len(sizes)):
+        p, g, m, v = (x[k] for x in old)
+        want = plain.step(p, g, m, v, t, hyper["lr"], b1, b2, hyper["eps"], hyper["weight_decay"])
+        close_param(ps[k], want[0], p, dtypes[0], hyper["lr"])
+        # a product, a multiply-add and two constants rounded: two half steps of each term and one of the sum
+        assert ((ms[k].cpu().double() - want[1]).abs() <= 3 * U * ((b1 * m).abs() + ((1 - b1) * g.double()).abs()) + 1e-45).all()
+        assert ((vs[k].cpu().double() - want[2]).abs() <= 4 * U * (b2 * v + (1 - b2) * g.double().square()) + 1e-45).all()
+        assert torch.equal(gs[k].cpu(), g)
+        if copies and dtypes[0] == torch.float32:
+            assert torch.equal(cs[k], ps[k].bfloat16())
+
+
+def check_step8(device, dtypes, t, sizes=SIZES, seed=7, first_index=2, offset=0):
+    """One step from moments that were written by earlier steps; `offset`: where the tensors start in their memory."""
+    ps, gs, _, _ = tensors(sizes, dtypes, device)
+    if offset:
+        move = lambda xs: [torch.zeros(x.numel() + offset, dtype=x.dtype, device=device)[offset:].copy_(x) for x in xs]  # noqa: E731
+        ps, gs = move(ps), move(gs)
+    state = [ops.adamw_state8(p) for p in ps]
+    if offset:
+        state = [(move([a])[0], move([b])[0], s) for a, b, s in state]
+    ms, vs, ss = ([s[i] for s in state] for i in range(3))
+    b1, b2 = HYPER["betas"]
+    for j in range(1, 3):
+        ops.adamw_step(ps, gs, ms, vs, step=j, scales=ss, seed=seed, **HYPER)
+        gs = [g * 0.7 + g.roll(1) * 0.5 if g.numel() > 1 else g for g in gs]
+    old = [[t.cpu().clone() for t in x] for x in (ps, gs, ms, vs, ss)]
+    ops.adamw_step(ps, gs, ms, vs, step=t, scales=ss, seed=seed, first_index=first_index, **HYPER)
+    for k, n in enumerate(sizes):
+        m0, v0 = plain.read(old[2][k], old[3][k], old[4][k])
+        want, m, v = plain.step(old[0][k], old[1][k], m0, v0, t, HYPER["lr"], b1, b2, HYPER["eps"], HYPER["weight_decay"])
+        close_param(ps[k], want, old[0][k], dtypes[0], HYPER["lr"])
+        random = plain.random_bits(seed, t, first_index + k, n)
+        # the moments (4 half steps), the scale (their largest, divided: 5), its reciprocal and the product (2)
+        slack = 12 * U
+        for x, row, largest, table, u, code in ((m, 0, 480, plain.FIRST, random & 0xFFFF, ms[k]), (v, 1, 496, plain.SECOND, random >> 16, vs[k])):
+            scale = ss[k][row].cpu().double()
+            assert ((scale - plain.tops(x) / largest).abs() <= 6 * U * scale + 2.0 ** -126).all()
+            lo, hi = plain.codes(x, plain.spread(ss[k][row].cpu(), n), table, (u.double() + 0.5) / 65536, slack)
+            c = code.cpu().long().flatten()
+            if row == 0:
+                # the first moment is a difference where its two terms cancel: allow what they leave
+                terms = (b1 * m0.abs() + (1 - b1) * old[1][k].double().abs()) * 4 * U / plain.spread(ss[k][0].cpu(), n).clamp(min=1e-300)
+                lo2, _ = plain.codes((x.abs() / plain.spread(ss[k][0].cpu(), n) - terms).clamp(min=0), torch.ones(n, dtype=torch.float64), table,
+                                     (u.double() + 0.5) / 65536, slack)
+                _, hi2 = plain.codes(x.abs() / plain.spread(ss[k][0].cpu(), n) + terms, torch.ones(n, dtype=torch.float64), table,
+                                     (u.double() + 0.5) / 65536, slack)
+                lo, hi = torch.minimum(lo, lo2), torch.maximum(hi, hi2)
+                assert ((c & 127 >= lo) & (c & 127 <= hi)).all()
+                assert (((c > 127) == (x < 0)) | (c & 127 == 0)).all()
+            else:
+                assert ((c >= lo.clamp(min=1)) & (c <= hi.clamp(min=1)) | (x == 0) & (c == 0)).all()
+    outs = [[torch.empty_like(p, dtype=d) for p in ms] for d in (torch.float32, torch.float32)]
+    ops.adamw_read8(ms, vs, ss, *outs)
+    for k, n in enumerate(sizes):
+        m, v = plain.read(ms[k], vs[k], ss[k])
+        assert ((outs[0][k].cpu().double() - m).abs() <= U * m.abs() + 1e-45).all()
+        assert ((outs[1][k].cpu().double() - v).abs() <= U * v.abs() + 1e-45).all()
+
+
+@pytest.mark.parametrize("dtypes", TYPES)
+@pytest.mark.parametrize("t", [1, 1000])
+def test_step_with_fp32_moments(dtypes, t):
+    check_step32("cpu", dtypes, t)
+
+
+@pytest.mark.parametrize("dtypes", TYPES)
+def test_step_with_8_bit_moments(dtypes):
+    check_step8("cpu", dtypes, 3)
+
+
+def check_mean(device):
+    """Moments that a step changes by less than a code's distance follow their mean: a constant gradient after another one."""
+    n = 1 << 14
+    p, g = torch.zeros(n, device=device), torch.full((n,), 1e-3, device=device)
+    g[::256] = 4e-3  # the largest of each block
+    m, v, s = ops.adamw_state8(p)
+    for t in range(1, 2001):
+        if t == 1001:
+            g *= 0.5
+        ops.adamw_step([p], [g], [m], [v], step=t, lr=0.0, weight_decay=0.0, scales=[s], seed=3)
+    mean_m, mean_v, ref = torch.zeros(1, device=device), torch.zeros(1, device=device), 0.0
+    out = torch.empty_like(p), torch.empty_like(p)
+    ops.adamw_read8([m], [v], [s], [out[0]], [out[1]])
+    keep = torch.arange(n, device=device) % 256 != 0
+    mean_m, mean_v = out[0][keep].double().mean().item(), out[1][keep].double().mean().item()
+    for t in range(1, 2001):
+        ref = 0.999 * ref + 0.001 * ((1e-3 if t <= 1000 else 5e-4) ** 2)
+    # standard error of the mean over 16320 elements: a code's rounding varies by at most 1/64 of its square (v: an element in
+    # between two codes a sixteenth apart), summed over 500 steps' memory: 35 % of an element, 0.3 % of the mean; five of them
+    assert abs(mean_v / ref - 1) < 0.015
+    assert abs(mean_m / 5e-4 - 1) < 0.005
+
+
+def test_8_bit_moments_follow_their_mean():
+    check_mean("cpu")
+
+
+def check_special(device):
+    z = lambda *v: torch.tensor(v, dtype=torch.float32, device=device)  # noqa: E731
+    # no gradient ever: nothing moves but by the weight decay
+    p, g = z(1.0, -2.0), z(0.0, 0.0)
+    m, v, s = ops.adamw_state8(p)
+    ops.adamw_step([p], [g], [m], [v], step=1, lr=0.1, weight_decay=0.5, scales=[s])
+    assert torch.equal(p.cpu(), torch.tensor([0.95, -1.9])) and not m.any() and not v.any() and not s.any()
+    # gradients at the ends of fp32's range, and one that is not finite: that block, and no other, is lost
+    p = torch.zeros(512, device=device)
+    g = torch.full((512,), 1e-20, device=device)
+    g[300] = float("inf")
+    m, v, s = ops.adamw_state8(p)
+    ops.adamw_step([p], [g], [m], [v], step=1, lr=0.1, scales=[s])
+    assert torch.isfinite(p[:256]).all() and torch.isfinite(s[:, 0]).all() and s[:, 1].isnan().all()
+    out = torch.empty_like(p), torch.empty_like(p)
+    ops.adamw_read8([m], [v], [s], [out[0]], [out[1]])
+    assert out[0][256:].isnan().all() and torch.isfinite(out[0][:256]).all()
+    # moments below the smallest normal number: held or lost, never infinite
+    for size in (1e-36, 1e-38, 1e-42, 1e-45):
+        p, g = torch.zeros(300, device=device), torch.full((300,), size, device=device)
+        m, v, s = ops.adamw_state8(p)
+        for t in range(1, 4):
+            ops.adamw_step([p], [g], [m], [v], step=t, lr=0.1, scales=[s])
+        assert torch.isfinite(p).all() and torch.isfinite(s).all()
+    # empty lists and empty tensors
+    assert ops.adamw_step([], [], [], [], step=1, lr=0.1) == 0
+    e = torch.empty(0, device=device)
+    ops.adamw_step([e], [e.clone()], [e.clone()], [e.clone()], step=1, lr=0.1)
+    # matrices whose elements lie in another order than their rows
+    p = torch.randn(30, 20, device=device).t()
+    g, m, v = (torch.rand(30, 20, device=device).t() for _ in range(3))
+    want = plain.step(p.cpu(), g.cpu(), m.cpu(), v.cpu(), 5, 0.1, 0.9, 0.999, 1e-8, 0.01)
+    ops.adamw_step([p], [g], [m], [v], step=5, lr=0.1)
+    close_param(p, want[0], torch.ones(20, 30) * 4, torch.float32, 0.1)
+
+
+def test_special_values():
+    check_special("cpu")
+
+
+def check_refusals(device):
+    t = lambda n=8, d=torch.float32: torch.zeros(n, dtype=d, device=device)  # noqa: E731
+    good = dict(step=1, lr=0.1)
+    s8 = ops.adamw_state8(t())
+    both = t(12)
+    for args, more in [
+        (([t()], [t()], [t()], []), good),                                               # lists of different lengths
+        (([t()], [t(9)], [t()], [t()]), good),                                           # sizes
+        (([t(8, torch.float64)], [t(8, torch.float64)], [t()], [t()]), good),            # types
+        (([t(8, torch.bfloat16)], [t(8, torch.float16)], [t()], [t()]), good),
+        (([t()], [t()], [t(8, torch.bfloat16)], [t(8, torch.bfloat16)]), good),
+        (([t()], [t()], [s8[0]], [s8[1]]), good),                                        # codes without scales
+        (([t()], [t()], [t()], [t()]), dict(good, scales=[s8[2]])),                      # scales without codes
+        (([t()], [t()], [s8[0]], [s8[1]]), dict(good, scales=[torch.zeros(2, 2, device=device)])),
+        (([t()], [t()], [t()], [t()]), dict(good, copies=[t()])),                        # a copy that is not bf16
+        (([t(), t(8, torch.bfloat16)], [t(), t(8, torch.bfloat16)], [t(), t()], [t(), t()]), good),  # two kinds
+        (([t(16)[::2]], [t()], [t()], [t()]), good),                                     # gaps
+        (([both[:8]], [both[4:]], [t()], [t()]), good),                                  # a gradient inside its parameter
+        (([both[:8], both[4:]], [t(), t()], [t(), t()], [t(), t()]), good),              # parameters that overlap
+        (([t()], [t()], [t()], [t()]), dict(good, step=0)),
+        (([t()], [t()], [t()], [t()]), dict(good, step=torch.tensor([1, 2], device=device))),
+        (([t()], [t()], [t()], [t()]), dict(good, step=torch.tensor(1.0, device=device))),
+        (([t()], [t()], [t()], [t()]), dict(good, lr=-1.0)),
+        (([t()], [t()], [t()], [t()]), dict(good, lr=float("nan"))),
+        (([t()], [t()], [t()], [t()]), dict(good, betas=(0.9, 1.0))),
+        (([t()], [t()], [t()], [t()]), dict(good, eps=-1e-8)),
+        (([t().to_sparse()], [t()], [t()], [t()]), good),
+    ]:
+        with pytest.raises(RuntimeError):
+            ops.adamw_step(*args, **more)
+    one = t()
+    with pytest.raises(RuntimeError):  # the same tensor twice
+        ops.adamw_step([one, one], [t(), t()], [t(), t()], [t(), t()], **good)
+    with pytest.raises(RuntimeError):
+        ops.adamw_read8([s8[0]], [s8[1]], [s8[2]], [t()], [t(8, torch.bfloat16)])
+    with pytest.raises(RuntimeError):
+        ops.adamw_read8([s8[0]], [s8[1]], [s8[2]], [t(9)], [t(9)])
+    with pytest.raises(RuntimeError):
+        ops.adamw_read8([s8[0]], [s8[1]], [s8[2]], [one], [one])
+
+
+def test_refusals():
+    check_refusals("cpu")
+
+
+def check_step_on_device(device):
+    """A step's number in a tensor gives what the same number of the host gives, to the bit."""
+    for bits in (32, 8):
+        got = []
+        for number in (17, torch.tensor([17], device=device)):
+            ps, gs, ms, vs = tensors([300, 77], (torch.float32, torch.float32), device)
+            more = {}
+            if bits == 8:
+                state = [ops.adamw_state8(p) for p in ps]
+                ms, vs, ss = ([s[i] for s in state] for i in range(3))
+                more = dict(scales=ss, seed=5)
+            ops.adamw_step(ps, gs, ms, vs, step=number, **HYPER, **more)
+            got.append(ps + ms + vs)
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_step_number_in_a_tensor():
+    check_step_on_device("cpu")
