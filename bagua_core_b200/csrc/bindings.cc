@@ -1052,6 +1052,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
              return p.step(gs, step_numbers(step), seed);
            },
            py::arg("groups"), py::arg("step"), py::arg("seed"))
+      .def("add_grad_buffer", &trainer::AdamWPlan::add_grad_buffer, py::arg("grad"))
       .def("zero_grad", &trainer::AdamWPlan::zero_grad, py::arg("stream"));
   m.def(
       "adamw_step",

@@ -98,10 +98,16 @@ void AdamWPlan::add(const at::Tensor& p, const at::Tensor& g, const at::Tensor& 
   a.group = group;
   segs_.push_back(a);
   if (!keep) return;
-  if (g.scalar_type() == at::kFloat) grads_.add(g);
   keep_.insert(keep_.end(), {p, g, m, v});
   if (scales) keep_.push_back(*scales);
   if (copy) keep_.push_back(*copy);
+}
+
+void AdamWPlan::add_grad_buffer(const at::Tensor& g) {
+  BAGUA_CHECK(g.scalar_type() == at::kFloat && g.is_contiguous() && (g.is_cuda() ? (int)g.device().index() : -1) == device_, Tensor,
+              "gradients are zeroed as contiguous float32 buffers on the plan's device");
+  grads_.add(g);
+  keep_.push_back(g);
 }
 
 void AdamWPlan::check_apart() const {

@@ -29,6 +29,8 @@ class AdamWPlan {
   void check_apart() const;
   // On the current stream of the tensors' device; returns the number of kernels launched.
   int step(const std::vector<adamw::GroupValues>& groups, const StepNumbers& numbers, uint64_t seed);
+  // A buffer of fp32 gradients that zero_grad() clears, whole.
+  void add_grad_buffer(const at::Tensor& g);
   void zero_grad(uint64_t stream) { grads_.zero(device_, stream); }
   // Keeps the tensors of the plan alive (a plan that lives for one call does not need it).
   bool keep = false;

@@ -42,4 +42,4 @@ from .communication import (  # noqa: F401
     init_process_group,
 )
 from .distributed import BaguaModule, with_bagua  # noqa: F401
-from .optim import FlatSGD  # noqa: F401
+from .optim import FlatAdamW, FlatSGD  # noqa: F401

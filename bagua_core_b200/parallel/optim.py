@@ -4,16 +4,18 @@ The reference contains no optimizer (it is only the communication engine); the b
 named for it train with SGD momentum 0.9, so the engine ships the obvious companion: since
 gradients already live in flat buckets, parameters and momentum are laid out the same way
 and `step()` is ONE sm_100a kernel over all buckets (read p, g, m; write p, m: 20 bytes per
-parameter, the HBM minimum) instead of torch's multi-tensor loops.
+parameter, the HBM minimum) instead of torch's multi-tensor loops.  `FlatAdamW` does the same
+for AdamW, with moments in fp32 (28 bytes per parameter) or in 8 bits (16).
 """
 from __future__ import annotations
 
 from operator import is_
-from typing import List
+from typing import List, Tuple
 
 import torch
 
 from .._native import C as _C
+from ..ops.adamw import adamw_read8, adamw_state8, adamw_step
 
 
 def _is_dense(t: torch.Tensor) -> bool:
@@ -29,29 +31,16 @@ def _is_dense(t: torch.Tensor) -> bool:
     return True
 
 
-class FlatSGD(torch.optim.Optimizer):
-    """torch.optim.SGD semantics (momentum, dampening, weight decay, Nesterov).
+class _FlatOptimizer(torch.optim.Optimizer):
+    """What optimizers on flat buckets have in common: parameters laid out as their gradients are, bf16 copies, the parameters
+    that lie outside, and the gradients' zeroing.  A subclass keeps its state in the entries of `_flat` (`_lay_out_state`) and
+    builds the native plan that steps them (`_make_plan`)."""
 
-    Before `with_bagua` attaches it (or for parameters outside any bucket) it updates
-    parameter by parameter with the same kernel.  A parameter that was laid out in a flat buffer is stepped
-    with it, in the group that it was in then, as long as the buffer lives.
-
-    `bf16_shadow=True`: for buckets of gradients (algorithms that do not communicate weights) the
-    step kernel also writes every updated parameter rounded to bf16 into a second flat buffer, and
-    each parameter gets a view of it (`bagua_core_b200.ops.shadow`); `ConvBiasReLU`,
-    `ConvBiasReLUPool` and `ShadowLinear` under bf16 autocast then read their weights from there
-    instead of casting the fp32 master weights in every forward pass.  After changing a parameter
-    by other means than this optimizer or torch's in-place ops, call `refresh_bf16()`."""
-
-    def __init__(self, params, lr: float = 1e-3, momentum: float = 0.0, dampening: float = 0.0,
-                 weight_decay: float = 0.0, nesterov: bool = False, bf16_shadow: bool = False):
-        if nesterov and (momentum <= 0 or dampening != 0):
-            raise ValueError("Nesterov momentum requires a momentum and zero dampening")
-        defaults = dict(lr=lr, momentum=momentum, dampening=dampening, weight_decay=weight_decay, nesterov=nesterov)
+    def __init__(self, params, defaults, bf16_shadow: bool):
         super().__init__(params, defaults)
         self._flat: List[dict] = []
         self._attached_ids = set()
-        self._plan = None   # the flat buffers, laid out for the native step (`_C.SgdPlan`)
+        self._plan = None   # the flat buffers, laid out for the native step
         self._loose = None  # (the groups' parameters, [(group index, parameter outside the flat buffers)])
         self._steps = 0
         self.kernel_launches = 0
@@ -102,8 +91,8 @@ class FlatSGD(torch.optim.Optimizer):
                     p.grad = flat_g[off:off + n].as_strided(tuple(p.shape), tuple(p.stride()))
                     self._attached_ids.add(id(p))
                     off += n
-                self._flat.append({"p": b.flattened, "g": flat_g, "m": torch.zeros_like(flat_g),
-                                   "runs": self._group_runs(b)})
+                self._flat.append({"p": b.flattened, "g": flat_g, "runs": self._group_runs(b)})
+                self._lay_out_state(self._flat[-1], b)
                 continue
             if b.flattened is None or any(t.kind != "grad" for t in b.tensors):
                 continue
@@ -122,7 +111,8 @@ class FlatSGD(torch.optim.Optimizer):
                     p.set_(flat_p.untyped_storage(), off, shape, stride)
                     self._attached_ids.add(id(p))
                     off += n
-            entry = {"p": flat_p, "g": b.flattened, "m": torch.zeros_like(flat_p), "runs": self._group_runs(b)}
+            entry = {"p": flat_p, "g": b.flattened, "runs": self._group_runs(b)}
+            self._lay_out_state(entry, b)
             if self.bf16_shadow:
                 from ..ops.shadow import BF16Shadow
 
@@ -136,12 +126,7 @@ class FlatSGD(torch.optim.Optimizer):
                     off += n
                 entry["h"] = flat_h
             self._flat.append(entry)
-        # one entry per run of parameters that share a parameter group (usually one per bucket), stepped with
-        # its own group's hyperparameters as they are at the time (schedulers change them in place)
-        self._plan = _C.SgdPlan() if self._flat else None
-        for f in self._flat:
-            for lo, hi, gi in f["runs"]:
-                self._plan.add(f["p"][lo:hi], f["g"][lo:hi], f["m"][lo:hi], f["h"][lo:hi] if "h" in f else None, gi)
+        self._plan = self._make_plan() if self._flat else None
 
     def _stream(self):
         return _C.current_stream(self._flat[0]["p"])
@@ -162,6 +147,65 @@ class FlatSGD(torch.optim.Optimizer):
             known = self._loose = ([list(g["params"]) for g in groups],
                                    [(gi, p) for gi, g in enumerate(groups) for p in g["params"] if id(p) not in self._attached_ids])
         return [(groups[gi], p) for gi, p in known[1]] if known[1] else ()
+
+    def _validate_shadows(self):
+        """The bf16 copies equal the parameters now: remember the parameters' versions."""
+        for p in self._shadowed:
+            p._bagua_bf16.version = p._version
+        self.shadows_valid = True
+
+    @torch.no_grad()
+    def refresh_bf16(self):
+        """Recomputes the bf16 copies from the parameters (after the weights were changed by something
+        the copies cannot notice, or to use them before the first step)."""
+        for f in self._flat:
+            if "h" in f:
+                f["h"].copy_(f["p"])
+        if self._shadowed:
+            self._validate_shadows()
+
+    def zero_grad(self, set_to_none: bool = False):
+        """Zero the flat gradient buffers in one launch; gradients stay views
+        of the bucket (never set to None, which would detach them from the bucket)."""
+        if self._plan is not None:
+            self._plan.zero_grad(self._stream())
+        for _, p in self._loose_params():
+            if p.grad is not None:
+                p.grad.zero_()
+
+
+class FlatSGD(_FlatOptimizer):
+    """torch.optim.SGD semantics (momentum, dampening, weight decay, Nesterov).
+
+    Before `with_bagua` attaches it (or for parameters outside any bucket) it updates
+    parameter by parameter with the same kernel.  A parameter that was laid out in a flat buffer is stepped
+    with it, in the group that it was in then, as long as the buffer lives.
+
+    `bf16_shadow=True`: for buckets of gradients (algorithms that do not communicate weights) the
+    step kernel also writes every updated parameter rounded to bf16 into a second flat buffer, and
+    each parameter gets a view of it (`bagua_core_b200.ops.shadow`); `ConvBiasReLU`,
+    `ConvBiasReLUPool` and `ShadowLinear` under bf16 autocast then read their weights from there
+    instead of casting the fp32 master weights in every forward pass.  After changing a parameter
+    by other means than this optimizer or torch's in-place ops, call `refresh_bf16()`."""
+
+    def __init__(self, params, lr: float = 1e-3, momentum: float = 0.0, dampening: float = 0.0,
+                 weight_decay: float = 0.0, nesterov: bool = False, bf16_shadow: bool = False):
+        if nesterov and (momentum <= 0 or dampening != 0):
+            raise ValueError("Nesterov momentum requires a momentum and zero dampening")
+        defaults = dict(lr=lr, momentum=momentum, dampening=dampening, weight_decay=weight_decay, nesterov=nesterov)
+        super().__init__(params, defaults, bf16_shadow)
+
+    def _lay_out_state(self, entry, bucket):
+        entry["m"] = torch.zeros_like(entry["p"])
+
+    def _make_plan(self):
+        # one entry per run of parameters that share a parameter group (usually one per bucket), stepped with
+        # its own group's hyperparameters as they are at the time (schedulers change them in place)
+        plan = _C.SgdPlan()
+        for f in self._flat:
+            for lo, hi, gi in f["runs"]:
+                plan.add(f["p"][lo:hi], f["g"][lo:hi], f["m"][lo:hi], f["h"][lo:hi] if "h" in f else None, gi)
+        return plan
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -205,27 +249,191 @@ class FlatSGD(torch.optim.Optimizer):
         self._steps += 1
         return loss
 
-    def _validate_shadows(self):
-        """The bf16 copies equal the parameters now: remember the parameters' versions."""
-        for p in self._shadowed:
-            p._bagua_bf16.version = p._version
-        self.shadows_valid = True
+
+class FlatAdamW(_FlatOptimizer):
+    """torch.optim.AdamW semantics: Adam whose weight decay is taken from the weights, not through the gradient.
+
+    Laid out by `with_bagua` as `FlatSGD` is: one kernel steps all buckets, and with `bf16_shadow=True` also writes the bf16
+    copies of the weights.  Parameters outside any bucket are stepped as lists, a launch for each kind of them, and may be
+    float32, float16 or bfloat16.  Each parameter counts its own steps.
+
+    `state_bits=8`: the moments are held in 8 bits (`bagua_core_b200.ops.adamw`), 2 bytes per parameter instead of 8;
+    `seed` is that of their rounding, the same on all ranks.  `moments(p)` reads a parameter's moments.
+
+    The state of a parameter (`state[p]`, `state_dict()`, `load_state_dict()`) is `step` with `exp_avg` and `exp_avg_sq`, to which
+    8 bits add `scales`; it goes along when a bucket is laid out (again).  A step cannot be captured into a CUDA graph,
+    since its number is counted on the host; `bagua_core_b200.ops.adamw_step` takes one that lies on the device."""
+
+    def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, bf16_shadow: bool = False, state_bits: int = 32, seed: int = 0):
+        if lr < 0 or eps < 0 or weight_decay < 0 or not all(0 <= b < 1 for b in betas):
+            raise ValueError("AdamW needs lr, eps and weight_decay of 0 or more and betas from 0 to below 1")
+        if state_bits not in (8, 32):
+            raise ValueError("moments are held in 8 or 32 bits")
+        if not 0 <= seed < 1 << 64:
+            raise ValueError("the seed is a number of 64 bits")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay), bf16_shadow)
+        self.state_bits = state_bits
+        self.seed = seed
+        self._plan_groups: List[List[int]] = []  # [parameter group, steps done] of each group of the plan
+        self._plan_group_of = {}                 # id(parameter in the flat buffers) -> index of its group there
+        self._plan_tensors = 0
+
+    # ---- state -----------------------------------------------------------------------
+    def _new_state(self, p):
+        if self.state_bits == 8:
+            m, v, scales = adamw_state8(p)
+            return {"step": 0, "exp_avg": m, "exp_avg_sq": v, "scales": scales}
+        m, v = (torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format, requires_grad=False) for _ in range(2))
+        return {"step": 0, "exp_avg": m, "exp_avg_sq": v}
+
+    def bagua_attach(self, bm):
+        self._sync_steps()
+        super().bagua_attach(bm)
 
     @torch.no_grad()
-    def refresh_bf16(self):
-        """Recomputes the bf16 copies from the parameters (after the weights were changed by something
-        the copies cannot notice, or to use them before the first step)."""
-        for f in self._flat:
-            if "h" in f:
-                f["h"].copy_(f["p"])
-        if self._shadowed:
-            self._validate_shadows()
+    def _lay_out_state(self, entry, bucket):
+        # a flat buffer for each moment; in 8 bits with scales for each parameter, whose blocks end where it ends
+        dtype = torch.uint8 if self.state_bits == 8 else torch.float32
+        flat = {k: torch.zeros_like(entry["p"], dtype=dtype) for k in ("exp_avg", "exp_avg_sq")}
+        off = 0
+        entry["owners"] = []
+        for t in bucket.tensors:
+            p, n = t.owner, t.owner.numel()
+            state = {"step": 0, **{k: f[off:off + n].as_strided(tuple(p.shape), tuple(p.stride())) for k, f in flat.items()}}
+            if self.state_bits == 8:
+                state["scales"] = torch.zeros(2, (n + _C.moment8_block - 1) // _C.moment8_block, device=p.device)
+            if p in self.state and "step" in self.state[p]:  # steps taken before, here or in another layout
+                self._copy_state(state, self.state[p])
+            self.state[p] = state
+            entry["owners"].append((p, off, off + n))
+            off += n
+        entry["m"], entry["v"] = flat["exp_avg"], flat["exp_avg_sq"]
 
-    def zero_grad(self, set_to_none: bool = False):
-        """Zero the flat gradient buffers in one launch; gradients stay views
-        of the bucket (never set to None, which would detach them from the bucket)."""
+    def _make_plan(self):
+        plan = _C.AdamWPlan()
+        self._plan_groups, self._plan_group_of, self._plan_tensors = [], {}, 0
+        known = {}
+        group_of = {id(p): gi for gi, g in enumerate(self.param_groups) for p in g["params"]}
+
+        def plan_group(gi, step):
+            if (gi, step) not in known:
+                known[gi, step] = len(self._plan_groups)
+                self._plan_groups.append([gi, step])
+            return known[gi, step]
+
+        for f in self._flat:
+            flats = [f["p"], f["g"], f["m"], f["v"]]
+            pieces = []  # [from, to, group in the plan, scales]
+            for p, lo, hi in f["owners"]:
+                state = self.state[p]
+                k = self._plan_group_of[id(p)] = plan_group(group_of[id(p)], state["step"])
+                if self.state_bits == 32 and pieces and pieces[-1][2] == k:
+                    pieces[-1][1] = hi  # a run of parameters that are stepped alike is one piece
+                else:
+                    pieces.append([lo, hi, k, state.get("scales")])
+            for lo, hi, k, scales in pieces:
+                plan.add(*(x[lo:hi] for x in flats), scales, f["h"][lo:hi] if "h" in f else None, k)
+            self._plan_tensors += len(pieces)
+            plan.add_grad_buffer(f["g"])
+        return plan
+
+    def _sync_steps(self):
+        """The steps that the plan has counted, into the parameters' state."""
+        for f in self._flat:
+            for p, _, _ in f["owners"]:
+                if p in self.state:
+                    self.state[p]["step"] = self._plan_groups[self._plan_group_of[id(p)]][1]
+
+    def _copy_state(self, to, saved):
+        names = set(to)
+        if set(saved) != names or any(saved[k].shape != to[k].shape for k in names - {"step"}):
+            raise ValueError(f"the saved state of a parameter is not that of moments in {self.state_bits} bits of its size")
+        for k in names - {"step"}:
+            if saved[k].dtype != to[k].dtype:
+                raise ValueError(f"the saved moments are {saved[k].dtype}, not {to[k].dtype}")
+            to[k].copy_(saved[k])
+        to["step"] = int(saved["step"])
+
+    def state_dict(self):
+        self._sync_steps()
+        return super().state_dict()
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        # (torch's own would cast the codes of 8-bit moments to the parameters' type)
+        held, saved = dict(self.state), state_dict["state"]
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+            state = held[p] if id(p) in self._attached_ids else self._new_state(p)
+            if i in saved:
+                self._copy_state(state, saved[i])
+            elif id(p) in self._attached_ids:
+                self._copy_state(state, self._new_state(p))
+            else:
+                continue  # made by its first step
+            self.state[p] = state
+        if self._flat:
+            self._plan = self._make_plan()
+
+    def moments(self, p) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(first, second) moment of a parameter that was stepped or laid out, in fp32."""
+        s = self.state[p]
+        if self.state_bits == 32:
+            return s["exp_avg"].clone(), s["exp_avg_sq"].clone()
+        m, v = (torch.empty_like(s["exp_avg"], dtype=torch.float32) for _ in range(2))
+        adamw_read8([s["exp_avg"]], [s["exp_avg_sq"]], [s["scales"]], [m], [v])
+        return m, v
+
+    # ---- stepping --------------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
         if self._plan is not None:
-            self._plan.zero_grad(self._stream())
-        for _, p in self._loose_params():
-            if p.grad is not None:
-                p.grad.zero_()
+            values = []
+            for gi, done in self._plan_groups:
+                g = self.param_groups[gi]
+                values.append((g["lr"], *g["betas"], g["eps"], g["weight_decay"]))
+            self.kernel_launches += self._plan.step(values, [done + 1 for _, done in self._plan_groups], self.seed)
+            for group in self._plan_groups:
+                group[1] += 1
+        if self._shadowed and not self.shadows_valid:
+            self._validate_shadows()
+        self._step_loose()
+        self._steps += 1
+        return loss
+
+    def _step_loose(self):
+        kinds, back = {}, []  # one call for each kind of parameters
+        for group, p in self._loose_params():
+            if p.grad is None:
+                continue
+            if p not in self.state or "step" not in self.state[p]:
+                self.state[p] = self._new_state(p)
+            state, g, w = self.state[p], p.grad, p
+            if not _is_dense(p):
+                w = p.contiguous()
+                back.append((p, w))
+            m = state["exp_avg"]
+            if m.stride() != w.stride():  # the parameter has been laid out anew since
+                for k in ("exp_avg", "exp_avg_sq"):
+                    state[k] = torch.empty_like(w, dtype=m.dtype).copy_(state[k])
+            if g.layout == torch.strided and g.stride() != w.stride():
+                g = torch.empty_like(w, dtype=g.dtype).copy_(g)
+            key = (id(group), state["step"], p.device, p.dtype, g.dtype)
+            kinds.setdefault(key, (group, []))[1].append((w, g, state))
+        first = self._plan_tensors
+        for (_, done, *_), (group, parts) in kinds.items():
+            self.kernel_launches += adamw_step(
+                [w for w, _, _ in parts], [g for _, g, _ in parts], [s["exp_avg"] for _, _, s in parts], [s["exp_avg_sq"] for _, _, s in parts],
+                step=done + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                scales=[s["scales"] for _, _, s in parts] if self.state_bits == 8 else None, seed=self.seed, first_index=first)
+            first += len(parts)
+            for _, _, s in parts:
+                s["step"] += 1
+        for p, w in back:
+            p.copy_(w)

@@ -26,6 +26,8 @@ def main():
     ap.add_argument("--algorithm", default="gradient_allreduce",
                     choices=["gradient_allreduce", "bytegrad", "decentralized", "shift_one", "low_precision", "qadam",
                              "async"])
+    ap.add_argument("--optimizer", default="sgd", choices=["sgd", "adamw", "adamw8"],
+                    help="adamw8: AdamW with its moments in 8 bits (qadam brings an optimizer of its own)")
     ap.add_argument("--steps", type=int, default=10)
     ap.add_argument("--batch", type=int, default=8)
     args = ap.parse_args()
@@ -44,7 +46,10 @@ def main():
         opt = P.QAdamOptimizer(model.parameters(), lr=1e-3, warmup_steps=max(1, args.steps // 2))
         algo = P.QAdamAlgorithm(opt)
     else:
-        opt = P.FlatSGD(model.parameters(), lr=0.01, momentum=0.9)
+        if args.optimizer == "sgd":
+            opt = P.FlatSGD(model.parameters(), lr=0.01, momentum=0.9)
+        else:
+            opt = P.FlatAdamW(model.parameters(), lr=1e-3, state_bits=8 if args.optimizer == "adamw8" else 32)
         algo = {
             "gradient_allreduce": P.GradientAllReduceAlgorithm,
             "bytegrad": P.ByteGradAlgorithm,

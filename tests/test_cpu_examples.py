@@ -36,3 +36,8 @@ def test_host_overhead_benchmark_runs_and_a_ready_mark_stays_cheap():
     row = json.loads(out.strip().splitlines()[-1])
     assert set(row) >= {"mark_us", "bucket_us", "wrapper_us"}
     assert 0 < row["mark_us"] < 5.0, row
+
+
+def test_training_example_runs_with_adamw_and_8_bit_moments():
+    out = _run("examples/train_synthetic.py", "--model", "mlp", "--optimizer", "adamw8", "--steps", "4")
+    assert "step 3: loss" in out
