@@ -59,6 +59,7 @@ SOURCES = [
     "kernels/conv_wgrad.cu",
     "kernels/model_ops_cpu.cc",
     "kernels/encoder_ops.cu",
+    "kernels/embedding.cu",
     "kernels/adamw.cu",
     "kernels/adamw_host.cc",
 ]

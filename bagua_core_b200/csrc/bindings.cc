@@ -13,6 +13,7 @@
 #include <pybind11/stl.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/extension.h>
 
@@ -998,6 +999,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embed_layer_norm", &trainer::embed_layer_norm, py::arg("ids"), py::arg("tokens"), py::arg("positions"),
         py::arg("types"), py::arg("weight"), py::arg("bias"), py::arg("eps"), py::arg("accumulate"),
         "layer_norm(tokens[ids] + positions[:seq] + types[0]) in bf16.");
+  m.def("embedding", [](const at::Tensor& ids, const at::Tensor& table, double scale, int64_t padding, const py::object& type, bool accumulate) {
+          std::optional<at::ScalarType> to;
+          if (!type.is_none()) {
+            TORCH_CHECK(THPDtype_Check(type.ptr()), "dtype must be a torch.dtype");
+            to = reinterpret_cast<THPDtype*>(type.ptr())->scalar_type;
+          }
+          return trainer::embedding(ids, table, scale, padding, to, accumulate);
+        }, py::arg("ids"), py::arg("table"), py::arg("scale"), py::arg("padding"), py::arg("dtype"), py::arg("accumulate"),
+        "scale * table[ids], with the gradient by sorted tokens.");
   m.attr("max_embedding_tokens") = encoder_ops::kMaxTokens;
   m.def("attention", &trainer::attention, py::arg("qkv"), py::arg("heads"), py::arg("dropout"),
         "Multi-head attention of a packed bf16 projection (the attention kernel is the library's).");

@@ -1,0 +1,511 @@
+// See embedding.h.
+#include <cooperative_groups.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "embedding.h"
+#include "index_report.cuh"
+#include "launch.cuh"
+#include "typed_vec.cuh"
+
+namespace bagua {
+namespace embedding {
+
+namespace {
+
+namespace cg = cooperative_groups;
+using namespace kernels;
+using encoder_ops::IndexReport;
+using encoder_ops::report_index;
+
+constexpr int kThreads = 256;
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ---- lookup -------------------------------------------------------------------------------------
+// A thread takes eight columns of a row, or, where rows do not lie on 16 bytes, one.
+template <typename Id, typename W, typename O, bool kVec>
+__global__ void __launch_bounds__(kThreads)
+    lookup_kernel(const Id* __restrict__ ids, const W* __restrict__ table, int64_t rows, int64_t row_stride, O* __restrict__ out, int64_t n,
+                  int64_t H, int columns, float scale, IndexReport* report) {
+  wait_for_predecessor();
+  const int per = kThreads / columns;  // rows of a block
+  const int64_t t = (int64_t)blockIdx.x * per + threadIdx.x / columns;
+  const int64_t c = ((int64_t)blockIdx.y * columns + threadIdx.x % columns) * (kVec ? 8 : 1);
+  if (t >= n || c >= H) return;
+  const int64_t id = (int64_t)ids[t];
+  const bool known = id >= 0 && id < rows;
+  if (!known && c == 0) report_index(report, encoder_ops::kTokenId, id);
+  if constexpr (kVec) {
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = nanf("");
+    if (known) {
+      widen8(load8(table + id * row_stride + c), f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] *= scale;
+    }
+    store8(out + t * H + c, narrow8<O>(f));
+  } else {
+    out[t * H + c] = from_float<O>(known ? to_float(table[id * row_stride + c]) * scale : nanf(""));
+  }
+}
+
+// ---- sorting ------------------------------------------------------------------------------------
+// A token's key is its row, or `rows` for those without a part in the gradient, which so come last.  Stable, least significant digit
+// first: a pass puts the tokens in the order of 8 bits and leaves equal ones as they were.
+constexpr int kDigits = 256;
+struct Keys {
+  int64_t rows, padding;
+  template <typename Id>
+  __device__ __forceinline__ uint32_t operator()(Id id) const {
+    const int64_t v = (int64_t)id;
+    return (uint32_t)(v >= 0 && v < rows && v != padding ? v : rows);
+  }
+};
+
+// Number of a lane's key among the equal digits of its warp's keys so far, which `seen` counts.  All lanes of the warp come here.
+__device__ __forceinline__ uint32_t rank_in_warp(uint32_t* seen, uint32_t digit, bool valid) {
+  const uint32_t peers = __match_any_sync(0xffffffffu, valid ? digit : (uint32_t)kDigits);
+  const int lane = (int)threadIdx.x & 31;
+  const uint32_t before = valid ? seen[digit] : 0u;
+  __syncwarp();
+  if (valid && (peers >> lane) == 1u) seen[digit] = before + __popc(peers);  // the last of them
+  __syncwarp();
+  return before + __popc(peers & ((1u << lane) - 1u));
+}
+
+// Sorting in blocks that hand tiles to each other through memory.
+constexpr int kRounds = 8, kTile = kThreads * kRounds, kWarps = kThreads / 32;
+// counts[digit][tile]; `present`: a bit for each row that occurs (first pass only).
+template <typename Id>
+__global__ void __launch_bounds__(kThreads)
+    histogram_kernel(const Id* __restrict__ ids, const uint32_t* __restrict__ keys, Keys key, int64_t n, int shift, uint32_t* __restrict__ counts,
+                     int tiles, uint32_t* __restrict__ present) {
+  __shared__ uint32_t s_count[kDigits];
+  wait_for_predecessor();
+  s_count[threadIdx.x] = 0;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kTile;
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = base + r * kThreads + threadIdx.x;
+    if (i >= n) break;
+    const uint32_t k = keys ? keys[i] : key(ids[i]);
+    atomicAdd(&s_count[(k >> shift) & (kDigits - 1)], 1u);
+    if (present && k < key.rows) atomicOr(&present[k / 32], 1u << (k % 32));
+  }
+  __syncthreads();
+  counts[(int64_t)threadIdx.x * tiles + blockIdx.x] = s_count[threadIdx.x];
+}
+constexpr int kScanThreads = 1024;
+// Exclusive sums of n counts, in one block.
+__global__ void __launch_bounds__(kScanThreads) scan_kernel(uint32_t* __restrict__ counts, int64_t n) {
+  __shared__ uint32_t s_warp[32];
+  __shared__ uint32_t s_total;
+  wait_for_predecessor();
+  const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
+  uint32_t carry = 0;
+  for (int64_t base = 0; base < n; base += kScanThreads * 4) {
+    const int64_t i = base + (int64_t)threadIdx.x * 4;
+    uint32_t v[4], sum = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = i + k < n ? counts[i + k] : 0u;
+      sum += v[k];
+    }
+    uint32_t up = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += x;
+    }
+    if (lane == 31) s_warp[warp] = up;
+    __syncthreads();
+    if (warp == 0) {
+      uint32_t w = s_warp[lane], wu = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, wu, o);
+        if (lane >= o) wu += x;
+      }
+      s_warp[lane] = wu - w;
+      if (lane == 31) s_total = wu;
+    }
+    __syncthreads();
+    uint32_t at = carry + s_warp[warp] + up - sum;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (i + k < n) counts[i + k] = at;
+      at += v[k];
+    }
+    carry += s_total;
+    __syncthreads();
+  }
+}
+template <typename Id>
+__global__ void __launch_bounds__(kThreads)
+    scatter_kernel(const Id* __restrict__ ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ places, Keys key, int64_t n,
+                   int shift, const uint32_t* __restrict__ offsets, int tiles, uint32_t* __restrict__ keys_out,
+                   uint32_t* __restrict__ places_out) {
+  __shared__ uint32_t s_seen[kWarps][kDigits];
+  wait_for_predecessor();
+  const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
+  for (int k = (int)threadIdx.x; k < kWarps * kDigits; k += kThreads) s_seen[0][k] = 0;
+  __syncthreads();
+  // a warp's keys are neighbours
+  const int64_t base = (int64_t)blockIdx.x * kTile + warp * (kTile / kWarps) + lane;
+  uint32_t k[kRounds], p[kRounds], rank[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = base + r * 32;
+    const bool valid = i < n;
+    k[r] = !valid ? 0u : keys ? keys[i] : key(ids[i]);
+    p[r] = !valid ? 0u : places ? places[i] : (uint32_t)i;
+    rank[r] = rank_in_warp(s_seen[warp], (k[r] >> shift) & (kDigits - 1), valid);
+  }
+  __syncthreads();
+  {
+    uint32_t at = offsets[(int64_t)threadIdx.x * tiles + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const uint32_t c = s_seen[w][threadIdx.x];
+      s_seen[w][threadIdx.x] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    if (base + r * 32 >= n) break;
+    const uint32_t to = s_seen[warp][(k[r] >> shift) & (kDigits - 1)] + rank[r];
+    keys_out[to] = k[r];
+    places_out[to] = p[r];
+  }
+}
+
+// ---- sums ---------------------------------------------------------------------------------------
+// The sorted tokens are cut into chunks of equal length.  A group of lanes takes a chunk and 8 columns a lane, adds up the rows of
+// equal tokens in their order and writes each sum to its row of the table.  Sums over a border between chunks go to scratch, two rows
+// a chunk (of the run that comes in, of the run that goes out), and join_kernel adds those up in the chunks' order.  In the same
+// launch, further warps clear the rows that do not occur.
+struct SumArgs {
+  const uint32_t *keys, *places;
+  const uint32_t* present;  // null: rows that do not occur are left alone
+  float* partial;
+  int64_t n, rows, H, chunks, sum_blocks;
+  int length;   // of a chunk, a multiple of 32
+  int slices;   // of a row's columns
+  float scale;
+};
+
+// The column of element k of a lane that stands at `lane` in a slice of `width` lanes.
+template <bool kVec>
+__device__ __forceinline__ int64_t column(int slice, int lane, int width, int k) {
+  return (int64_t)slice * width * 8 + (kVec ? lane * 8 + k : k * width + lane);
+}
+template <typename T, bool kVec>
+__device__ __forceinline__ Raw8<T> load_row(const T* row, int slice, int lane, int width, int64_t H) {
+  if constexpr (kVec) {
+    const int64_t c = column<true>(slice, lane, width, 0);
+    if (c < H) return load8(row + c);
+    return Raw8<T>{};
+  } else {
+    Raw8<T> r{};
+    T* x = reinterpret_cast<T*>(&r);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t c = column<false>(slice, lane, width, k);
+      if (c < H) x[k] = row[c];
+    }
+    return r;
+  }
+}
+template <typename T, bool kVec>
+__device__ __forceinline__ void store_row(T* row, const float (&f)[8], int slice, int lane, int width, int64_t H) {
+  if constexpr (kVec) {
+    const int64_t c = column<true>(slice, lane, width, 0);
+    if (c < H) store8(row + c, narrow8<T>(f));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t c = column<false>(slice, lane, width, k);
+      if (c < H) row[c] = from_float<T>(f[k]);
+    }
+  }
+}
+template <typename T, bool kVec>
+__device__ __forceinline__ void finish_row(T* row, float (&f)[8], float scale, bool accumulate, int slice, int lane, int width, int64_t H) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] *= scale;
+  if (accumulate) {
+    float old[8];
+    widen8(load_row<T, kVec>(row, slice, lane, width, H), old);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] += old[k];
+  }
+  store_row<T, kVec>(row, f, slice, lane, width, H);
+}
+
+template <typename D, typename W, bool kVec, int kWidth>
+__global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ SumArgs a, const D* __restrict__ dout, W* __restrict__ dtable) {
+  wait_for_predecessor();
+  const int warp_lane = (int)threadIdx.x & 31;
+  if (blockIdx.x >= a.sum_blocks) {  // rows that do not occur, 32 to a warp
+    const int64_t unit = (int64_t)(blockIdx.x - a.sum_blocks) * (kThreads / 32) + (threadIdx.x >> 5);
+    const int64_t word = unit / a.slices;
+    const int slice = (int)(unit % a.slices);
+    if (word * 32 >= a.rows) return;
+    const int64_t left = a.rows - word * 32;
+    uint32_t absent = ~a.present[word] & (left >= 32 ? 0xffffffffu : (1u << left) - 1u);
+    constexpr int groups = 32 / kWidth;
+    const int lane = warp_lane % kWidth, group = warp_lane / kWidth;
+    const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int r = group; r < 32; r += groups)
+      if (absent >> r & 1u) store_row<W, kVec>(dtable + (word * 32 + r) * a.H, zero, slice, lane, kWidth, a.H);
+    return;
+  }
+  const int64_t unit = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kWidth;
+  const int lane = warp_lane % kWidth;
+  const int64_t chunk = unit / a.slices;
+  const int slice = (int)(unit % a.slices);
+  const bool on = chunk < a.chunks;
+  const int64_t lo = on ? chunk * a.length : 0, hi = on ? min(lo + a.length, a.n) : 0;
+  const uint32_t none = (uint32_t)a.rows;
+  // what lies on the two borders
+  const uint32_t before = lo > 0 ? a.keys[lo - 1] : none, behind = hi < a.n ? a.keys[hi] : none;
+  float acc[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+  uint32_t run = none;  // whose sum `acc` is
+  bool first = true;    // it is the chunk's first run
+  auto flush = [&](bool last) {
+    if (run == none) return;
+    const bool in = first && run == before, out = last && run == behind;
+    if (in || out)
+      store_row<float, kVec>(a.partial + (2 * chunk + (in ? 0 : 1)) * a.H, acc, slice, lane, kWidth, a.H);
+    else
+      finish_row<W, kVec>(dtable + (int64_t)run * a.H, acc, a.scale, a.present == nullptr, slice, lane, kWidth, a.H);
+  };
+  constexpr int kAhead = 8 / (sizeof(D) / 2) < 4 ? 4 : 8 / (sizeof(D) / 2);  // rows on their way
+  for (int64_t base = lo; __any_sync(0xffffffffu, base < hi); base += kWidth) {
+    // tokens of this turn, one a lane
+    const int64_t mine = base + lane;
+    const uint32_t key = mine < hi ? a.keys[mine] : none;
+    const uint32_t place = mine < hi ? a.places[mine] : 0u;
+    if (!__any_sync(0xffffffffu, key != none)) break;  // the rest has no part
+#pragma unroll 1
+    for (int j0 = 0; j0 < kWidth; j0 += kAhead) {
+      Raw8<D> row[kAhead];
+      uint32_t id[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        id[j] = __shfl_sync(0xffffffffu, key, j0 + j, kWidth);
+        const uint32_t p = __shfl_sync(0xffffffffu, place, j0 + j, kWidth);
+        if (id[j] != none) row[j] = load_row<D, kVec>(dout + (int64_t)p * a.H, slice, lane, kWidth, a.H);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (id[j] == none) continue;
+        if (id[j] != run) {
+          if (run != none) {
+            flush(false);
+            first = false;
+          }
+          run = id[j];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+        }
+        float f[8];
+        widen8(row[j], f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += f[k];
+      }
+      __syncwarp();
+    }
+  }
+  flush(true);
+}
+
+// Sums over borders: a block takes a run that leaves its first chunk, and 128 columns; its 8 rows of threads add up every eighth chunk's
+// part each.
+constexpr int kJoinColumns = 32, kJoinRows = kThreads / kJoinColumns;
+template <typename W>
+__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ SumArgs a, W* __restrict__ dtable) {
+  __shared__ float s_acc[kJoinRows][kJoinColumns * 4];
+  wait_for_predecessor();
+  const int64_t chunk = blockIdx.x, lo = chunk * a.length, hi = lo + a.length;  // hi < n: the last chunk is not among these
+  const uint32_t none = (uint32_t)a.rows, run = a.keys[hi - 1];
+  if (run == none || a.keys[hi] != run || (lo > 0 && a.keys[lo - 1] == run && a.keys[lo] == run)) return;
+  // the run's last chunk: a search for the end of its keys
+  int64_t below = hi, above = a.n;  // keys[below] == run, keys[above] != run
+  while (above - below > 1) {
+    const int64_t mid = (below + above) / 2;
+    if (a.keys[mid] == run)
+      below = mid;
+    else
+      above = mid;
+  }
+  const int64_t last = below / a.length;
+  const int tx = (int)threadIdx.x % kJoinColumns, ty = (int)threadIdx.x / kJoinColumns;
+  const int64_t c0 = (int64_t)blockIdx.y * kJoinColumns * 4 + tx;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int64_t k = chunk + ty; k <= last; k += kJoinRows) {
+    const float* row = a.partial + (2 * k + (k == chunk ? 1 : 0)) * a.H;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c0 + e * kJoinColumns < a.H) acc[e] += row[c0 + e * kJoinColumns];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s_acc[ty][e * kJoinColumns + tx] = acc[e];
+  __syncthreads();
+  if (threadIdx.x >= kJoinColumns * 4) return;
+  const int64_t c = (int64_t)blockIdx.y * kJoinColumns * 4 + threadIdx.x;
+  if (c >= a.H) return;
+  float s = 0.f;
+#pragma unroll
+  for (int r = 0; r < kJoinRows; ++r) s += s_acc[r][threadIdx.x];
+  W* out = dtable + (int64_t)run * a.H + c;
+  s *= a.scale;
+  *out = from_float<W>(a.present ? s : s + to_float(*out));
+}
+
+// ---- plans --------------------------------------------------------------------------------------
+struct Plan {
+  int64_t tiles, chunks, sum_blocks;
+  int length, slices, width;
+  size_t keys, counts, present, partial, bytes;  // offsets into the scratch
+};
+Plan plan(int64_t n, int64_t rows, int64_t H) {
+  Plan p{};
+  auto take = [&p](size_t bytes) {
+    const size_t at = p.bytes;
+    p.bytes += align_up(bytes, 256);
+    return at;
+  };
+  p.tiles = ceil_div(n, kTile);
+  p.width = H > 128 ? 32 : H > 64 ? 16 : 8;
+  p.slices = (int)ceil_div(H, p.width * 8);
+  // As many chunks as keep every SM's warps busy, as long as a chunk's two rows of scratch are few next to its own.
+  const int64_t lanes = (int64_t)148 * 1024, units = std::max<int64_t>(1, lanes / p.width / p.slices);
+  p.length = (int)std::min<int64_t>(1024, std::max<int64_t>(32, ceil_div(ceil_div(n, units), 32) * 32));
+  p.chunks = ceil_div(n, p.length);
+  p.sum_blocks = ceil_div(p.chunks * p.slices * p.width, kThreads);
+  p.keys = take((size_t)n * 4 * 4);
+  p.counts = take((size_t)p.tiles * kDigits * 4);
+  p.present = take((size_t)ceil_div(rows, 32) * 4);
+  p.partial = take((size_t)p.chunks * 2 * H * 4);
+  return p;
+}
+
+template <typename Id>
+int sort(const Ids& ids, Keys key, const Plan& p, uint32_t* buffers, uint32_t* counts, uint32_t* present, const uint32_t** keys,
+         const uint32_t** places, cudaStream_t s) {
+  const int64_t n = ids.n;
+  int bits = 1;
+  while (bits < 32 && (key.rows >> bits) != 0) ++bits;
+  uint32_t* k[2] = {buffers, buffers + 2 * n};
+  const uint32_t *in_k = nullptr, *in_p = nullptr;
+  int launches = 0, to = 0;
+  for (int shift = 0; shift < bits; shift += 8, to ^= 1) {
+    launch_overlapped(histogram_kernel<Id>, dim3((unsigned)p.tiles), dim3(kThreads), s, (const Id*)ids.data, in_k, key, n, shift, counts,
+                      (int)p.tiles, shift == 0 ? present : nullptr);
+    launch_overlapped(scan_kernel, dim3(1), dim3(kScanThreads), s, counts, p.tiles * kDigits);
+    launch_overlapped(scatter_kernel<Id>, dim3((unsigned)p.tiles), dim3(kThreads), s, (const Id*)ids.data, in_k, in_p, key, n, shift, counts,
+                      (int)p.tiles, k[to], k[to] + n);
+    in_k = k[to];
+    in_p = k[to] + n;
+    launches += 3;
+  }
+  *keys = in_k;
+  *places = in_p;
+  return launches;
+}
+
+template <typename D, typename W>
+void sums(const SumArgs& a, const Plan& p, const void* dout, void* dtable, cudaStream_t s) {
+  const bool vec = a.H % 8 == 0 && ((uintptr_t)dout | (uintptr_t)dtable) % 16 == 0;
+  const int64_t clear = a.present ? ceil_div(ceil_div(a.rows, 32) * a.slices, kThreads / 32) : 0;
+  const dim3 grid((unsigned)(a.sum_blocks + clear));
+  auto go = [&](auto kernel) { launch_overlapped(kernel, grid, dim3(kThreads), s, a, (const D*)dout, (W*)dtable); };
+  if (vec)
+    p.width == 32 ? go(sum_kernel<D, W, true, 32>) : p.width == 16 ? go(sum_kernel<D, W, true, 16>) : go(sum_kernel<D, W, true, 8>);
+  else
+    p.width == 32 ? go(sum_kernel<D, W, false, 32>) : p.width == 16 ? go(sum_kernel<D, W, false, 16>) : go(sum_kernel<D, W, false, 8>);
+  if (a.chunks > 1)
+    launch_overlapped(join_kernel<W>, dim3((unsigned)(a.chunks - 1), (unsigned)ceil_div(a.H, kJoinColumns * 4)), dim3(kThreads), s, a, (W*)dtable);
+}
+
+template <typename F>
+void typed(DType t, F&& f) {
+  switch (t) {
+    case DType::F32: f((float*)nullptr); return;
+    case DType::F16: f((__half*)nullptr); return;
+    case DType::BF16: f((__nv_bfloat16*)nullptr); return;
+    default: throw BaguaError(ErrorKind::Tensor, std::string("embedding: unsupported type ") + dtype_name(t));
+  }
+}
+
+}  // namespace
+
+void lookup(const Ids& ids, const void* table, DType table_type, int64_t rows, int64_t row_stride, int64_t H, float scale, void* out,
+            DType out_type, cudaStream_t s) {
+  BAGUA_CHECK(ids.n > 0 && ids.n <= kMaxTokens && H > 0, Tensor, "embedding: " << ids.n << " tokens of " << H << " columns");
+  typed(table_type, [&](auto* w) {
+    using W = std::remove_pointer_t<decltype(w)>;
+    typed(out_type, [&](auto* o) {
+      using O = std::remove_pointer_t<decltype(o)>;
+      auto go = [&](auto* id) {
+        using Id = std::remove_pointer_t<decltype(id)>;
+        const bool vec = H % 8 == 0 && ((uintptr_t)table | (uintptr_t)out | (uintptr_t)(row_stride * (int64_t)sizeof(W))) % 16 == 0;
+        const int64_t wide = ceil_div(H, vec ? 8 : 1);
+        int columns = 1;
+        while (columns < kThreads && columns < wide) columns *= 2;
+        const int64_t slices = ceil_div(wide, columns);
+        BAGUA_CHECK(slices < 65536, Tensor, "embedding: " << H << " columns");
+        const dim3 grid((unsigned)ceil_div(ids.n, kThreads / columns), (unsigned)slices);
+        launch_overlapped(vec ? lookup_kernel<Id, W, O, true> : lookup_kernel<Id, W, O, false>, grid, dim3(kThreads), s, (const Id*)ids.data,
+                          (const W*)table, rows, row_stride, (O*)out, ids.n, H, columns, scale, encoder_ops::index_report());
+      };
+      ids.wide ? go((int64_t*)nullptr) : go((int32_t*)nullptr);
+    });
+  });
+}
+
+size_t backward_scratch_bytes(int64_t n, int64_t rows, int64_t H) { return plan(n, rows, H).bytes; }
+
+int backward(const Ids& ids, const void* dout, DType dout_type, int64_t rows, int64_t H, float scale, int64_t padding, void* dtable,
+             DType table_type, bool accumulate, void* scratch, cudaStream_t s) {
+  BAGUA_CHECK(ids.n > 0 && ids.n <= kMaxTokens && rows > 0 && rows <= kMaxRows && H > 0, Tensor,
+              "embedding backward: " << ids.n << " tokens, " << rows << " rows of " << H << " columns");
+  BAGUA_CHECK(!accumulate || table_type == DType::F32, Tensor, "embedding gradients are added to in float32");
+  const Plan p = plan(ids.n, rows, H);
+  BAGUA_CHECK(ceil_div(H, kJoinColumns * 4) < 65536 && p.sum_blocks + ceil_div(ceil_div(rows, 32) * p.slices, kThreads / 32) < (1ll << 31), Tensor,
+              "embedding backward: " << rows << " rows of " << H << " columns");
+  auto at = [&](size_t offset) { return (uint32_t*)((char*)scratch + offset); };
+  uint32_t* present = accumulate ? nullptr : at(p.present);
+  if (present) BAGUA_CUDA_CHECK(cudaMemsetAsync(present, 0, (size_t)ceil_div(rows, 32) * 4, s));
+  SumArgs a{};
+  const Keys key{rows, padding};
+  int launches = ids.wide ? sort<int64_t>(ids, key, p, at(p.keys), at(p.counts), present, &a.keys, &a.places, s)
+                          : sort<int32_t>(ids, key, p, at(p.keys), at(p.counts), present, &a.keys, &a.places, s);
+  a.present = present;
+  a.partial = (float*)at(p.partial);
+  a.n = ids.n;
+  a.rows = rows;
+  a.H = H;
+  a.chunks = p.chunks;
+  a.sum_blocks = p.sum_blocks;
+  a.length = p.length;
+  a.slices = p.slices;
+  a.scale = scale;
+  typed(dout_type, [&](auto* d) {
+    typed(table_type, [&](auto* w) { sums<std::remove_pointer_t<decltype(d)>, std::remove_pointer_t<decltype(w)>>(a, p, dout, dtable, s); });
+  });
+  return launches + 1 + (p.chunks > 1);
+}
+
+}  // namespace embedding
+}  // namespace bagua

@@ -11,6 +11,7 @@
 
 #include "../common.h"
 #include "encoder_ops.h"
+#include "index_report.cuh"
 #include "launch.cuh"
 #include "model_ops_bodies.cuh"
 
@@ -56,41 +57,6 @@ __global__ void __launch_bounds__(kFoldCols * kFoldRows)
 void fold(const float* partial, float* out, int blocks, int C, bool accumulate, cudaStream_t s) {
   launch_overlapped(fold_kernel, dim3((C + kFoldCols - 1) / kFoldCols), dim3(kFoldCols, kFoldRows), s, partial, out, blocks, C,
                     accumulate);
-}
-
-// ---- indices outside their table -------------------------------------------------------------------
-// A kernel skips them and leaves the last one here, in host memory: the value first, then that there is one.
-struct IndexReport {
-  long long value[2];  // by kind: a token's id, a span's target
-  unsigned int seen[2];
-};
-enum { kTokenId = 0, kSpanTarget = 1 };
-__device__ __noinline__ void report_index(IndexReport* r, int kind, int64_t value) {
-  *(volatile long long*)&r->value[kind] = value;
-  __threadfence_system();
-  *(volatile unsigned int*)&r->seen[kind] = 1u;
-}
-// One per device, never given back: a captured graph keeps its address.
-IndexReport* index_report() {
-  static std::atomic<IndexReport*> reports[64] = {};
-  static std::mutex mu;
-  int dev = 0;
-  BAGUA_CUDA_CHECK(cudaGetDevice(&dev));
-  BAGUA_CHECK(dev >= 0 && dev < 64, Tensor, "device index " << dev << " out of range");
-  if (IndexReport* r = reports[dev].load(std::memory_order_acquire)) return r;
-  std::lock_guard<std::mutex> g(mu);
-  if (!reports[dev].load()) {
-    // allowed while a stream is being captured, as nothing is enqueued
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    BAGUA_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
-    IndexReport* r = nullptr;
-    const cudaError_t e = cudaHostAlloc((void**)&r, sizeof(IndexReport), cudaHostAllocMapped);
-    BAGUA_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
-    BAGUA_CUDA_CHECK(e);
-    std::memset(r, 0, sizeof(IndexReport));
-    reports[dev].store(r, std::memory_order_release);
-  }
-  return reports[dev].load();
 }
 
 // ---- embedding ------------------------------------------------------------------------------------
@@ -383,15 +349,39 @@ __global__ void __launch_bounds__(kThreads)
 
 }  // namespace
 
+IndexReport* index_report() {
+  static std::atomic<IndexReport*> reports[64] = {};
+  static std::mutex mu;
+  int dev = 0;
+  BAGUA_CUDA_CHECK(cudaGetDevice(&dev));
+  BAGUA_CHECK(dev >= 0 && dev < 64, Tensor, "device index " << dev << " out of range");
+  if (IndexReport* r = reports[dev].load(std::memory_order_acquire)) return r;
+  std::lock_guard<std::mutex> g(mu);
+  if (!reports[dev].load()) {
+    // allowed while a stream is being captured, as nothing is enqueued
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    BAGUA_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    IndexReport* r = nullptr;
+    const cudaError_t e = cudaHostAlloc((void**)&r, sizeof(IndexReport), cudaHostAllocMapped);
+    BAGUA_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    BAGUA_CUDA_CHECK(e);
+    std::memset(r, 0, sizeof(IndexReport));
+    reports[dev].store(r, std::memory_order_release);
+  }
+  return reports[dev].load();
+}
+
 void check_indices() {
+  static const char* const what[kIndexKinds][2] = {{"the token id ", ", which is not in the table"},
+                                                   {"the span target ", ", which is not in the sequence"},
+                                                   {"the target ", ", which is not in the vocabulary"}};
   IndexReport* r = index_report();
-  for (int kind : {kTokenId, kSpanTarget}) {
+  for (int kind = 0; kind < kIndexKinds; ++kind) {
     volatile unsigned int* seen = &r->seen[kind];
     if (*seen == 0) continue;
     const long long value = *(volatile long long*)&r->value[kind];
     *seen = 0;
-    throw BaguaError(ErrorKind::Tensor, (kind == kTokenId ? "an earlier call was given the token id " : "an earlier call was given the span target ") +
-                                            std::to_string(value) + (kind == kTokenId ? ", which is not in the table" : ", which is not in the sequence"));
+    throw BaguaError(ErrorKind::Tensor, std::string("an earlier call was given ") + what[kind][0] + std::to_string(value) + what[kind][1]);
   }
 }
 

@@ -17,7 +17,7 @@
 namespace bagua {
 namespace encoder_ops {
 
-// Throws if a kernel on the current device has met a token id outside its table or a span target outside its sequence since
+// Throws if a kernel on the current device has met a token id outside its table, a span target outside its sequence or a target outside its vocabulary since
 // the last look.  Such a call goes on with NaN in the index's place; the error comes with the next one whose host side
 // looks after the kernel ran, as with any error that a device finds.
 void check_indices();

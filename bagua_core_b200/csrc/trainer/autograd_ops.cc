@@ -4,6 +4,7 @@
 #include <ATen/cuda/CUDAEvent.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/autograd.h>
 #include <torch/csrc/autograd/function.h>
@@ -13,12 +14,14 @@
 #include <torch/csrc/autograd/variable.h>
 
 #include <array>
+#include <cmath>
 #include <functional>
 #include <memory>
 #include <mutex>
 #include <unordered_map>
 
 #include "../common.h"
+#include "../kernels/embedding.h"
 #include "../kernels/encoder_ops.h"
 #include "../kernels/kernels.h"
 #include "../kernels/model_ops.h"
@@ -689,6 +692,57 @@ struct EmbedNode : public EncoderNode {
   }
 };
 
+// ---- lookup by token -----------------------------------------------------------------------------
+bool kernel_type(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
+DType kernel_dtype(at::ScalarType t) { return t == at::kFloat ? DType::F32 : t == at::kHalf ? DType::F16 : DType::BF16; }
+
+at::Tensor lookup_composition(const at::Tensor& ids, const at::Tensor& table, double scale, int64_t padding, at::ScalarType type) {
+  // ids outside the table: rows of NaN without a gradient
+  const at::Tensor known = ids.ge(0).logical_and(ids.lt(table.size(0)));
+  const at::Tensor rows = at::embedding(table.to(at::kFloat), ids.to(at::kLong).masked_fill(known.logical_not(), 0), padding);
+  return (rows * scale).masked_fill(known.logical_not().unsqueeze(-1), NAN).to(type);
+}
+
+struct LookupNode : public EncoderNode {
+  SavedVariable ids;
+  at::Tensor table;
+  double scale = 1;
+  int64_t padding = -1;
+  at::ScalarType type = at::kFloat;
+
+  std::string name() const override { return "BaguaEmbeddingBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    ids.reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(1);
+    uses_done();
+    if (!grads[0].defined() || !task_should_compute_output(0)) return out;
+    encoder_ops::check_indices();
+    const at::Tensor id = ids.unpack();
+    if (c10::GradMode::is_enabled())
+      return differentiable_gradients(
+          *this, [&](const auto& in) { return lookup_composition(id, in[0], scale, padding, type); }, {{table.detach(), {0}}}, grads[0]);
+    const int64_t n = id.numel(), rows = table.size(0), H = table.size(1);
+    const bool add = adds_contiguous(0, table);
+    if (!add && (n == 0 || table.numel() == 0)) {
+      out[0] = at::zeros(table.sizes(), table.options());
+    } else if (n > 0 && table.numel() > 0) {
+      const at::Tensor d = grads[0].contiguous();
+      if (!add) out[0] = fresh(table.sizes(), table.scalar_type(), table);
+      // the framework's memory, not this package's pool: a graph that is being captured keeps it
+      const at::Tensor scratch = fresh({(int64_t)embedding::backward_scratch_bytes(n, rows, H)}, at::kByte, table);
+      count_launches(embedding::backward({id.data_ptr(), id.scalar_type() == at::kLong, n}, d.data_ptr(), kernel_dtype(d.scalar_type()), rows, H,
+                                         (float)scale, padding, add ? table.grad().data_ptr() : out[0].data_ptr(),
+                                         kernel_dtype(table.scalar_type()), add, scratch.data_ptr(), stream_of(table)));
+    }
+    if (add) added(0, table);
+    return out;
+  }
+};
+
 at::Tensor span_loss_composition(const at::Tensor& logits, const at::Tensor& start, const at::Tensor& end) {
   const at::Tensor f = logits.to(at::kFloat);
   return (at::cross_entropy_loss(f.select(2, 0), start) + at::cross_entropy_loss(f.select(2, 1), end)) / 2;
@@ -975,6 +1029,60 @@ at::Tensor embed_layer_norm(const at::Tensor& ids, const at::Tensor& tok, const 
     torch::autograd::set_history(y[0], node);
   }
   return y[0];
+}
+
+at::Tensor embedding(const at::Tensor& ids, const at::Tensor& table, double scale, int64_t padding, std::optional<at::ScalarType> type,
+                     bool accumulate) {
+  BAGUA_CHECK(table.dim() == 2 && table.layout() == at::kStrided && kernel_type(table.scalar_type()) && (table.is_cuda() || table.is_cpu()), Tensor,
+              "embedding needs a table [rows, columns] of float32, float16 or bfloat16 on a GPU or the host");
+  BAGUA_CHECK((ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) && ids.layout() == at::kStrided && ids.device() == table.device(),
+              Tensor, "embedding needs ids of int64 or int32 on the table's device");
+  const at::ScalarType to = type.value_or(table.scalar_type());
+  BAGUA_CHECK(kernel_type(to), Tensor, "embedding gives float32, float16 or bfloat16");
+  const int64_t n = ids.numel(), rows = table.size(0), H = table.size(1);
+  BAGUA_CHECK(padding >= -1 && padding < std::max<int64_t>(rows, 1), Tensor, "padding row " << padding << " of a table of " << rows << " rows");
+  BAGUA_CHECK(n <= embedding::kMaxTokens && rows <= embedding::kMaxRows, Tensor, "embedding takes " << embedding::kMaxTokens << " tokens and "
+                                                                                                    << embedding::kMaxRows << " rows at most");
+  BAGUA_CHECK(std::isfinite(scale) && std::isfinite((float)scale), Tensor, "embedding needs a finite scale");
+  if (!table.is_cuda() || watched({&ids, &table})) {
+    c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
+    if (table.is_cpu() && n > 0 && !watched({&ids})) {
+      const int64_t low = ids.min().item<int64_t>(), high = ids.max().item<int64_t>();
+      BAGUA_CHECK(low >= 0 && high < rows, Tensor, "token id " << (low < 0 ? low : high) << " is not in the table of " << rows << " rows");
+    }
+    return lookup_composition(ids, table, scale, padding, to);
+  }
+  const c10::cuda::CUDAGuard on(table.device());
+  std::shared_ptr<LookupNode> node;
+  if (torch::autograd::compute_requires_grad(table)) {
+    node = std::shared_ptr<LookupNode>(new LookupNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(table));
+  }
+  encoder_ops::check_indices();
+  at::Tensor idc, y;
+  {
+    PlainDispatch plain;
+    idc = ids.contiguous();
+    const at::Tensor w = H <= 1 || table.stride(1) == 1 ? table : table.contiguous();
+    std::vector<int64_t> sizes = ids.sizes().vec();
+    sizes.push_back(H);
+    y = fresh(sizes, to, table);
+    if (y.numel() > 0) {
+      embedding::lookup({idc.data_ptr(), idc.scalar_type() == at::kLong, n}, w.data_ptr(), kernel_dtype(w.scalar_type()), rows, w.stride(0), H,
+                        (float)scale, y.data_ptr(), kernel_dtype(to), stream_of(table));
+      count_launches(1);
+    }
+  }
+  if (node) {
+    node->ids = SavedVariable(idc, false);
+    node->table = table;
+    node->scale = scale;
+    node->padding = padding;
+    node->type = to;
+    if (accumulate) node->accumulate_gradients({&table});
+    torch::autograd::set_history(y, node);
+  }
+  return y;
 }
 
 at::Tensor span_loss(const at::Tensor& logits, const at::Tensor& start, const at::Tensor& end) {

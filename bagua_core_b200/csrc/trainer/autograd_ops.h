@@ -44,6 +44,11 @@ at::Tensor add_layer_norm(const at::Tensor& x, const std::optional<at::Tensor>& 
 at::Tensor embed_layer_norm(const at::Tensor& ids, const at::Tensor& tok, const at::Tensor& pos, const at::Tensor& typ,
                             const at::Tensor& gamma, const at::Tensor& beta, double eps, bool accumulate);
 
+// scale * table[ids] in `type` (the table's by default), ids of int64 or int32 in any shape; `padding` (-1: none): a row without gradient.  With
+// `accumulate`, the backward adds the gradient to the table's fp32 `.grad` itself where nobody can tell the difference.
+at::Tensor embedding(const at::Tensor& ids, const at::Tensor& table, double scale, int64_t padding, std::optional<at::ScalarType> type,
+                     bool accumulate);
+
 // (cross_entropy(logits[..., 0], start) + cross_entropy(logits[..., 1], end)) / 2 of bf16 logits [batch, seq, 2] with int64
 // positions [batch]; rows with position -100 do not count.
 at::Tensor span_loss(const at::Tensor& logits, const at::Tensor& start, const at::Tensor& end);

@@ -10,6 +10,7 @@ import torch
 
 from .._native import C as _C
 from .. import BaguaTensorPy
+from .token_embedding import ScaledEmbedding, embedding  # noqa: F401
 from .adamw import adamw_read8, adamw_state8, adamw_step  # noqa: F401
 
 
