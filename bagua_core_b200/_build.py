@@ -60,6 +60,7 @@ SOURCES = [
     "kernels/model_ops_cpu.cc",
     "kernels/encoder_ops.cu",
     "kernels/embedding.cu",
+    "kernels/token_log_probs.cu",
     "kernels/adamw.cu",
     "kernels/adamw_host.cc",
 ]

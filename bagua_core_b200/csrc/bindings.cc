@@ -24,6 +24,7 @@
 #include "kernels/kernels.h"
 #include "kernels/encoder_ops.h"
 #include "kernels/model_ops.h"
+#include "kernels/token_log_probs.h"
 #include "ops/comm_op.h"
 #include "pool/resource_pool.h"
 #include "runtime/backend.h"
@@ -999,6 +1000,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embed_layer_norm", &trainer::embed_layer_norm, py::arg("ids"), py::arg("tokens"), py::arg("positions"),
         py::arg("types"), py::arg("weight"), py::arg("bias"), py::arg("eps"), py::arg("accumulate"),
         "layer_norm(tokens[ids] + positions[:seq] + types[0]) in bf16.");
+  m.def("token_log_probs", &trainer::token_log_probs, py::arg("logits"), py::arg("targets"), py::arg("top"), py::arg("ignore_index"),
+        "[log probabilities of targets, entropies, values and ids of the likeliest tokens] of rows of logits.");
+  m.attr("max_top_tokens") = token_log_probs::kMaxTop;
   m.def("embedding", [](const at::Tensor& ids, const at::Tensor& table, double scale, int64_t padding, const py::object& type, bool accumulate) {
           std::optional<at::ScalarType> to;
           if (!type.is_none()) {

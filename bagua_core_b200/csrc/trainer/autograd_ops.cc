@@ -16,6 +16,7 @@
 #include <array>
 #include <cmath>
 #include <functional>
+#include <limits>
 #include <memory>
 #include <mutex>
 #include <unordered_map>
@@ -25,6 +26,7 @@
 #include "../kernels/encoder_ops.h"
 #include "../kernels/kernels.h"
 #include "../kernels/model_ops.h"
+#include "../kernels/token_log_probs.h"
 #include "../tensor/tensor.h"
 #include "gemm.h"
 
@@ -772,6 +774,100 @@ struct SpanLossNode : public Node {
   }
 };
 
+// ---- log probabilities ---------------------------------------------------------------------------
+// {log probabilities, entropies} in fp32, as the kernels define them for rows that are ignored, masked or not finite.
+std::vector<at::Tensor> log_prob_composition(const at::Tensor& logits, const at::Tensor& targets, int64_t ignored) {
+  const double inf = std::numeric_limits<double>::infinity();
+  const int64_t vocab = logits.size(-1);
+  const at::Tensor scored = targets.ne(ignored), known = targets.ge(0).logical_and(targets.lt(vocab));
+  const at::Tensor all = logits.to(at::kFloat).contiguous();
+  const at::Tensor none = all.eq(-inf).all(-1);
+  // where() keeps what is not finite out of the gradients
+  const at::Tensor x = at::where(scored.logical_and(none.logical_not()).unsqueeze(-1), all, 0.0);
+  const at::Tensor ls = at::log_softmax(x, -1), p = ls.exp();
+  at::Tensor lp = ls.gather(-1, targets.masked_fill(known.logical_not(), 0).unsqueeze(-1)).squeeze(-1);
+  lp = at::where(none, -inf, lp);
+  lp = at::where(known, lp, std::numeric_limits<double>::quiet_NaN());
+  lp = at::where(scored, lp, 0.0);
+  // (the largest NaN-preserving lower bound: 0 * -inf has no place in the sum)
+  const at::Tensor entropy = at::where(scored.logical_and(none.logical_not()), (p * ls.clamp_min(-1e30)).sum(-1).neg(), 0.0);
+  return {lp, entropy};
+}
+// {values, ids} of the likeliest tokens, detached.
+std::vector<at::Tensor> top_composition(const at::Tensor& logits, const at::Tensor& targets, int64_t top, int64_t ignored) {
+  const double inf = std::numeric_limits<double>::infinity();
+  const at::Tensor all = logits.detach().to(at::kFloat).contiguous();
+  const auto sorted = at::sort(all, /*stable=*/true, -1, /*descending=*/true);
+  const at::Tensor lse = at::logsumexp(all, {-1}, true), lost = lse.isnan().logical_or(lse.eq(inf)).squeeze(-1).unsqueeze(-1);
+  const at::Tensor best = std::get<0>(sorted).narrow(-1, 0, top);
+  at::Tensor v = at::where(best.eq(-inf), best, best - lse), ids = std::get<1>(sorted).narrow(-1, 0, top);
+  v = at::where(lost, std::numeric_limits<double>::quiet_NaN(), v);
+  ids = ids.masked_fill(lost, -1);
+  const at::Tensor skipped = targets.eq(ignored).unsqueeze(-1);
+  return {v.masked_fill(skipped, -inf), ids.masked_fill(skipped, -1)};
+}
+
+// Logits as rows: [rows, vocab] with neighbouring columns, a view where there is one.
+at::Tensor logit_rows(const at::Tensor& logits) {
+  const at::Tensor x = logits.reshape({-1, logits.size(-1)});
+  return x.size(1) <= 1 || x.stride(1) == 1 ? x : x.contiguous();
+}
+
+struct LogProbNode : public Node {
+  SavedVariable logits, targets, stats;
+  int64_t ignored = -100;
+
+  std::string name() const override { return "BaguaTokenLogProbsBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&logits, &targets, &stats}) v->reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(1);
+    if ((!grads[0].defined() && !grads[1].defined()) || !task_should_compute_output(0)) return out;
+    encoder_ops::check_indices();
+    const at::Tensor given = logits.unpack(), t = targets.unpack(), st = stats.unpack();
+    if (c10::GradMode::is_enabled()) {
+      const auto f = [&](const auto& in) {
+        const auto r = log_prob_composition(in[0], t, ignored);
+        at::Tensor y;
+        for (int k = 0; k < 2; ++k)
+          if (grads[k].defined()) {
+            // (a row whose log probability is not finite has no gradient: its factor would make one)
+            const at::Tensor part = at::where(r[k].detach().eq(-std::numeric_limits<double>::infinity()), 0.0, r[k]).mul(grads[k]).sum();
+            y = y.defined() ? y + part : part;
+          }
+        return y;
+      };
+      return differentiable_gradients(*this, f, {{given, {0}}}, at::ones({}, given.options().dtype(at::kFloat)));
+    }
+    const at::Tensor x = logit_rows(given.detach());
+    const int64_t rows = x.size(0), vocab = x.size(1), elements = 16 / (int64_t)x.element_size();
+    // rows of the gradient lie as far from 16-byte borders as the logits' do, so that both are moved 16 bytes at a time
+    const int64_t stride = rows > 1 ? vocab + ((x.stride(0) - vocab) % elements + elements) % elements : vocab;
+    const int64_t lead = (int64_t)((uintptr_t)x.data_ptr() % 16) / (int64_t)x.element_size();
+    at::Tensor dx;
+    if (stride == vocab && lead == 0) {
+      dx = fresh(given.sizes(), x.scalar_type(), x);
+    } else {
+      std::vector<int64_t> strides(given.dim(), 1);
+      for (int64_t k = given.dim() - 2, step = stride; k >= 0; step *= given.size(k--)) strides[k] = step;
+      dx = fresh({lead + rows * stride}, x.scalar_type(), x).as_strided(given.sizes(), strides, lead);
+    }
+    at::Tensor g[2];
+    for (int k = 0; k < 2; ++k)
+      if (grads[k].defined()) g[k] = grads[k].reshape({-1});
+    token_log_probs::backward({x.data_ptr(), kernel_dtype(x.scalar_type()), rows, vocab, x.stride(0)}, t.data_ptr<int64_t>(),
+                              (const token_log_probs::RowStats*)st.data_ptr(), g[0].defined() ? g[0].data_ptr<float>() : nullptr,
+                              g[0].defined() ? g[0].stride(0) : 0, g[1].defined() ? g[1].data_ptr<float>() : nullptr,
+                              g[1].defined() ? g[1].stride(0) : 0, dx.data_ptr(), stride, stream_of(x));
+    count_launches(1);
+    out[0] = dx;
+    return out;
+  }
+};
+
 // q, k, v as views of the packed projection; backward writes their gradients into one packed tensor.
 struct SplitHeadsNode : public Node {
   int64_t batch = 0, seq = 0, heads = 0, dim = 0;
@@ -1124,6 +1220,71 @@ at::Tensor span_loss(const at::Tensor& logits, const at::Tensor& start, const at
     torch::autograd::set_history(loss, node);
   }
   return loss;
+}
+
+std::vector<at::Tensor> token_log_probs(const at::Tensor& logits, const at::Tensor& targets, int64_t top, int64_t ignored) {
+  BAGUA_CHECK(logits.dim() >= 1 && logits.layout() == at::kStrided && kernel_type(logits.scalar_type()) && (logits.is_cuda() || logits.is_cpu()),
+              Tensor, "token_log_probs needs logits [..., vocabulary] of float32, float16 or bfloat16 on a GPU or the host");
+  BAGUA_CHECK(targets.scalar_type() == at::kLong && targets.layout() == at::kStrided && targets.device() == logits.device() &&
+                  targets.sizes() == logits.sizes().slice(0, logits.dim() - 1),
+              Tensor, "token_log_probs needs an int64 target for each row of logits, on their device");
+  const int64_t vocab = logits.size(-1), rows = targets.numel();
+  BAGUA_CHECK(vocab >= 1 && vocab <= token_log_probs::kMaxVocab && rows <= token_log_probs::kMaxRows, Tensor,
+              "token_log_probs: " << rows << " rows of " << vocab << " logits");
+  BAGUA_CHECK(top >= 0 && top <= token_log_probs::kMaxTop && top <= vocab, Tensor,
+              "token_log_probs gives 0 to " << std::min<int64_t>(token_log_probs::kMaxTop, vocab) << " alternatives here, not " << top);
+  std::vector<at::Tensor> out(4);
+  if (!logits.is_cuda() || rows == 0 || watched({&logits, &targets})) {
+    c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
+    if (logits.is_cpu() && rows > 0 && !watched({&logits, &targets})) {
+      const at::Tensor bad = targets.lt(0).logical_or(targets.ge(vocab)).logical_and(targets.ne(ignored));
+      BAGUA_CHECK(!bad.any().item<bool>(), Tensor, "target " << targets.masked_select(bad)[0].item<int64_t>() << " is not in the vocabulary of " << vocab);
+    }
+    const auto both = log_prob_composition(logits, targets, ignored);
+    out[0] = both[0];
+    out[1] = both[1];
+    if (top) {
+      const auto best = top_composition(logits, targets, top, ignored);
+      out[2] = best[0];
+      out[3] = best[1];
+    }
+    return out;
+  }
+  const c10::cuda::CUDAGuard on(logits.device());
+  std::shared_ptr<LogProbNode> node;
+  if (torch::autograd::compute_requires_grad(logits)) {
+    node = std::shared_ptr<LogProbNode>(new LogProbNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+  }
+  encoder_ops::check_indices();
+  at::Tensor t, stats;
+  {
+    PlainDispatch plain;
+    const at::Tensor x = logit_rows(logits);
+    t = targets.contiguous();
+    for (int k = 0; k < 2; ++k) out[k] = fresh(targets.sizes(), at::kFloat, x);
+    if (top) {
+      std::vector<int64_t> sizes = targets.sizes().vec();
+      sizes.push_back(top);
+      out[2] = fresh(sizes, at::kFloat, x);
+      out[3] = fresh(sizes, at::kLong, x);
+    }
+    if (node) stats = fresh({rows, (int64_t)(sizeof(token_log_probs::RowStats) / sizeof(float))}, at::kFloat, x);
+    token_log_probs::forward({x.data_ptr(), kernel_dtype(x.scalar_type()), rows, vocab, x.stride(0)}, t.data_ptr<int64_t>(), ignored, (int)top,
+                             out[0].data_ptr<float>(), out[1].data_ptr<float>(), top ? out[2].data_ptr<float>() : nullptr,
+                             top ? out[3].data_ptr<int64_t>() : nullptr, node ? (token_log_probs::RowStats*)stats.data_ptr() : nullptr,
+                             stream_of(x));
+    count_launches(1);
+  }
+  if (node) {
+    node->logits = SavedVariable(logits, false);
+    node->targets = SavedVariable(t, false);
+    node->stats = SavedVariable(stats, false);
+    node->ignored = ignored;
+    torch::autograd::set_history(out[0], node);
+    torch::autograd::set_history(out[1], node);
+  }
+  return out;
 }
 
 at::Tensor attention(const at::Tensor& qkv, int64_t heads, double dropout) {

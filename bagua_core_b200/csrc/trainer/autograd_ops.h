@@ -53,6 +53,10 @@ at::Tensor embedding(const at::Tensor& ids, const at::Tensor& table, double scal
 // positions [batch]; rows with position -100 do not count.
 at::Tensor span_loss(const at::Tensor& logits, const at::Tensor& start, const at::Tensor& end);
 
+// {log probabilities of `targets`, entropies, values and ids of the `top` likeliest tokens} of rows of logits [..., vocab]
+// (csrc/kernels/token_log_probs.h); targets [...] of int64.  The first two can be differentiated.  top == 0: the last two are undefined.
+std::vector<at::Tensor> token_log_probs(const at::Tensor& logits, const at::Tensor& targets, int64_t top, int64_t ignored);
+
 // Multi-head attention of a packed projection qkv [batch, seq, 3 * heads * dim] (bf16, CUDA): [batch, seq, heads * dim].
 at::Tensor attention(const at::Tensor& qkv, int64_t heads, double dropout);
 

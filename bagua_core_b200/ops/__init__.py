@@ -11,6 +11,7 @@ import torch
 from .._native import C as _C
 from .. import BaguaTensorPy
 from .token_embedding import ScaledEmbedding, embedding  # noqa: F401
+from .token_log_probs import TokenLogProbs, token_log_probs  # noqa: F401
 from .adamw import adamw_read8, adamw_state8, adamw_step  # noqa: F401
 
 

@@ -1,0 +1,262 @@
+"""Log probabilities of given tokens, entropies, alternatives (`ops.token_log_probs`) and the logits' gradient, against their
+definition in 64 bits, on the host.  The GPU runs the same checks (`test_gpu_token_log_probs.py`)."""
+import math
+
+import pytest
+import torch
+
+import bagua_core_b200.ops as ops
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+U = 2.0 ** -24  # half a step of fp32
+INF = float("inf")
+
+
+def plain(x, targets, top, ignored, a=None, b=None):
+    """(log probs, entropies, values, ids, gradient) in 64 bits of rows [n, vocab]."""
+    x = x.detach().cpu().double()
+    t = targets.cpu()
+    n, vocab = x.shape
+    scored = t != ignored
+    none = (x == -INF).all(1)
+    lost = (x.isnan() | (x == INF)).any(1)
+    d = x - torch.where(none | lost, 0.0, x.amax(1))[:, None]  # differences first: values may be as large as fp32's
+    lp_all = torch.where(x == -INF, -INF, d - d.exp().sum(1).log()[:, None])
+    lp_all[lost] = math.nan
+    p = torch.where(none[:, None], 0.0, lp_all.exp())
+    plogp = torch.where(p > 0, p * lp_all, 0.0)
+    plogp[lost] = math.nan
+    entropy = torch.where(none, 0.0, -plogp.sum(1))
+    hit = torch.zeros_like(x).scatter_(1, t.clamp(0, vocab - 1)[:, None], 1.0)
+    lp = lp_all.gather(1, t.clamp(0, vocab - 1)[:, None])[:, 0]
+    order = torch.sort(torch.where(x.isnan(), -INF, x), dim=1, descending=True, stable=True)
+    values, ids = lp_all.gather(1, order.indices)[:, :top], order.indices[:, :top].clone()
+    ids[lost] = -1
+    values[~scored], ids[~scored] = -INF, -1
+    grad = None
+    if a is not None:
+        a, b = a.cpu().double(), b.cpu().double()
+        grad = a[:, None] * (hit - p) - b[:, None] * (plogp + p * entropy[:, None])
+        grad[~scored | none] = 0
+    return torch.where(scored, lp, 0.0), torch.where(scored, entropy, 0.0), values, ids, grad
+
+
+def close(got, want, bound):
+    got = got.detach().cpu().double()
+    same = (got == want) | (got.isnan() & want.isnan())
+    assert (same | ((got - want).abs() <= bound)).all(), float(((got - want).abs() - bound).masked_fill(same, -1).max())
+
+
+def logits(n, vocab, dtype, seed=0, size=3.0, masked=0.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, vocab, generator=g) * size * torch.rand(n, 1, generator=g)
+    if masked:
+        x[torch.rand(n, vocab, generator=g) < masked] = -INF
+    return x.to(dtype), torch.randint(0, vocab, (n,), generator=g)
+
+
+def check(x, targets, top=0, ignored=-100, backward=True, make=lambda x: x):
+    """`make`: the tensor of the same values that the operator is given."""
+    n, vocab = x.shape
+    y = make(x.detach()).requires_grad_(backward)
+    r = ops.token_log_probs(y, targets.to(y.device), top, ignored)
+    g = torch.Generator().manual_seed(5)
+    a, b = torch.randn(n, generator=g), torch.randn(n, generator=g)
+    lp, entropy, values, ids, grad = plain(x, targets, top, ignored, a, b)
+    # each exponential 2^-22, its argument two half steps of its size (below 2^7 where it counts), a sum of up to vocab / 256 + 64 terms in a
+    # row; then logarithm, difference and product
+    off = 2.0 ** -22 + (vocab / 256 + 64 + 2 ** 8) * U
+    size = x.detach().cpu().double().nan_to_num(0, 0, 0).abs().clamp(max=1e30)
+    m = torch.where(size.isinf(), 0, size).amax(1)
+    close(r.log_probs, lp, off + 4 * U * (lp.abs().nan_to_num(0, 0, 0) + m))
+    close(r.entropy, entropy, 2 * off * (1 + entropy.abs().nan_to_num(0, 0, 0) + 4))
+    if top:
+        assert r.top_ids.shape == (n, top) and torch.equal(r.top_ids.cpu(), ids)
+        close(r.top_log_probs, values, off + 4 * U * (values.abs().nan_to_num(0, 0, 0) + m[:, None]))
+        assert not r.top_log_probs.requires_grad
+    else:
+        assert r.top_ids is None and r.top_log_probs is None
+    if backward:
+        (d,) = torch.autograd.grad((r.log_probs, r.entropy), y, (a.to(y.device), b.to(y.device)))
+        assert d.shape == y.shape and d.dtype == y.dtype
+        half = torch.finfo(x.dtype).eps / 2
+        lpa = torch.log_softmax(x.detach().cpu().double().clamp(min=-1e30), 1).nan_to_num(0, 0, 0).abs().clamp(max=100)
+        p = torch.exp(-lpa)
+        entropy = entropy.abs().nan_to_num(0, 0, 0)
+        # (where p is below 2^-100 nothing is left of it)
+        parts = p * (a.abs()[:, None] + b.abs()[:, None] * (lpa + entropy[:, None] + 4).double()) + a.abs()[:, None] * 0
+        close(d, grad, 4 * off * parts + half * grad.abs().nan_to_num(0, 0, 0) + U * a.abs()[:, None] * 2 + torch.finfo(x.dtype).smallest_normal * half + 2.0 ** -100)
+    return r
+
+
+SIZES = [(1, 1), (3, 2), (4, 7), (5, 33), (9, 255), (3, 1000)]
+
+
+@pytest.mark.parametrize("dtype", TYPES.values())
+@pytest.mark.parametrize("n,vocab", SIZES)
+def test_against_the_definition(n, vocab, dtype):
+    x, t = logits(n, vocab, dtype)
+    check(x, t, min(vocab, 5))
+    x, t = logits(n, vocab, dtype, masked=0.5)
+    check(x, t, min(vocab, 32))
+
+
+def check_special(device):
+    for dtype in TYPES.values():
+        low = torch.finfo(dtype).min
+        for vocab in (40, 3000):
+            x, t = logits(12, vocab, dtype)
+            x[0] = -INF                  # no token left
+            x[1] = low                   # all equal, at the type's lowest value
+            x[2, 1:] = low               # one left by a mask of that value
+            x[3, 1:] = -INF              # one left
+            x[4, 7] = math.nan
+            x[5, 3] = INF
+            x[6] = torch.finfo(dtype).max
+            x[7, ::2] = low
+            x[8] = x[8, 0]               # all equal
+            x[9, 5] = x[9].max() + 1
+            x[9, 20] = x[9, 5]           # two equal at the top
+            t[10] = -100
+            x[11] = -INF
+            t[11] = -100
+            t[2], t[3], t[9] = 0, 0, 20
+            check(x.to(device), t, 6)
+            check(x.to(device), t, 32)
+            x[10] = math.nan             # a row that is not looked at
+            r = check(x.to(device), t, 1)
+            assert r.log_probs[10] == 0 and r.entropy[10] == 0
+            # another mark, which may be a token
+            check(x.to(device), t.masked_fill(t == -100, 4), 2, ignored=4)
+
+
+def test_special_rows():
+    check_special("cpu")
+
+
+def check_layouts(device):
+    x, t = logits(24, 37, torch.bfloat16)
+    x, t = x.to(device), t.to(device)
+    want = ops.token_log_probs(x, t, 3)
+
+    # The order of a row's sum follows its alignment: two orders differ by at most what each may be off (37 terms, sums and
+    # values below 2^5), gradients by that relative to 1 and then by a step of bf16.
+    off = 2 * (2.0 ** -22 + (37 + 64) * U) * 8
+
+    def alike(d, first):
+        return ((d.double() - first.double()).abs() <= 2 * off + 2.0 ** -7 * first.double().abs()).all()
+
+    def same(y, shape, u=t):
+        y = y.requires_grad_()
+        r = ops.token_log_probs(y, u.view(shape), 3)
+        assert r.log_probs.shape == shape and torch.equal(r.top_ids.reshape(24, 3), want.top_ids) and r.top_ids.shape == (*shape, 3)
+        assert all(((p.reshape(q.shape) - q).abs() <= off).all() for p, q in zip(r[:3], want[:3]))
+        (d,) = torch.autograd.grad((r.log_probs.sum(), r.entropy.sum()), y)
+        assert d.shape == y.shape
+        return d.reshape(24, 37)
+
+    first = same(x.clone(), (24,))
+    assert alike(same(x.clone().view(2, 3, 4, 37), (2, 3, 4)), first)
+    for pad in (1, 3, 11):  # a vocabulary padded to a multiple: rows that start anywhere
+        wide = torch.full((24, 37 + pad), 9.0, dtype=x.dtype, device=device)
+        wide[:, :37] = x
+        assert alike(same(wide[:, :37], (24,)), first)
+        wide[:, pad:] = x
+        assert alike(same(wide[:, pad:].unflatten(0, (4, 6)), (4, 6)), first)
+    assert alike(same(x.t().contiguous().t(), (24,)), first)
+    half = torch.zeros(48, 37, dtype=x.dtype, device=device)
+    half[::2] = x
+    assert alike(same(half[::2], (24,)), first)
+    swapped = x.view(4, 6, 37).transpose(0, 1).contiguous().transpose(0, 1)  # rows in another order
+    assert alike(same(swapped, (4, 6)), first)
+    one = ops.token_log_probs(x[5], t[5], 2)
+    assert one.log_probs.shape == () and (one.log_probs - want.log_probs[5]).abs() <= off and torch.equal(one.top_ids, want.top_ids[5, :2])
+    # one row for many targets: the gradients of a broadcast row are summed
+    row = x[:1].float().requires_grad_()
+    u = torch.arange(37, device=device)
+    lp = ops.token_log_probs(row.expand(37, 37), u).log_probs
+    (d,) = torch.autograd.grad(lp.sum(), row)
+    p = torch.softmax(row.detach().double(), 1)
+    assert (d.double() - (1 - 37 * p)).abs().max() <= 37 * 40 * U
+    # no rows
+    for shape in ((0, 5), (2, 0, 5)):
+        e = torch.zeros(shape, device=device, requires_grad=True)
+        r = ops.token_log_probs(e, torch.zeros(shape[:-1], dtype=torch.int64, device=device), 2)
+        assert r.log_probs.shape == shape[:-1] and r.top_ids.shape == (*shape[:-1], 2)
+        r.log_probs.sum().backward()
+        assert e.grad.shape == shape
+
+
+def test_layouts():
+    check_layouts("cpu")
+
+
+def check_partial_gradients(device):
+    x, t = logits(6, 50, torch.float32)
+    for k in range(2):
+        y = x.to(device).requires_grad_()
+        r = ops.token_log_probs(y, t.to(device))
+        (d,) = torch.autograd.grad(r[k].sum(), y)
+        a, b = torch.full((6,), float(k == 0)), torch.full((6,), float(k == 1))
+        want = plain(x, t, 0, -100, a, b)[4]
+        assert (d.cpu().double() - want).abs().max() <= 400 * U
+    # against differences in 64 bits of the definition
+    eps = 1e-5
+    y = x.to(device).requires_grad_()
+    r = ops.token_log_probs(y, t.to(device))
+    (d,) = torch.autograd.grad((2.0 * r.log_probs - 0.5 * r.entropy).sum(), y)
+    for i, j in ((0, 0), (2, 49), (5, int(t[5]))):
+        ends = []
+        for s in (1, -1):
+            z = x.double().clone()
+            z[i, j] += s * eps
+            lp, h, *_ = plain(z, t, 0, -100)
+            ends.append(float((2.0 * lp - 0.5 * h).sum()))
+        assert abs((ends[0] - ends[1]) / (2 * eps) - float(d[i, j])) < 1e-5
+
+
+def test_one_gradient_of_two():
+    check_partial_gradients("cpu")
+
+
+def check_second_order(device):
+    x, t = logits(3, 6, torch.float32)
+    x[0, 2] = -INF
+    t[2] = -100
+    f = lambda y: (lambda r: (r.log_probs * torch.tensor([1.0, -2.0, 3.0], device=device)).sum() + r.entropy.sum())(ops.token_log_probs(y, t.to(device)))  # noqa: E731
+
+    def g(y):
+        r = torch.log_softmax(y, 1)
+        p = r.exp()
+        lp = r.gather(1, t.to(device)[:, None].clamp(min=0))[:, 0]
+        h = -(p * r.clamp(min=-1e30)).sum(1)
+        return lp[0] - 2 * lp[1] + h[0] + h[1]
+
+    ys = [x.to(device).requires_grad_() for _ in range(2)]
+    v = torch.randn(3, 6, generator=torch.Generator().manual_seed(2)).to(device)
+    v[0, 2] = 0
+    got = []
+    for fn, y in zip((f, g), ys):
+        (d,) = torch.autograd.grad(fn(y), y, create_graph=True)
+        got.append((d.detach(), torch.autograd.grad((d * v).sum(), y)[0]))
+    assert torch.allclose(got[0][0], got[1][0], atol=1e-6) and torch.allclose(got[0][1], got[1][1], atol=1e-6)
+
+
+def test_second_order():
+    check_second_order("cpu")
+
+
+def check_refusals(device):
+    x, t = torch.zeros(3, 5, device=device), torch.zeros(3, dtype=torch.int64, device=device)
+    for args in ((x.double(), t), (x.long(), t), (x, t.int()), (x, t[:2]), (x, t.view(3, 1)), (x, t, 6), (x, t, -1), (x[:, :0], t),
+                 (torch.zeros((), device=device), t), (torch.zeros(3, 50, device=device), t, 33), (x.to_sparse(), t)):
+        with pytest.raises(RuntimeError):
+            ops.token_log_probs(*args)
+
+
+def test_refusals():
+    check_refusals("cpu")
+    x = torch.zeros(3, 5)
+    for bad in (-1, 5):
+        with pytest.raises(RuntimeError, match="not in the vocabulary"):
+            ops.token_log_probs(x, torch.tensor([0, bad, -100]))
