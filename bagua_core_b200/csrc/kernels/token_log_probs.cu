@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "index_report.cuh"
 #include "launch.cuh"
@@ -22,7 +23,6 @@ using encoder_ops::report_index;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr unsigned kFull = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kNoToken = 0x7fffffff;
 
 __device__ __forceinline__ float exp2_fast(float x) {  // to 2^-22
   float y;
@@ -98,51 +98,141 @@ __device__ __forceinline__ void add(Sums& a, const float (&x)[N], float largest)
   }
 }
 
+// ---- parts of a row -----------------------------------------------------------------------------
+// Elements in front of the first 16-byte border, whole vectors, elements behind them; `part` of `parts` of the vectors is lo .. hi.
+struct RowParts {
+  int front, behind, rest, lo, hi;  // rest: elements outside the vectors
+};
+template <typename T>
+__device__ __forceinline__ RowParts row_parts(const T* x, int vocab, int part, int parts) {
+  constexpr int kVec = 16 / sizeof(T);
+  RowParts r;
+  r.front = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
+  const int vectors = (vocab - r.front) / kVec;
+  r.behind = r.front + vectors * kVec;
+  r.rest = vocab - r.behind + r.front;
+  r.lo = (int)((int64_t)vectors * part / parts);
+  r.hi = (int)((int64_t)vectors * (part + 1) / parts);
+  return r;
+}
+
 // ---- alternatives -------------------------------------------------------------------------------
-// A warp keeps the 32 best it has seen, one a lane, the best first; equal values in the order of their ids.
+// The `top` largest of a group of threads' values, equal ones in the order of their ids, -inf and NaN not among them.
+//
+// A list kept along the way costs ten times the pass itself (64 rows of 131072, 20 alternatives: 98 us).  Here the first
+// pass leaves each thread's largest value, which the sums have anyway.  The top-th largest of those is a floor: that many values at
+// least are not below it, and in rows that are not ordered hardly more.  A second pass, from L2, collects the values that
+// reach the floor, and those few are put in order by counting, for each, the better ones.
 struct Best {
   float value;
   int id;
 };
-__device__ __forceinline__ bool better(float v, int id, float than, int than_id) { return v > than || (v == than && id < than_id); }
-__device__ __forceinline__ void insert(Best& b, float v, int id) {
-  const int lane = (int)threadIdx.x & 31;
-  const int at = __popc(__ballot_sync(kFull, better(b.value, b.id, v, id)));
-  const float up = __shfl_up_sync(kFull, b.value, 1);
-  const int up_id = __shfl_up_sync(kFull, b.id, 1);
-  if (lane > at) {
-    b.value = up;
-    b.id = up_id;
-  } else if (lane == at) {
-    b.value = v;
-    b.id = id;
-  }
+__device__ __forceinline__ bool better(const Best& a, const Best& b) { return a.value > b.value || (a.value == b.value && a.id < b.id); }
+constexpr int kNoToken = 0x7fffffff;
+constexpr int kRoom = 256;  // candidates of a group; where more reach the floor (equal values), they are taken a few at a time
+
+template <int kGroup>
+__device__ __forceinline__ void sync_group() {
+  if constexpr (kGroup == 32)
+    __syncwarp();
+  else
+    __syncthreads();
 }
-// The last of the `top` best, which a candidate has to be better than.
-struct Bar {
-  float value;
-  int id;
+template <int kGroup>
+struct TopScratch {
+  float largest[kGroup];
+  Best found[kRoom];
+  int count;
+  float floor;
 };
-__device__ __forceinline__ Bar bar_of(const Best& b, int top) { return Bar{__shfl_sync(kFull, b.value, top - 1), __shfl_sync(kFull, b.id, top - 1)}; }
-// One candidate a lane.
-__device__ __forceinline__ void offer(Best& b, Bar& bar, int top, float v, int id, bool valid) {
-  unsigned mask = __ballot_sync(kFull, valid && better(v, id, bar.value, bar.id));
-  while (mask) {
-    const int from = __ffs(mask) - 1;
-    mask &= mask - 1;
-    const float cv = __shfl_sync(kFull, v, from);
-    const int ci = __shfl_sync(kFull, id, from);
-    if (!better(cv, ci, bar.value, bar.id)) continue;
-    insert(b, cv, ci);
-    bar = bar_of(b, top);
+
+// Calls f(value, id) for the elements of a thread's part of a row.
+template <typename T, int kGroup, typename F>
+__device__ __forceinline__ void each_value(const T* x, int vocab, int part, int parts, F&& f) {
+  constexpr int kVec = 16 / sizeof(T);
+  const int tid = (int)threadIdx.x % kGroup;
+  const RowParts r = row_parts(x, vocab, part, parts);
+  if (part == 0 && tid < r.rest) {
+    const int id = tid < r.front ? tid : r.behind + tid - r.front;
+    const float v[1] = {to_float(x[id])};
+    f(v, id);
+  }
+  const uint4* v = reinterpret_cast<const uint4*>(x + r.front);
+#pragma unroll 4
+  for (int i = r.lo + tid; i < r.hi; i += kGroup) {
+    const uint4 raw = v[i];
+    const T* e = reinterpret_cast<const T*>(&raw);
+    float w[kVec];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) w[j] = to_float(e[j]);
+    f(w, r.front + i * kVec);
   }
 }
-// fp32 in the order of whole numbers, for a maximum over warps
-__device__ __forceinline__ int ordered(float x) {
-  const int b = __float_as_int(x);
-  return b ^ ((b >> 31) & 0x7fffffff);
+
+// The group's best into best[0 .. top), kNoToken where there are no more; `largest`: of this thread's values.  All threads of the group.
+template <typename T, int kGroup>
+__device__ __forceinline__ void choose(const T* x, int vocab, int part, int parts, int top, float largest, TopScratch<kGroup>& s, Best* best) {
+  const int tid = (int)threadIdx.x % kGroup;
+  s.largest[tid] = largest;
+  if (tid == 0) s.count = 0;
+  sync_group<kGroup>();
+  {
+    int before = 0;
+#pragma unroll 8
+    for (int k = 0; k < kGroup; ++k) before += s.largest[k] > largest || (s.largest[k] == largest && k < tid);
+    if (before == top - 1) s.floor = largest;
+  }
+  sync_group<kGroup>();
+  const float floor = s.floor;
+  each_value<T, kGroup>(x, vocab, part, parts, [&](const auto& v, int id) {
+    constexpr int n = sizeof(v) / sizeof(float);
+    float most = v[0];
+#pragma unroll
+    for (int j = 1; j < n; ++j) most = fmaxf(most, v[j]);
+    if (most >= floor && most > -INFINITY) {
+#pragma unroll
+      for (int j = 0; j < n; ++j)
+        if (v[j] >= floor && v[j] > -INFINITY) {
+          const int at = atomicAdd(&s.count, 1);
+          if (at < kRoom) s.found[at] = Best{v[j], id + j};
+        }
+    }
+  });
+  sync_group<kGroup>();
+  const int count = s.count;
+  if (count <= kRoom) {
+    for (int k = tid; k < top; k += kGroup) best[k] = Best{-INFINITY, kNoToken};
+    sync_group<kGroup>();
+    for (int k = tid; k < count; k += kGroup) {
+      const Best mine = s.found[k];
+      int before = 0;
+      for (int o = 0; o < count; ++o) before += better(s.found[o], mine);
+      if (before < top) best[before] = mine;
+    }
+    sync_group<kGroup>();
+    return;
+  }
+  // Too many of one value: one alternative after the other, each the best behind the one before.
+  Best last{INFINITY, -1};
+  for (int k = 0; k < top; ++k) {
+    Best mine{-INFINITY, kNoToken};
+    each_value<T, kGroup>(x, vocab, part, parts, [&](const auto& v, int id) {
+      constexpr int n = sizeof(v) / sizeof(float);
+#pragma unroll
+      for (int j = 0; j < n; ++j) {
+        const Best c{v[j], id + j};
+        if (v[j] > -INFINITY && better(last, c) && better(c, mine)) mine = c;
+      }
+    });
+    s.found[tid] = mine;
+    sync_group<kGroup>();
+    for (int o = 0; o < kGroup; ++o)
+      if (better(s.found[o], mine)) mine = s.found[o];
+    if (tid == 0) best[k] = mine;
+    last = mine;
+    sync_group<kGroup>();
+  }
 }
-__device__ __forceinline__ float unordered(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
 
 // ---- forward ------------------------------------------------------------------------------------
 template <typename T>
@@ -157,9 +247,9 @@ struct ForwardArgs {
   int vocab, top;
 };
 
-// A row's results, from its sums and, lane by lane, its best; by one warp.
+// A row's results, by one warp, from its sums and its best, of which lane k has the k-th.
 template <typename T, bool kTop>
-__device__ __forceinline__ void finish(const ForwardArgs<T>& a, int64_t row, const T* x, int64_t target, const Sums& u, const Best& best) {
+__device__ __forceinline__ void finish(const ForwardArgs<T>& a, int64_t row, const T* x, int64_t target, const Sums& u, Best best) {
   const int lane = (int)threadIdx.x & 31;
   const bool none = u.m == -INFINITY && u.s == 0.f, known = target >= 0 && target < a.vocab;
   const float log_s = log2f(u.s);
@@ -169,10 +259,13 @@ __device__ __forceinline__ void finish(const ForwardArgs<T>& a, int64_t row, con
     return (__fmaf_rn(v, kLog2e, -__fmul_rn(u.m, kLog2e)) - log_s) * kLn2;
   };
   if constexpr (kTop) {
+    // fewer tokens than asked for: the first of those at -inf, which are among the row's first `top`
+    const int found = __popc(__ballot_sync(kFull, lane < a.top && best.id != kNoToken));
+    const unsigned gone = __ballot_sync(kFull, lane < a.top && to_float(x[min(lane, a.vocab - 1)]) == -INFINITY);
+    if (lane >= found && lane < a.top) best = Best{-INFINITY, (int)__fns(gone, 0, lane - found + 1)};
     if (lane < a.top) {
-      const bool there = u.s == u.s && best.id != kNoToken;
-      a.top_values[row * a.top + lane] = u.s == u.s ? (there ? log_prob(best.value) : -INFINITY) : nanf("");
-      a.top_ids[row * a.top + lane] = there ? best.id : -1;
+      a.top_values[row * a.top + lane] = u.s == u.s ? log_prob(best.value) : nanf("");
+      a.top_ids[row * a.top + lane] = u.s == u.s ? best.id : -1;
     }
   }
   if (lane != 0) return;
@@ -198,40 +291,27 @@ __device__ __forceinline__ void finish_ignored(const ForwardArgs<T>& a, int64_t 
   if (a.stats) a.stats[row] = RowStats{0.f, 0.f, 0.f, 0.f};
 }
 
-// Elements in front of the first 16-byte border of a row, and whole vectors behind it.
-template <typename T>
-__device__ __forceinline__ int in_front(const T* x, int vocab) {
-  return min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
-}
-
-// The sums and the best of a part of a row, by a group of threads: `part` of `parts` of its vectors, and with part 0 what lies in front of and behind
-// them.  Four vectors of a thread are under way together.
+// The sums of a part of a row, by a group of threads: with part 0 also of what lies outside its vectors.  Four vectors of a thread are under way
+// together.
 constexpr int kAhead = 4;
-template <typename T, bool kTop, int kGroup>
-__device__ __forceinline__ void scan(const T* x, int vocab, int part, int parts, int top, int* gate, Sums& u, Best& best) {
+template <typename T, int kGroup>
+__device__ __forceinline__ Sums scan(const T* x, int vocab, int part, int parts) {
   constexpr int kVec = 16 / sizeof(T), kN = kVec * kAhead;
   const int tid = (int)threadIdx.x % kGroup;
-  const int front = in_front(x, vocab), vectors = (vocab - front) / kVec;
-  const int lo = (int)((int64_t)vectors * part / parts), hi = (int)((int64_t)vectors * (part + 1) / parts);
-  const uint4* v = reinterpret_cast<const uint4*>(x + front);
-  u = Sums{-INFINITY, 0.f, 0.f};
-  best = Best{-INFINITY, kNoToken};
-  Bar bar{-INFINITY, kNoToken};
-  if (part == 0) {
-    const int behind = front + vectors * kVec, rest = vocab - behind + front;
-    const int id = tid < front ? tid : behind + tid - front;
-    const bool valid = tid < rest;
-    const float one[1] = {valid ? to_float(x[id]) : -INFINITY};
-    add(u, one, one[0]);
-    if constexpr (kTop) offer(best, bar, top, one[0], id, valid);
+  const RowParts r = row_parts(x, vocab, part, parts);
+  const uint4* v = reinterpret_cast<const uint4*>(x + r.front);
+  Sums u{-INFINITY, 0.f, 0.f};
+  if (part == 0 && tid < r.rest) {
+    const float one[1] = {to_float(x[tid < r.front ? tid : r.behind + tid - r.front])};
+    add(u, one, fmaxf(-INFINITY, one[0]));
   }
-  for (int base = lo; base < hi; base += kAhead * kGroup) {
+  for (int base = r.lo + tid; base < r.hi; base += kAhead * kGroup) {
     uint4 raw[kAhead];
     bool in[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      in[k] = base + k * kGroup + tid < hi;
-      if (in[k]) raw[k] = v[base + k * kGroup + tid];
+      in[k] = base + k * kGroup < r.hi;
+      if (in[k]) raw[k] = v[base + k * kGroup];
     }
     float f[kN], largest = -INFINITY;
 #pragma unroll
@@ -244,40 +324,39 @@ __device__ __forceinline__ void scan(const T* x, int vocab, int part, int parts,
       }
     }
     add(u, f, largest);
-    if constexpr (kTop) {
-      // another warp's bar: no value below it is among the row's best
-      const float floor = gate ? unordered(*(volatile int*)gate) : -INFINITY;
-      if (__any_sync(kFull, largest >= fmaxf(bar.value, floor))) {
-#pragma unroll
-        for (int k = 0; k < kN; ++k)
-          offer(best, bar, top, f[k], front + (base + k / kVec * kGroup + tid) * kVec + k % kVec, in[k / kVec] && f[k] >= floor);
-        if (gate && (threadIdx.x & 31) == 0) atomicMax(gate, ordered(bar.value));
-      }
-    }
   }
+  return u;
 }
 
 // A warp for each row.
 template <typename T, bool kTop>
 __global__ void __launch_bounds__(kThreads) forward_short_kernel(const __grid_constant__ ForwardArgs<T> a) {
+  __shared__ TopScratch<32> s_top[kTop ? kWarps : 1];
+  __shared__ Best s_best[kTop ? kWarps : 1][32];
   wait_for_predecessor();
-  const int64_t row = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * kWarps + warp;
   if (row >= a.rows) return;
   const int64_t target = a.targets[row];
   if (target == a.ignored) return finish_ignored<T, kTop>(a, row);
-  Sums u;
-  Best best;
   const T* x = a.x + row * a.stride;
-  scan<T, kTop, 32>(x, a.vocab, 0, 1, a.top, nullptr, u, best);
+  const Sums u = scan<T, 32>(x, a.vocab, 0, 1);
+  Best best{-INFINITY, kNoToken};
+  if constexpr (kTop) {
+    choose<T, 32>(x, a.vocab, 0, 1, a.top, u.m, s_top[warp], s_best[warp]);
+    if (lane < a.top) best = s_best[warp][lane];
+  }
   finish<T, kTop>(a, row, x, target, combine_warp(u), best);
 }
 
 // A block, or a cluster of blocks, for each row.
+constexpr int kMaxParts = 8;
 template <typename T, bool kTop>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ ForwardArgs<T> a, int parts) {
   __shared__ Sums s_sums[kWarps];
-  __shared__ Best s_best[kTop ? kWarps : 1][32];
-  __shared__ int s_gate;
+  __shared__ TopScratch<kTop ? kThreads : 1> s_top;
+  __shared__ Best s_best[kTop ? 32 : 1];
+  __shared__ Best s_all[kTop ? kMaxParts * 32 : 1];
   wait_for_predecessor();
   const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
   const int64_t row = (int64_t)blockIdx.x / parts;
@@ -287,37 +366,46 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
     if (part == 0 && warp == 0) finish_ignored<T, kTop>(a, row);
     return;
   }
-  if constexpr (kTop) {
-    if (threadIdx.x == 0) s_gate = ordered(-INFINITY);
-    __syncthreads();
-  }
-  Sums u;
-  Best best;
   const T* x = a.x + row * a.stride;
-  scan<T, kTop, kThreads>(x, a.vocab, part, parts, a.top, &s_gate, u, best);
+  Sums u = scan<T, kThreads>(x, a.vocab, part, parts);
+  if constexpr (kTop) choose<T, kThreads>(x, a.vocab, part, parts, a.top, u.m, s_top, s_best);
   u = combine_warp(u);
   if (lane == 0) s_sums[warp] = u;
-  if constexpr (kTop) s_best[warp][lane] = best;
   if (parts == 1)
     __syncthreads();
   else
     cg::this_cluster().sync();
-  if (part == 0 && warp == 0) {
-    Bar bar{-INFINITY, kNoToken};
-    if constexpr (kTop) bar = bar_of(best, a.top);
-    for (int p = 0; p < parts; ++p) {
-      const Sums* sums = parts == 1 ? s_sums : cg::this_cluster().map_shared_rank(s_sums, p);
-      const Best* bests = parts == 1 ? &s_best[0][0] : cg::this_cluster().map_shared_rank(&s_best[0][0], p);
-      for (int w = 0; w < kWarps; ++w) {
-        if (p == 0 && w == 0) continue;
-        u = combine(u, sums[w]);
-        if constexpr (kTop) {
-          const Best c = bests[w * 32 + lane];
-          offer(best, bar, a.top, c.value, c.id, lane < a.top && c.id != kNoToken);
-        }
+  if (part == 0) {
+    Best best{-INFINITY, kNoToken};
+    if constexpr (kTop) {
+      if (parts == 1) {
+        if (warp == 0 && lane < a.top) best = s_best[lane];
+      } else {
+        // warp p brings part p's best; each finds its place among all of them
+        Best mine{-INFINITY, kNoToken};
+        if (warp < parts && lane < a.top) mine = cg::this_cluster().map_shared_rank(s_best, warp)[lane];
+        s_all[threadIdx.x] = mine;
+        __syncthreads();
+        int before = 0;
+        for (int p = 0; p < parts; ++p)
+          for (int k = 0; k < a.top; ++k) before += better(s_all[p * 32 + k], mine);
+        __syncthreads();
+        if (threadIdx.x < 32) s_all[threadIdx.x] = Best{-INFINITY, kNoToken};
+        __syncthreads();
+        if (mine.id != kNoToken && before < a.top) s_all[before] = mine;
+        __syncthreads();
+        if (warp == 0 && lane < a.top) best = s_all[lane];
       }
     }
-    finish<T, kTop>(a, row, x, target, u, best);
+    if (warp == 0) {
+      // the sums of up to 64 warps, in the same tree whatever their number
+      Sums all{-INFINITY, 0.f, 0.f};
+      for (int k = lane; k < parts * kWarps; k += 32) {
+        const Sums* from = parts == 1 ? s_sums : cg::this_cluster().map_shared_rank(s_sums, k / kWarps);
+        all = combine(all, from[k % kWarps]);
+      }
+      finish<T, kTop>(a, row, x, target, combine_warp(all), best);
+    }
   }
   if (parts > 1) cg::this_cluster().sync();  // a block's shared memory is read by the first
 }
@@ -348,12 +436,11 @@ __device__ __forceinline__ void backward_part(const BackwardArgs<T>& g, int64_t 
   const int tid = (int)threadIdx.x % kGroup;
   const T* x = g.x + row * g.stride;
   T* dx = g.dx + row * g.dx_stride;
-  const int front = in_front(x, g.vocab), vectors = (g.vocab - front) / kVec;
-  const int lo = (int)((int64_t)vectors * part / parts), hi = (int)((int64_t)vectors * (part + 1) / parts);
+  const RowParts r = row_parts(x, g.vocab, part, parts);
+  const int front = r.front, lo = r.lo, hi = r.hi, rest = r.rest;
   const uint4* v = reinterpret_cast<const uint4*>(x + front);
   uint4* dv = reinterpret_cast<uint4*>(dx + front);
-  const int behind = front + vectors * kVec, rest = g.vocab - behind + front;
-  const int id = tid < front ? tid : behind + tid - front;  // outside the vectors, with part 0
+  const int id = tid < front ? tid : r.behind + tid - front;  // outside the vectors, with part 0
   const RowStats st = g.stats[row];
   if (st.counts == 0.f) {
     for (int i = lo + tid; i < hi; i += kGroup) dv[i] = make_uint4(0, 0, 0, 0);
@@ -402,7 +489,7 @@ template <typename T>
 int forward_parts(int64_t rows, int64_t vocab) {
   int parts = 1;
   const int64_t vectors = vocab * (int64_t)sizeof(T) / 16;
-  while (parts < 8 && rows * parts < 2 * 148 && vectors / (2 * parts) >= kThreads) parts *= 2;
+  while (parts < kMaxParts && rows * parts < 2 * 148 && vectors / (2 * parts) >= kThreads) parts *= 2;
   return parts;
 }
 
