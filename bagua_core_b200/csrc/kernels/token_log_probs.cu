@@ -563,10 +563,11 @@ __global__ void __launch_bounds__(kThreads) forward_short_kernel(const __grid_co
 
 // A block, or a cluster of 2^shift blocks, for each row.
 constexpr int kMaxParts = 8;
-template <typename T, bool kTop>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ ForwardArgs<T> a, int shift) {
-  __shared__ Sums s_sums[kWarps];
-  __shared__ TopScratch<kThreads> s_top;
+template <typename T, bool kTop, int kGroup>
+__global__ void __launch_bounds__(kGroup) forward_kernel(const __grid_constant__ ForwardArgs<T> a, int shift) {
+  constexpr int kGroupWarps = kGroup / 32;
+  __shared__ Sums s_sums[kGroupWarps];
+  __shared__ TopScratch<kGroup> s_top;
   __shared__ Key s_best[kTop ? 32 : 1], s_all[kTop ? kMaxParts * 32 : 1], s_joined[32];
   wait_for_predecessor();
   const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5, parts = 1 << shift;
@@ -580,13 +581,13 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
     return;
   }
   const RowPart r = row_part(x, a.vocab, part, shift);
-  Sums u = scan<T, kTop, kThreads>(x, r, s_top.step);
+  Sums u = scan<T, kTop, kGroup>(x, r, s_top.step);
   if (shift > 0 && target == a.ignored) {  // all blocks of a cluster
     if (part == 0 && warp == 0) finish_ignored<T, kTop>(a, row);
     return;
   }
   const float at_target = part == 0 && target >= 0 && target < a.vocab ? to_float(x[target]) : 0.f;  // asked for now, needed last
-  if constexpr (kTop) choose<T, kThreads>(x, r, a.top, u.m, s_top, s_best);
+  if constexpr (kTop) choose<T, kGroup>(x, r, a.top, u.m, s_top, s_best);
   u = combine_warp<T>(u);
   if (lane == 0) s_sums[warp] = u;
   if (shift == 0)
@@ -600,10 +601,10 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
         if (warp == 0 && lane < a.top) best = s_best[lane];
       } else {
         // the parts' best, each of which finds its place among all of them
-        for (int p = warp; p < parts; p += kWarps) s_all[p * 32 + lane] = lane < a.top ? cg::this_cluster().map_shared_rank(s_best, p)[lane] : kNoKey;
+        for (int p = warp; p < parts; p += kGroupWarps) s_all[p * 32 + lane] = lane < a.top ? cg::this_cluster().map_shared_rank(s_best, p)[lane] : kNoKey;
         if (threadIdx.x < 32) s_joined[threadIdx.x] = kNoKey;
         __syncthreads();
-        for (int p = warp; p < parts; p += kWarps) {
+        for (int p = warp; p < parts; p += kGroupWarps) {
           const Key mine = s_all[p * 32 + lane];
           int before = 0;
           for (int q = 0; q < parts; ++q)
@@ -619,13 +620,13 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
       // the sums of up to 64 warps
       Sums all{-INFINITY, 0.f, 0.f};
       if (shift == 0) {
-        if (lane < kWarps) all = s_sums[lane];
+        if (lane < kGroupWarps) all = s_sums[lane];
       } else {
         Sums two[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int w = lane + 32 * k;
-          two[k] = w < parts * kWarps ? cg::this_cluster().map_shared_rank(s_sums, w / kWarps)[w % kWarps] : Sums{-INFINITY, 0.f, 0.f};
+          two[k] = w < parts * kGroupWarps ? cg::this_cluster().map_shared_rank(s_sums, w / kGroupWarps)[w % kGroupWarps] : Sums{-INFINITY, 0.f, 0.f};
         }
         all.m = fmaxf(two[0].m, two[1].m);
 #pragma unroll
@@ -746,6 +747,10 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
 
 // Up to so many values, a warp takes a row.
 constexpr int64_t kShort = 1024;
+// Many rows of few bytes go to blocks of half as many threads: more rows are under way, and the blocks' joint steps at a row's end cost less.  us with
+// 128 / 256 threads: 4096 rows of 30522 in bf16 46.5 / 49.1, with 20 alternatives 63 / 79; but 517 such rows 9.6 / 9.0, 2000 of 32003 in
+// fp32 47.9 / 44.0, 2000 of 131072 in bf16 88.2 / 85.9.
+constexpr int64_t kManyRows = 4 * 148, kSmallRow = 64 << 10;
 
 // Blocks of a cluster for a row, as a power of two: enough for two blocks on each SM, as long as each has a vector for every thread.
 template <typename T>
@@ -785,10 +790,12 @@ void launch_forward(const ForwardArgs<T>& a, cudaStream_t s) {
     return;
   }
   const int shift = forward_shift<T>(a.rows, a.vocab);
-  if (shift == 0)
-    launch_overlapped(forward_kernel<T, kTop>, dim3((unsigned)a.rows), dim3(kThreads), s, a, 0);
+  if (shift > 0)
+    launch_clusters(forward_kernel<T, kTop, kThreads>, (int)a.rows, 1 << shift, dim3(kThreads), s, a, shift);
+  else if (a.rows >= kManyRows && (int64_t)a.vocab * (int64_t)sizeof(T) <= kSmallRow)
+    launch_overlapped(forward_kernel<T, kTop, kThreads / 2>, dim3((unsigned)a.rows), dim3(kThreads / 2), s, a, 0);
   else
-    launch_clusters(forward_kernel<T, kTop>, (int)a.rows, 1 << shift, dim3(kThreads), s, a, shift);
+    launch_overlapped(forward_kernel<T, kTop, kThreads>, dim3((unsigned)a.rows), dim3(kThreads), s, a, 0);
 }
 
 }  // namespace
