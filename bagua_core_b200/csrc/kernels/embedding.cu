@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "embedding.h"
 #include "index_report.cuh"
@@ -24,31 +26,63 @@ constexpr int kThreads = 256;
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---- lookup -------------------------------------------------------------------------------------
-// A thread takes eight columns of a row, or, where rows do not lie on 16 bytes, one.
-template <typename Id, typename W, typename O, bool kVec>
+// A thread takes eight columns of a row.  Ids that fit no 16 bytes a row go the other way: a warp takes a row, its lanes pairs of columns or
+// single ones, eight of them under way together (40001 rows of 333 in fp16: 73 us with a thread for each element).
+template <typename Id, typename W, typename O>
 __global__ void __launch_bounds__(kThreads)
     lookup_kernel(const Id* __restrict__ ids, const W* __restrict__ table, int64_t rows, int64_t row_stride, O* __restrict__ out, int64_t n,
-                  int64_t H, int columns, float scale, IndexReport* report) {
+                  int64_t H, int shift, float scale, IndexReport* report) {
   wait_for_predecessor();
-  const int per = kThreads / columns;  // rows of a block
-  const int64_t t = (int64_t)blockIdx.x * per + threadIdx.x / columns;
-  const int64_t c = ((int64_t)blockIdx.y * columns + threadIdx.x % columns) * (kVec ? 8 : 1);
+  const int columns = 1 << shift;  // threads of a row
+  const int64_t t = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> shift;
+  const int64_t c = ((int64_t)blockIdx.y * columns + (threadIdx.x & (columns - 1))) * 8;
   if (t >= n || c >= H) return;
   const int64_t id = (int64_t)ids[t];
   const bool known = id >= 0 && id < rows;
   if (!known && c == 0) report_index(report, encoder_ops::kTokenId, id);
-  if constexpr (kVec) {
-    float f[8];
+  float f[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = nanf("");
-    if (known) {
-      widen8(load8(table + id * row_stride + c), f);
+  for (int k = 0; k < 8; ++k) f[k] = nanf("");
+  if (known) {
+    widen8(load8(table + id * row_stride + c), f);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] *= scale;
+    for (int k = 0; k < 8; ++k) f[k] *= scale;
+  }
+  store8(out + t * H + c, narrow8<O>(f));
+}
+template <typename T, int N>
+struct alignas(N * sizeof(T)) Few {
+  T x[N];
+};
+template <typename Id, typename W, typename O, int kFew>
+__global__ void __launch_bounds__(kThreads)
+    lookup_any_kernel(const Id* __restrict__ ids, const W* __restrict__ table, int64_t rows, int64_t row_stride, O* __restrict__ out, int64_t n,
+                      int64_t H, float scale, IndexReport* report) {
+  wait_for_predecessor();
+  const int lane = (int)threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (t >= n) return;
+  const int64_t id = (int64_t)ids[t];
+  const bool known = id >= 0 && id < rows;
+  if (!known && lane == 0) report_index(report, encoder_ops::kTokenId, id);
+  const W* row = table + (known ? id : 0) * row_stride;
+  constexpr int kAhead = 8;
+  for (int64_t c0 = lane * kFew; c0 < H; c0 += kAhead * 32 * kFew) {
+    Few<W, kFew> w[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t c = c0 + k * 32 * kFew;
+      if (known && c < H) w[k] = *reinterpret_cast<const Few<W, kFew>*>(row + c);
     }
-    store8(out + t * H + c, narrow8<O>(f));
-  } else {
-    out[t * H + c] = from_float<O>(known ? to_float(table[id * row_stride + c]) * scale : nanf(""));
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t c = c0 + k * 32 * kFew;
+      if (c >= H) break;
+      Few<O, kFew> o;
+#pragma unroll
+      for (int e = 0; e < kFew; ++e) o.x[e] = from_float<O>(known ? to_float(w[k].x[e]) * scale : nanf(""));
+      *reinterpret_cast<Few<O, kFew>*>(out + t * H + c) = o;
+    }
   }
 }
 
@@ -65,9 +99,17 @@ struct Keys {
   }
 };
 
-// Number of a lane's key among the equal digits of its warp's keys so far, which `seen` counts.  All lanes of the warp come here.
+// Number of a lane's key among the equal digits of its warp's keys so far, which `seen` counts.  All lanes of the warp come here.  (Equal digits are
+// found bit by bit: the instruction that matches values takes a turn for each different one, 15,700 cycles for 8192 keys where
+// this takes 3,000.)
+template <int kBits>
 __device__ __forceinline__ uint32_t rank_in_warp(uint32_t* seen, uint32_t digit, bool valid) {
-  const uint32_t peers = __match_any_sync(0xffffffffu, valid ? digit : (uint32_t)kDigits);
+  uint32_t peers = __ballot_sync(0xffffffffu, valid);
+#pragma unroll
+  for (int b = 0; b < kBits; ++b) {
+    const uint32_t set = __ballot_sync(0xffffffffu, digit >> b & 1u);
+    peers &= digit >> b & 1u ? set : ~set;
+  }
   const int lane = (int)threadIdx.x & 31;
   const uint32_t before = valid ? seen[digit] : 0u;
   __syncwarp();
@@ -78,11 +120,11 @@ __device__ __forceinline__ uint32_t rank_in_warp(uint32_t* seen, uint32_t digit,
 
 // Sorting in blocks that hand tiles to each other through memory.
 constexpr int kRounds = 8, kTile = kThreads * kRounds, kWarps = kThreads / 32;
-// counts[digit][tile]; `present`: a bit for each row that occurs (first pass only).
+// counts[digit][tile].
 template <typename Id>
 __global__ void __launch_bounds__(kThreads)
     histogram_kernel(const Id* __restrict__ ids, const uint32_t* __restrict__ keys, Keys key, int64_t n, int shift, uint32_t* __restrict__ counts,
-                     int tiles, uint32_t* __restrict__ present) {
+                     int tiles) {
   __shared__ uint32_t s_count[kDigits];
   wait_for_predecessor();
   s_count[threadIdx.x] = 0;
@@ -94,27 +136,32 @@ __global__ void __launch_bounds__(kThreads)
     if (i >= n) break;
     const uint32_t k = keys ? keys[i] : key(ids[i]);
     atomicAdd(&s_count[(k >> shift) & (kDigits - 1)], 1u);
-    if (present && k < key.rows) atomicOr(&present[k / 32], 1u << (k % 32));
   }
   __syncthreads();
   counts[(int64_t)threadIdx.x * tiles + blockIdx.x] = s_count[threadIdx.x];
 }
-constexpr int kScanThreads = 1024;
-// Exclusive sums of n counts, in one block.
+constexpr int kScanThreads = 1024, kScanEach = 16;
+// Exclusive sums of n counts, a multiple of 4 of them on a 16-byte border, in one block.
 __global__ void __launch_bounds__(kScanThreads) scan_kernel(uint32_t* __restrict__ counts, int64_t n) {
   __shared__ uint32_t s_warp[32];
   __shared__ uint32_t s_total;
   wait_for_predecessor();
   const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
   uint32_t carry = 0;
-  for (int64_t base = 0; base < n; base += kScanThreads * 4) {
-    const int64_t i = base + (int64_t)threadIdx.x * 4;
-    uint32_t v[4], sum = 0;
+  for (int64_t base = 0; base < n; base += kScanThreads * kScanEach) {
+    uint4* at = reinterpret_cast<uint4*>(counts + base + (int64_t)threadIdx.x * kScanEach);
+    const int64_t left = (n - base) / 4 - (int64_t)threadIdx.x * (kScanEach / 4);  // vectors
+    uint32_t v[kScanEach], sum = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[k] = i + k < n ? counts[i + k] : 0u;
-      sum += v[k];
+    for (int k = 0; k < kScanEach / 4; ++k) {
+      const uint4 x = k < left ? at[k] : make_uint4(0, 0, 0, 0);
+      v[4 * k] = x.x;
+      v[4 * k + 1] = x.y;
+      v[4 * k + 2] = x.z;
+      v[4 * k + 3] = x.w;
     }
+#pragma unroll
+    for (int k = 0; k < kScanEach; ++k) sum += v[k];
     uint32_t up = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -134,15 +181,29 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(uint32_t* __restrict
       if (lane == 31) s_total = wu;
     }
     __syncthreads();
-    uint32_t at = carry + s_warp[warp] + up - sum;
+    uint32_t before = carry + s_warp[warp] + up - sum;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (i + k < n) counts[i + k] = at;
-      at += v[k];
+    for (int k = 0; k < kScanEach; ++k) {
+      const uint32_t c = v[k];
+      v[k] = before;
+      before += c;
     }
+#pragma unroll
+    for (int k = 0; k < kScanEach / 4; ++k)
+      if (k < left) at[k] = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
     carry += s_total;
     __syncthreads();
   }
+}
+// A bit for each row that occurs, set once: by the first of its sorted tokens.
+__device__ __forceinline__ void mark(uint32_t* present, const uint32_t* keys, int64_t i, uint32_t rows) {
+  const uint32_t k = keys[i];
+  if (k < rows && (i == 0 || keys[i - 1] != k)) atomicOr(&present[k / 32], 1u << (k % 32));
+}
+__global__ void __launch_bounds__(kThreads) mark_kernel(uint32_t* __restrict__ present, const uint32_t* __restrict__ keys, int64_t n, uint32_t rows) {
+  wait_for_predecessor();
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i < n) mark(present, keys, i, rows);
 }
 template <typename Id>
 __global__ void __launch_bounds__(kThreads)
@@ -163,7 +224,7 @@ __global__ void __launch_bounds__(kThreads)
     const bool valid = i < n;
     k[r] = !valid ? 0u : keys ? keys[i] : key(ids[i]);
     p[r] = !valid ? 0u : places ? places[i] : (uint32_t)i;
-    rank[r] = rank_in_warp(s_seen[warp], (k[r] >> shift) & (kDigits - 1), valid);
+    rank[r] = rank_in_warp<8>(s_seen[warp], (k[r] >> shift) & (kDigits - 1), valid);
   }
   __syncthreads();
   {
@@ -185,6 +246,129 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// Sorting in one launch: the blocks of a cluster hold all tokens in their shared memory and hand them to each other there.  A pass counts
+// its digits by warp, makes the counts into places by sums over warps, blocks and digits, puts the block's tokens in their order, and copies
+// them, now neighbours for the most part, to where they belong.  (Stored from where they were, one by one, they took five
+// times as long to get there.)
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortRounds = 8, kSortBlocks = 8;
+constexpr int64_t kSortTokens = (int64_t)kSortBlocks * kSortThreads * kSortRounds;
+constexpr int kSortBits = 9, kSortDigits = 1 << kSortBits;  // of a pass at most: two for up to 2^18 - 1 rows
+struct SortShared {
+  uint32_t seen[kSortWarps][kSortDigits];
+  uint32_t count[kSortDigits], offset[kSortDigits], warp[2][kSortDigits / 32];
+  // of a digit: where the block's tokens begin in the block's order, and how much further they go in everybody's
+  uint32_t own[kSortDigits];
+};
+size_t sort_shared_bytes(int rounds) { return sizeof(SortShared) + (size_t)rounds * kSortThreads * 2 * sizeof(uint2); }
+template <typename Id>
+__global__ void __launch_bounds__(kSortThreads)
+    sort_kernel(const Id* __restrict__ ids, Keys key, int n, int bits, int digit_bits, int rounds, uint32_t* keys_out, uint32_t* places_out,
+                uint32_t* __restrict__ present) {
+  extern __shared__ __align__(16) char s_memory[];
+  SortShared& s = *reinterpret_cast<SortShared*>(s_memory);
+  const int room = rounds * kSortThreads;  // tokens of a block
+  uint2* s_tokens = reinterpret_cast<uint2*>(s_memory + sizeof(SortShared));  // keys and places, of this pass and of the next
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), blocks = (int)cluster.num_blocks();
+  const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int first = warp * rounds * 32 + lane;  // a warp's tokens are neighbours
+  const int held = min(room, n - rank * room);  // may be negative
+  wait_for_predecessor();
+  if (present) {  // marked behind the cluster's next joint step
+    const int64_t words = (key.rows + 31) / 32;
+    for (int64_t i = rank * kSortThreads + tid; i < words; i += blocks * kSortThreads) present[i] = 0;
+  }
+  const int digits = 1 << digit_bits;
+  for (int shift = 0, from = 0; shift < bits; shift += digit_bits, from ^= 1) {
+    uint2* in = s_tokens + from * room;
+    for (int k = tid; k < kSortWarps * digits; k += kSortThreads) s.seen[k >> digit_bits][k & (digits - 1)] = 0;
+    __syncthreads();
+    uint2 token[kSortRounds];
+    uint32_t at[kSortRounds];
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+      if (r >= rounds) break;
+      const int slot = first + r * 32, i = rank * room + slot;
+      token[r] = slot >= held ? make_uint2(0, 0) : shift == 0 ? make_uint2(key(ids[i]), (uint32_t)i) : in[slot];
+    }
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+      if (r >= rounds) break;
+      at[r] = rank_in_warp<kSortBits>(s.seen[warp], (token[r].x >> shift) & (digits - 1), first + r * 32 < held);
+    }
+    __syncthreads();
+    if (tid < digits) {
+      uint32_t sum = 0;
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = s.seen[w][tid];
+        s.seen[w][tid] = sum;
+        sum += c;
+      }
+      s.count[tid] = sum;
+    }
+    cluster.sync();
+    uint32_t before = 0, all = 0, mine = 0, up = 0, own_up = 0;
+    if (tid < digits) {
+#pragma unroll
+      for (int b = 0; b < kSortBlocks; ++b) {
+        const uint32_t c = b < blocks ? cluster.map_shared_rank(s.count, b)[tid] : 0u;
+        before += b < rank ? c : 0u;
+        mine = b == rank ? c : mine;
+        all += c;
+      }
+      up = all;
+      own_up = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, up, o), y = __shfl_up_sync(0xffffffffu, own_up, o);
+        if (lane >= o) {
+          up += x;
+          own_up += y;
+        }
+      }
+      if (lane == 31) {
+        s.warp[0][warp] = up;
+        s.warp[1][warp] = own_up;
+      }
+    }
+    __syncthreads();
+    if (tid < digits) {
+      uint32_t sum = before + up - all, own = own_up - mine;
+#pragma unroll
+      for (int w = 0; w < kSortDigits / 32; ++w) {
+        sum += w < warp ? s.warp[0][w] : 0u;
+        own += w < warp ? s.warp[1][w] : 0u;
+      }
+      s.own[tid] = own;
+      s.offset[tid] = sum - own;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+      if (r >= rounds || first + r * 32 >= held) break;
+      const uint32_t digit = (token[r].x >> shift) & (digits - 1);
+      in[s.own[digit] + s.seen[warp][digit] + at[r]] = token[r];
+    }
+    __syncthreads();
+    const bool last = shift + digit_bits >= bits;
+    for (int slot = tid; slot < held; slot += kSortThreads) {
+      const uint2 t = in[slot];
+      const uint32_t to = (uint32_t)slot + s.offset[(t.x >> shift) & (digits - 1)];
+      if (last) {
+        keys_out[to] = t.x;
+        places_out[to] = t.y;
+      } else {
+        const uint32_t block = to / (uint32_t)room;
+        cluster.map_shared_rank(s_tokens, block)[(from ^ 1) * room + to - block * room] = t;
+      }
+    }
+    cluster.sync();
+  }
+  if (present)
+    for (int slot = tid; slot < held; slot += kSortThreads) mark(present, keys_out, (int64_t)rank * room + slot, (uint32_t)key.rows);
+}
+
 // ---- sums ---------------------------------------------------------------------------------------
 // The sorted tokens are cut into chunks of equal length.  A group of lanes takes a chunk and 8 columns a lane, adds up the rows of
 // equal tokens in their order and writes each sum to its row of the table.  Sums over a border between chunks go to scratch, two rows
@@ -195,7 +379,7 @@ struct SumArgs {
   const uint32_t* present;  // null: rows that do not occur are left alone
   float* partial;
   int64_t n, rows, H, chunks, sum_blocks;
-  int length;   // of a chunk, a multiple of 32
+  int length;   // of a chunk: 8, 16 or a multiple of 32
   int slices;   // of a row's columns
   float scale;
 };
@@ -295,8 +479,9 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ S
     const uint32_t key = mine < hi ? a.keys[mine] : none;
     const uint32_t place = mine < hi ? a.places[mine] : 0u;
     if (!__any_sync(0xffffffffu, key != none)) break;  // the rest has no part
+    const int turn = min(kWidth, a.length);
 #pragma unroll 1
-    for (int j0 = 0; j0 < kWidth; j0 += kAhead) {
+    for (int j0 = 0; j0 < turn; j0 += kAhead) {
       Raw8<D> row[kAhead];
       uint32_t id[kAhead];
 #pragma unroll
@@ -338,16 +523,13 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   const int64_t chunk = blockIdx.x, lo = chunk * a.length, hi = lo + a.length;  // hi < n: the last chunk is not among these
   const uint32_t none = (uint32_t)a.rows, run = a.keys[hi - 1];
   if (run == none || a.keys[hi] != run || (lo > 0 && a.keys[lo - 1] == run && a.keys[lo] == run)) return;
-  // the run's last chunk: a search for the end of its keys
-  int64_t below = hi, above = a.n;  // keys[below] == run, keys[above] != run
-  while (above - below > 1) {
-    const int64_t mid = (below + above) / 2;
-    if (a.keys[mid] == run)
-      below = mid;
-    else
-      above = mid;
+  // the run's last chunk: the last that begins with it
+  int64_t last = chunk;
+  for (int more = kThreads; more == kThreads;) {
+    const int64_t k = last + 1 + threadIdx.x;
+    more = __syncthreads_count(k < a.chunks && a.keys[k * a.length] == run);
+    last += more;
   }
-  const int64_t last = below / a.length;
   const int tx = (int)threadIdx.x % kJoinColumns, ty = (int)threadIdx.x / kJoinColumns;
   const int64_t c0 = (int64_t)blockIdx.y * kJoinColumns * 4 + tx;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -390,7 +572,8 @@ Plan plan(int64_t n, int64_t rows, int64_t H) {
   p.slices = (int)ceil_div(H, p.width * 8);
   // As many chunks as keep every SM's warps busy, as long as a chunk's two rows of scratch are few next to its own.
   const int64_t lanes = (int64_t)148 * 1024, units = std::max<int64_t>(1, lanes / p.width / p.slices);
-  p.length = (int)std::min<int64_t>(1024, std::max<int64_t>(32, ceil_div(ceil_div(n, units), 32) * 32));
+  const int64_t each = ceil_div(n, units);
+  p.length = each <= 8 ? 8 : each <= 16 ? 16 : (int)std::min<int64_t>(1024, ceil_div(each, 32) * 32);
   p.chunks = ceil_div(n, p.length);
   p.sum_blocks = ceil_div(p.chunks * p.slices * p.width, kThreads);
   p.keys = take((size_t)n * 4 * 4);
@@ -406,12 +589,32 @@ int sort(const Ids& ids, Keys key, const Plan& p, uint32_t* buffers, uint32_t* c
   const int64_t n = ids.n;
   int bits = 1;
   while (bits < 32 && (key.rows >> bits) != 0) ++bits;
+  if (n <= kSortTokens) {
+    int blocks = 1;
+    while (blocks < kSortBlocks && (int64_t)blocks * kSortThreads < n) blocks *= 2;
+    const int rounds = (int)ceil_div(n, (int64_t)blocks * kSortThreads);
+    const size_t shared = sort_shared_bytes(rounds);
+    static std::atomic<bool> allowed[64];
+    int device = 0;
+    BAGUA_CUDA_CHECK(cudaGetDevice(&device));
+    if (device >= 64 || !allowed[device].load(std::memory_order_acquire)) {
+      BAGUA_CUDA_CHECK(cudaFuncSetAttribute(sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sort_shared_bytes(kSortRounds)));
+      if (device < 64) allowed[device].store(true, std::memory_order_release);
+    }
+    const int passes = (bits + kSortBits - 1) / kSortBits, digit_bits = std::max(5, (bits + passes - 1) / passes);  // whole warps of digits
+    launch_clusters_shared(sort_kernel<Id>, 1, blocks, dim3(kSortThreads), shared, s, (const Id*)ids.data, key, (int)n, bits, digit_bits, rounds,
+                           buffers, buffers + n, present);
+    *keys = buffers;
+    *places = buffers + n;
+    return 1;
+  }
+  if (present) BAGUA_CUDA_CHECK(cudaMemsetAsync(present, 0, (size_t)ceil_div(key.rows, 32) * 4, s));
   uint32_t* k[2] = {buffers, buffers + 2 * n};
   const uint32_t *in_k = nullptr, *in_p = nullptr;
   int launches = 0, to = 0;
   for (int shift = 0; shift < bits; shift += 8, to ^= 1) {
     launch_overlapped(histogram_kernel<Id>, dim3((unsigned)p.tiles), dim3(kThreads), s, (const Id*)ids.data, in_k, key, n, shift, counts,
-                      (int)p.tiles, shift == 0 ? present : nullptr);
+                      (int)p.tiles);
     launch_overlapped(scan_kernel, dim3(1), dim3(kScanThreads), s, counts, p.tiles * kDigits);
     launch_overlapped(scatter_kernel<Id>, dim3((unsigned)p.tiles), dim3(kThreads), s, (const Id*)ids.data, in_k, in_p, key, n, shift, counts,
                       (int)p.tiles, k[to], k[to] + n);
@@ -421,7 +624,9 @@ int sort(const Ids& ids, Keys key, const Plan& p, uint32_t* buffers, uint32_t* c
   }
   *keys = in_k;
   *places = in_p;
-  return launches;
+  if (!present) return launches;
+  launch_overlapped(mark_kernel, dim3((unsigned)ceil_div(n, kThreads)), dim3(kThreads), s, present, in_k, n, (uint32_t)key.rows);
+  return launches + 1;
 }
 
 template <typename D, typename W>
@@ -459,15 +664,24 @@ void lookup(const Ids& ids, const void* table, DType table_type, int64_t rows, i
       using O = std::remove_pointer_t<decltype(o)>;
       auto go = [&](auto* id) {
         using Id = std::remove_pointer_t<decltype(id)>;
-        const bool vec = H % 8 == 0 && ((uintptr_t)table | (uintptr_t)out | (uintptr_t)(row_stride * (int64_t)sizeof(W))) % 16 == 0;
-        const int64_t wide = ceil_div(H, vec ? 8 : 1);
-        int columns = 1;
-        while (columns < kThreads && columns < wide) columns *= 2;
-        const int64_t slices = ceil_div(wide, columns);
-        BAGUA_CHECK(slices < 65536, Tensor, "embedding: " << H << " columns");
-        const dim3 grid((unsigned)ceil_div(ids.n, kThreads / columns), (unsigned)slices);
-        launch_overlapped(vec ? lookup_kernel<Id, W, O, true> : lookup_kernel<Id, W, O, false>, grid, dim3(kThreads), s, (const Id*)ids.data,
-                          (const W*)table, rows, row_stride, (O*)out, ids.n, H, columns, scale, encoder_ops::index_report());
+        // whether runs of so many elements start on multiples of their size, up to 16 bytes, in every row
+        auto fits = [&](int64_t e) {
+          const int64_t w = std::min<int64_t>(16, e * (int64_t)sizeof(W)), o = std::min<int64_t>(16, e * (int64_t)sizeof(O));
+          return H % e == 0 && (int64_t)((uintptr_t)table % w) == 0 && row_stride * (int64_t)sizeof(W) % w == 0 && (int64_t)((uintptr_t)out % o) == 0;
+        };
+        if (fits(8)) {
+          int shift = 0;
+          while ((1 << shift) < kThreads && (1 << shift) < H / 8) ++shift;
+          const int64_t slices = ceil_div(H / 8, 1 << shift);
+          BAGUA_CHECK(slices < 65536, Tensor, "embedding: " << H << " columns");
+          const dim3 grid((unsigned)ceil_div(ids.n, kThreads >> shift), (unsigned)slices);
+          launch_overlapped(lookup_kernel<Id, W, O>, grid, dim3(kThreads), s, (const Id*)ids.data, (const W*)table, rows, row_stride, (O*)out, ids.n,
+                            H, shift, scale, encoder_ops::index_report());
+        } else {
+          launch_overlapped(fits(2) ? lookup_any_kernel<Id, W, O, 2> : lookup_any_kernel<Id, W, O, 1>, dim3((unsigned)ceil_div(ids.n, kThreads / 32)),
+                            dim3(kThreads), s, (const Id*)ids.data, (const W*)table, rows, row_stride, (O*)out, ids.n, H, scale,
+                            encoder_ops::index_report());
+        }
       };
       ids.wide ? go((int64_t*)nullptr) : go((int32_t*)nullptr);
     });
@@ -486,7 +700,6 @@ int backward(const Ids& ids, const void* dout, DType dout_type, int64_t rows, in
               "embedding backward: " << rows << " rows of " << H << " columns");
   auto at = [&](size_t offset) { return (uint32_t*)((char*)scratch + offset); };
   uint32_t* present = accumulate ? nullptr : at(p.present);
-  if (present) BAGUA_CUDA_CHECK(cudaMemsetAsync(present, 0, (size_t)ceil_div(rows, 32) * 4, s));
   SumArgs a{};
   const Keys key{rows, padding};
   int launches = ids.wide ? sort<int64_t>(ids, key, p, at(p.keys), at(p.counts), present, &a.keys, &a.places, s)

@@ -41,7 +41,7 @@ inline void launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, cudaS
 // `clusters` clusters of `blocks` blocks each, which may start while the kernel in front of them ends.  More than 8 blocks need
 // cudaFuncAttributeNonPortableClusterSizeAllowed.
 template <typename... P, typename... A>
-inline void launch_clusters(void (*kernel)(P...), int clusters, int blocks, dim3 block, cudaStream_t s, A... args) {
+inline void launch_clusters_shared(void (*kernel)(P...), int clusters, int blocks, dim3 block, size_t shared, cudaStream_t s, A... args) {
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -51,10 +51,15 @@ inline void launch_clusters(void (*kernel)(P...), int clusters, int blocks, dim3
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(clusters * blocks));
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = shared;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   BAGUA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+}
+template <typename... P, typename... A>
+inline void launch_clusters(void (*kernel)(P...), int clusters, int blocks, dim3 block, cudaStream_t s, A... args) {
+  launch_clusters_shared(kernel, clusters, blocks, block, 0, s, args...);
 }
 
 // All blocks of the grid are resident together, or the launch fails.
