@@ -26,29 +26,39 @@ constexpr int kThreads = 256;
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---- lookup -------------------------------------------------------------------------------------
-// A thread takes eight columns of a row.  Ids that fit no 16 bytes a row go the other way: a warp takes a row, its lanes pairs of columns or
+// A thread takes eight columns of a row, or of four rows, whose loads wait for their ids together, where enough threads are left.  Rows that fit no 16 bytes a row go the other way: a warp takes a row, its lanes pairs of columns or
 // single ones, eight of them under way together (40001 rows of 333 in fp16: 73 us with a thread for each element).
-template <typename Id, typename W, typename O>
+constexpr int kRowsAhead = 4;
+constexpr int64_t kManyElements = 148ll * 2048 * 8 * kRowsAhead;
+template <typename Id, typename W, typename O, int kRows>
 __global__ void __launch_bounds__(kThreads)
     lookup_kernel(const Id* __restrict__ ids, const W* __restrict__ table, int64_t rows, int64_t row_stride, O* __restrict__ out, int64_t n,
                   int64_t H, int shift, float scale, IndexReport* report) {
   wait_for_predecessor();
   const int columns = 1 << shift;  // threads of a row
-  const int64_t t = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> shift;
+  const int per = kThreads >> shift;
+  const int64_t t0 = (int64_t)blockIdx.x * per * kRows + (threadIdx.x >> shift);
   const int64_t c = ((int64_t)blockIdx.y * columns + (threadIdx.x & (columns - 1))) * 8;
-  if (t >= n || c >= H) return;
-  const int64_t id = (int64_t)ids[t];
-  const bool known = id >= 0 && id < rows;
-  if (!known && c == 0) report_index(report, encoder_ops::kTokenId, id);
-  float f[8];
+  if (c >= H) return;
+  int64_t id[kRows];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) f[k] = nanf("");
-  if (known) {
-    widen8(load8(table + id * row_stride + c), f);
+  for (int k = 0; k < kRows; ++k) id[k] = t0 + k * per < n ? (int64_t)ids[t0 + k * per] : 0;
+  Raw8<W> raw[kRows];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] *= scale;
+  for (int k = 0; k < kRows; ++k)
+    if (t0 + k * per < n && id[k] >= 0 && id[k] < rows) raw[k] = load8(table + id[k] * row_stride + c);
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    const int64_t t = t0 + k * per;
+    if (t >= n) break;
+    const bool known = id[k] >= 0 && id[k] < rows;
+    if (!known && c == 0) report_index(report, encoder_ops::kTokenId, id[k]);
+    float f[8];
+    widen8(raw[k], f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = known ? f[e] * scale : nanf("");
+    store8(out + t * H + c, narrow8<O>(f));
   }
-  store8(out + t * H + c, narrow8<O>(f));
 }
 template <typename T, int N>
 struct alignas(N * sizeof(T)) Few {
@@ -84,6 +94,30 @@ __global__ void __launch_bounds__(kThreads)
       *reinterpret_cast<Few<O, kFew>*>(out + t * H + c) = o;
     }
   }
+}
+
+// ---- clearing -----------------------------------------------------------------------------------
+// The gradient's rows that no token names are zero.  Sorting keeps few blocks busy: its kernel lets this one start at once, which clears the
+// whole gradient meanwhile, and the rows that do occur are written again later.  Nothing is read here, and what was queued before the
+// sort has finished when it lets go, so that no block waits but the first, at its end: by that this kernel ends behind the sort, and what
+// follows it may rely on both.  (Cleared by the launch that writes the sums instead, and of rows that do not occur alone, 12288 tokens of
+// 30522 x 1024 took 67 us.)
+constexpr int kClearVecs = 4;
+constexpr int64_t kClearBytes = (int64_t)kThreads * kClearVecs * 16;  // of a block
+__global__ void __launch_bounds__(kThreads) clear_kernel(char* __restrict__ at, int64_t bytes) {  // `at` lies on 16 bytes
+  const int64_t base = (int64_t)blockIdx.x * kClearBytes;
+#pragma unroll
+  for (int k = 0; k < kClearVecs; ++k) {
+    const int64_t i = base + ((int64_t)k * kThreads + threadIdx.x) * 16;
+    if (i + 16 <= bytes) *reinterpret_cast<uint4*>(at + i) = make_uint4(0, 0, 0, 0);
+  }
+  if (blockIdx.x > 0) return;
+  const int64_t tail = bytes / 16 * 16;
+  if (threadIdx.x < bytes - tail) at[tail + threadIdx.x] = 0;
+  wait_for_predecessor();
+}
+void clear(void* at, int64_t bytes, cudaStream_t s) {
+  launch_overlapped(clear_kernel, dim3((unsigned)((bytes + kClearBytes - 1) / kClearBytes)), dim3(kThreads), s, (char*)at, bytes);
 }
 
 // ---- sorting ------------------------------------------------------------------------------------
@@ -142,10 +176,13 @@ __global__ void __launch_bounds__(kThreads)
 }
 constexpr int kScanThreads = 1024, kScanEach = 16;
 // Exclusive sums of n counts, a multiple of 4 of them on a 16-byte border, in one block.
-__global__ void __launch_bounds__(kScanThreads) scan_kernel(uint32_t* __restrict__ counts, int64_t n) {
+// Lets its successor start at once, and sets `zero` to 0.
+__global__ void __launch_bounds__(kScanThreads) scan_kernel(uint32_t* __restrict__ counts, int64_t n, uint32_t* __restrict__ zero) {
   __shared__ uint32_t s_warp[32];
   __shared__ uint32_t s_total;
   wait_for_predecessor();
+  let_successor_start();
+  if (threadIdx.x == 0) *zero = 0;
   const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
   uint32_t carry = 0;
   for (int64_t base = 0; base < n; base += kScanThreads * kScanEach) {
@@ -195,16 +232,6 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(uint32_t* __restrict
     __syncthreads();
   }
 }
-// A bit for each row that occurs, set once: by the first of its sorted tokens.
-__device__ __forceinline__ void mark(uint32_t* present, const uint32_t* keys, int64_t i, uint32_t rows) {
-  const uint32_t k = keys[i];
-  if (k < rows && (i == 0 || keys[i - 1] != k)) atomicOr(&present[k / 32], 1u << (k % 32));
-}
-__global__ void __launch_bounds__(kThreads) mark_kernel(uint32_t* __restrict__ present, const uint32_t* __restrict__ keys, int64_t n, uint32_t rows) {
-  wait_for_predecessor();
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i < n) mark(present, keys, i, rows);
-}
 template <typename Id>
 __global__ void __launch_bounds__(kThreads)
     scatter_kernel(const Id* __restrict__ ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ places, Keys key, int64_t n,
@@ -246,7 +273,7 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Sorting in one launch: the blocks of a cluster hold all tokens in their shared memory and hand them to each other there.  A pass counts
+// Sorting in one launch, which lets its successor start at once: the blocks of a cluster hold all tokens in their shared memory and hand them to each other there.  A pass counts
 // its digits by warp, makes the counts into places by sums over warps, blocks and digits, puts the block's tokens in their order, and copies
 // them, now neighbours for the most part, to where they belong.  (Stored from where they were, one by one, they took five
 // times as long to get there.)
@@ -262,8 +289,8 @@ struct SortShared {
 size_t sort_shared_bytes(int rounds) { return sizeof(SortShared) + (size_t)rounds * kSortThreads * 2 * sizeof(uint2); }
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads)
-    sort_kernel(const Id* __restrict__ ids, Keys key, int n, int bits, int digit_bits, int rounds, uint32_t* keys_out, uint32_t* places_out,
-                uint32_t* __restrict__ present) {
+    sort_kernel(const Id* __restrict__ ids, Keys key, int n, int bits, int digit_bits, int rounds, uint32_t* __restrict__ keys_out,
+                uint32_t* __restrict__ places_out, uint32_t* __restrict__ zero) {
   extern __shared__ __align__(16) char s_memory[];
   SortShared& s = *reinterpret_cast<SortShared*>(s_memory);
   const int room = rounds * kSortThreads;  // tokens of a block
@@ -274,10 +301,8 @@ __global__ void __launch_bounds__(kSortThreads)
   const int first = warp * rounds * 32 + lane;  // a warp's tokens are neighbours
   const int held = min(room, n - rank * room);  // may be negative
   wait_for_predecessor();
-  if (present) {  // marked behind the cluster's next joint step
-    const int64_t words = (key.rows + 31) / 32;
-    for (int64_t i = rank * kSortThreads + tid; i < words; i += blocks * kSortThreads) present[i] = 0;
-  }
+  let_successor_start();
+  if (rank == 0 && tid == 0) *zero = 0;
   const int digits = 1 << digit_bits;
   for (int shift = 0, from = 0; shift < bits; shift += digit_bits, from ^= 1) {
     uint2* in = s_tokens + from * room;
@@ -365,23 +390,21 @@ __global__ void __launch_bounds__(kSortThreads)
     }
     cluster.sync();
   }
-  if (present)
-    for (int slot = tid; slot < held; slot += kSortThreads) mark(present, keys_out, (int64_t)rank * room + slot, (uint32_t)key.rows);
 }
 
 // ---- sums ---------------------------------------------------------------------------------------
 // The sorted tokens are cut into chunks of equal length.  A group of lanes takes a chunk and 8 columns a lane, adds up the rows of
 // equal tokens in their order and writes each sum to its row of the table.  Sums over a border between chunks go to scratch, two rows
-// a chunk (of the run that comes in, of the run that goes out), and join_kernel adds those up in the chunks' order.  In the same
-// launch, further warps clear the rows that do not occur.
+// a chunk (of the run that comes in, of the run that goes out), and join_kernel adds those up in the chunks' order.
 struct SumArgs {
   const uint32_t *keys, *places;
-  const uint32_t* present;  // null: rows that do not occur are left alone
+  uint32_t *runs, *run_count;  // first chunks of the runs that go over a border
   float* partial;
-  int64_t n, rows, H, chunks, sum_blocks;
+  int64_t n, rows, H, chunks;
   int length;   // of a chunk: 8, 16 or a multiple of 32
   int slices;   // of a row's columns
   float scale;
+  bool accumulate;  // sums are added to what the rows hold
 };
 
 // The column of element k of a lane that stands at `lane` in a slice of `width` lanes.
@@ -432,24 +455,11 @@ __device__ __forceinline__ void finish_row(T* row, float (&f)[8], float scale, b
   store_row<T, kVec>(row, f, slice, lane, width, H);
 }
 
+constexpr int kSumBlocks = 3;  // resident on an SM
 template <typename D, typename W, bool kVec, int kWidth>
-__global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ SumArgs a, const D* __restrict__ dout, W* __restrict__ dtable) {
+__global__ void __launch_bounds__(kThreads, kSumBlocks) sum_kernel(const __grid_constant__ SumArgs a, const D* __restrict__ dout, W* __restrict__ dtable) {
   wait_for_predecessor();
   const int warp_lane = (int)threadIdx.x & 31;
-  if (blockIdx.x >= a.sum_blocks) {  // rows that do not occur, 32 to a warp
-    const int64_t unit = (int64_t)(blockIdx.x - a.sum_blocks) * (kThreads / 32) + (threadIdx.x >> 5);
-    const int64_t word = unit / a.slices;
-    const int slice = (int)(unit % a.slices);
-    if (word * 32 >= a.rows) return;
-    const int64_t left = a.rows - word * 32;
-    uint32_t absent = ~a.present[word] & (left >= 32 ? 0xffffffffu : (1u << left) - 1u);
-    constexpr int groups = 32 / kWidth;
-    const int lane = warp_lane % kWidth, group = warp_lane / kWidth;
-    const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int r = group; r < 32; r += groups)
-      if (absent >> r & 1u) store_row<W, kVec>(dtable + (word * 32 + r) * a.H, zero, slice, lane, kWidth, a.H);
-    return;
-  }
   const int64_t unit = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kWidth;
   const int lane = warp_lane % kWidth;
   const int64_t chunk = unit / a.slices;
@@ -467,29 +477,43 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ S
   auto flush = [&](bool last) {
     if (run == none) return;
     const bool in = first && run == before, out = last && run == behind;
-    if (in || out)
+    if (in || out) {
       store_row<float, kVec>(a.partial + (2 * chunk + (in ? 0 : 1)) * a.H, acc, slice, lane, kWidth, a.H);
-    else
-      finish_row<W, kVec>(dtable + (int64_t)run * a.H, acc, a.scale, a.present == nullptr, slice, lane, kWidth, a.H);
+      if (!in && slice == 0 && lane == 0) a.runs[atomicAdd(a.run_count, 1u)] = (uint32_t)chunk;
+    } else
+      finish_row<W, kVec>(dtable + (int64_t)run * a.H, acc, a.scale, a.accumulate, slice, lane, kWidth, a.H);
   };
-  constexpr int kAhead = 8 / (sizeof(D) / 2) < 4 ? 4 : 8 / (sizeof(D) / 2);  // rows on their way
+  constexpr int kAhead = 4;  // rows that are added while as many are on their way
+  const int turn = min(kWidth, a.length);
+  uint32_t next_key = lo + lane < hi ? a.keys[lo + lane] : none, next_place = lo + lane < hi ? a.places[lo + lane] : 0u;
   for (int64_t base = lo; __any_sync(0xffffffffu, base < hi); base += kWidth) {
-    // tokens of this turn, one a lane
-    const int64_t mine = base + lane;
-    const uint32_t key = mine < hi ? a.keys[mine] : none;
-    const uint32_t place = mine < hi ? a.places[mine] : 0u;
+    // tokens of this turn, one a lane, and of the next
+    const uint32_t key = next_key, place = next_place;
     if (!__any_sync(0xffffffffu, key != none)) break;  // the rest has no part
-    const int turn = min(kWidth, a.length);
+    const int64_t mine = base + kWidth + lane;
+    next_key = mine < hi ? a.keys[mine] : none;
+    next_place = mine < hi ? a.places[mine] : 0u;
+    Raw8<D> next[kAhead];
+    uint32_t next_id[kAhead];
+    auto load = [&](int j0) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        next_id[j] = __shfl_sync(0xffffffffu, key, j0 + j, kWidth);
+        const uint32_t p = __shfl_sync(0xffffffffu, place, j0 + j, kWidth);
+        if (next_id[j] != none) next[j] = load_row<D, kVec>(dout + (int64_t)p * a.H, slice, lane, kWidth, a.H);
+      }
+    };
+    load(0);
 #pragma unroll 1
     for (int j0 = 0; j0 < turn; j0 += kAhead) {
       Raw8<D> row[kAhead];
       uint32_t id[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        id[j] = __shfl_sync(0xffffffffu, key, j0 + j, kWidth);
-        const uint32_t p = __shfl_sync(0xffffffffu, place, j0 + j, kWidth);
-        if (id[j] != none) row[j] = load_row<D, kVec>(dout + (int64_t)p * a.H, slice, lane, kWidth, a.H);
+        row[j] = next[j];
+        id[j] = next_id[j];
       }
+      if (j0 + kAhead < turn) load(j0 + kAhead);
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         if (id[j] == none) continue;
@@ -514,53 +538,56 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ S
 }
 
 // Sums over borders: a block takes a run that leaves its first chunk, and 128 columns; its 8 rows of threads add up every eighth chunk's
-// part each.
+// part each.  The runs are listed in any order, each is added up in the chunks' order.
 constexpr int kJoinColumns = 32, kJoinRows = kThreads / kJoinColumns;
 template <typename W>
 __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ SumArgs a, W* __restrict__ dtable) {
   __shared__ float s_acc[kJoinRows][kJoinColumns * 4];
   wait_for_predecessor();
-  const int64_t chunk = blockIdx.x, lo = chunk * a.length, hi = lo + a.length;  // hi < n: the last chunk is not among these
-  const uint32_t none = (uint32_t)a.rows, run = a.keys[hi - 1];
-  if (run == none || a.keys[hi] != run || (lo > 0 && a.keys[lo - 1] == run && a.keys[lo] == run)) return;
-  // the run's last chunk: the last that begins with it
-  int64_t last = chunk;
-  for (int more = kThreads; more == kThreads;) {
-    const int64_t k = last + 1 + threadIdx.x;
-    more = __syncthreads_count(k < a.chunks && a.keys[k * a.length] == run);
-    last += more;
-  }
+  const int64_t slices = (a.H + kJoinColumns * 4 - 1) / (kJoinColumns * 4), items = *a.run_count * slices;
   const int tx = (int)threadIdx.x % kJoinColumns, ty = (int)threadIdx.x / kJoinColumns;
-  const int64_t c0 = (int64_t)blockIdx.y * kJoinColumns * 4 + tx;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t chunk = a.runs[item / slices], slice = item % slices;
+    const uint32_t run = a.keys[chunk * a.length + a.length - 1];
+    // the run's last chunk: the last that begins with it
+    int64_t last = chunk;
+    for (int more = kThreads; more == kThreads;) {
+      const int64_t k = last + 1 + threadIdx.x;
+      more = __syncthreads_count(k < a.chunks && a.keys[k * a.length] == run);
+      last += more;
+    }
+    const int64_t c0 = slice * kJoinColumns * 4 + tx;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int64_t k = chunk + ty; k <= last; k += kJoinRows) {
-    const float* row = a.partial + (2 * k + (k == chunk ? 1 : 0)) * a.H;
+    for (int64_t k = chunk + ty; k <= last; k += kJoinRows) {
+      const float* row = a.partial + (2 * k + (k == chunk ? 1 : 0)) * a.H;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (c0 + e * kJoinColumns < a.H) acc[e] += row[c0 + e * kJoinColumns];
+      for (int e = 0; e < 4; ++e)
+        if (c0 + e * kJoinColumns < a.H) acc[e] += row[c0 + e * kJoinColumns];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s_acc[ty][e * kJoinColumns + tx] = acc[e];
+    __syncthreads();
+    const int64_t c = slice * kJoinColumns * 4 + threadIdx.x;
+    if (threadIdx.x < kJoinColumns * 4 && c < a.H) {
+      float s = 0.f;
+#pragma unroll
+      for (int r = 0; r < kJoinRows; ++r) s += s_acc[r][threadIdx.x];
+      W* out = dtable + (int64_t)run * a.H + c;
+      s *= a.scale;
+      *out = from_float<W>(a.accumulate ? s + to_float(*out) : s);
+    }
+    __syncthreads();
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) s_acc[ty][e * kJoinColumns + tx] = acc[e];
-  __syncthreads();
-  if (threadIdx.x >= kJoinColumns * 4) return;
-  const int64_t c = (int64_t)blockIdx.y * kJoinColumns * 4 + threadIdx.x;
-  if (c >= a.H) return;
-  float s = 0.f;
-#pragma unroll
-  for (int r = 0; r < kJoinRows; ++r) s += s_acc[r][threadIdx.x];
-  W* out = dtable + (int64_t)run * a.H + c;
-  s *= a.scale;
-  *out = from_float<W>(a.present ? s : s + to_float(*out));
 }
 
 // ---- plans --------------------------------------------------------------------------------------
 struct Plan {
   int64_t tiles, chunks, sum_blocks;
   int length, slices, width;
-  size_t keys, counts, present, partial, bytes;  // offsets into the scratch
+  size_t keys, counts, runs, partial, bytes;  // offsets into the scratch
 };
-Plan plan(int64_t n, int64_t rows, int64_t H) {
+Plan plan(int64_t n, int64_t H) {
   Plan p{};
   auto take = [&p](size_t bytes) {
     const size_t at = p.bytes;
@@ -570,21 +597,21 @@ Plan plan(int64_t n, int64_t rows, int64_t H) {
   p.tiles = ceil_div(n, kTile);
   p.width = H > 128 ? 32 : H > 64 ? 16 : 8;
   p.slices = (int)ceil_div(H, p.width * 8);
-  // As many chunks as keep every SM's warps busy, as long as a chunk's two rows of scratch are few next to its own.
-  const int64_t lanes = (int64_t)148 * 1024, units = std::max<int64_t>(1, lanes / p.width / p.slices);
+  // As many chunks as the SMs hold at once: with more of them a second wave comes, and more runs go over borders.
+  const int64_t lanes = (int64_t)148 * kSumBlocks * kThreads, units = std::max<int64_t>(1, lanes / p.width / p.slices);
   const int64_t each = ceil_div(n, units);
   p.length = each <= 8 ? 8 : each <= 16 ? 16 : (int)std::min<int64_t>(1024, ceil_div(each, 32) * 32);
   p.chunks = ceil_div(n, p.length);
   p.sum_blocks = ceil_div(p.chunks * p.slices * p.width, kThreads);
   p.keys = take((size_t)n * 4 * 4);
   p.counts = take((size_t)p.tiles * kDigits * 4);
-  p.present = take((size_t)ceil_div(rows, 32) * 4);
+  p.runs = take((size_t)(p.chunks + 1) * 4);
   p.partial = take((size_t)p.chunks * 2 * H * 4);
   return p;
 }
 
 template <typename Id>
-int sort(const Ids& ids, Keys key, const Plan& p, uint32_t* buffers, uint32_t* counts, uint32_t* present, const uint32_t** keys,
+int sort(const Ids& ids, Keys key, const Plan& p, uint32_t* buffers, uint32_t* counts, uint32_t* zero, void* clear_at, int64_t clear_bytes, const uint32_t** keys,
          const uint32_t** places, cudaStream_t s) {
   const int64_t n = ids.n;
   int bits = 1;
@@ -602,20 +629,21 @@ int sort(const Ids& ids, Keys key, const Plan& p, uint32_t* buffers, uint32_t* c
       if (device < 64) allowed[device].store(true, std::memory_order_release);
     }
     const int passes = (bits + kSortBits - 1) / kSortBits, digit_bits = std::max(5, (bits + passes - 1) / passes);  // whole warps of digits
-    launch_clusters_shared(sort_kernel<Id>, 1, blocks, dim3(kSortThreads), shared, s, (const Id*)ids.data, key, (int)n, bits, digit_bits, rounds,
-                           buffers, buffers + n, present);
+    launch_clusters_shared(sort_kernel<Id>, 1, blocks, dim3(kSortThreads), shared, s, (const Id*)ids.data, key, (int)n, bits,
+                           digit_bits, rounds, buffers, buffers + n, zero);
+    if (clear_at) clear(clear_at, clear_bytes, s);
     *keys = buffers;
     *places = buffers + n;
-    return 1;
+    return clear_at ? 2 : 1;
   }
-  if (present) BAGUA_CUDA_CHECK(cudaMemsetAsync(present, 0, (size_t)ceil_div(key.rows, 32) * 4, s));
   uint32_t* k[2] = {buffers, buffers + 2 * n};
   const uint32_t *in_k = nullptr, *in_p = nullptr;
   int launches = 0, to = 0;
   for (int shift = 0; shift < bits; shift += 8, to ^= 1) {
     launch_overlapped(histogram_kernel<Id>, dim3((unsigned)p.tiles), dim3(kThreads), s, (const Id*)ids.data, in_k, key, n, shift, counts,
                       (int)p.tiles);
-    launch_overlapped(scan_kernel, dim3(1), dim3(kScanThreads), s, counts, p.tiles * kDigits);
+    launch_overlapped(scan_kernel, dim3(1), dim3(kScanThreads), s, counts, p.tiles * kDigits, zero);
+    if (clear_at && shift == 0) clear(clear_at, clear_bytes, s);
     launch_overlapped(scatter_kernel<Id>, dim3((unsigned)p.tiles), dim3(kThreads), s, (const Id*)ids.data, in_k, in_p, key, n, shift, counts,
                       (int)p.tiles, k[to], k[to] + n);
     in_k = k[to];
@@ -624,23 +652,22 @@ int sort(const Ids& ids, Keys key, const Plan& p, uint32_t* buffers, uint32_t* c
   }
   *keys = in_k;
   *places = in_p;
-  if (!present) return launches;
-  launch_overlapped(mark_kernel, dim3((unsigned)ceil_div(n, kThreads)), dim3(kThreads), s, present, in_k, n, (uint32_t)key.rows);
-  return launches + 1;
+  return launches + (clear_at != nullptr);
 }
 
 template <typename D, typename W>
 void sums(const SumArgs& a, const Plan& p, const void* dout, void* dtable, cudaStream_t s) {
   const bool vec = a.H % 8 == 0 && ((uintptr_t)dout | (uintptr_t)dtable) % 16 == 0;
-  const int64_t clear = a.present ? ceil_div(ceil_div(a.rows, 32) * a.slices, kThreads / 32) : 0;
-  const dim3 grid((unsigned)(a.sum_blocks + clear));
+  const dim3 grid((unsigned)p.sum_blocks);
   auto go = [&](auto kernel) { launch_overlapped(kernel, grid, dim3(kThreads), s, a, (const D*)dout, (W*)dtable); };
   if (vec)
     p.width == 32 ? go(sum_kernel<D, W, true, 32>) : p.width == 16 ? go(sum_kernel<D, W, true, 16>) : go(sum_kernel<D, W, true, 8>);
   else
     p.width == 32 ? go(sum_kernel<D, W, false, 32>) : p.width == 16 ? go(sum_kernel<D, W, false, 16>) : go(sum_kernel<D, W, false, 8>);
-  if (a.chunks > 1)
-    launch_overlapped(join_kernel<W>, dim3((unsigned)(a.chunks - 1), (unsigned)ceil_div(a.H, kJoinColumns * 4)), dim3(kThreads), s, a, (W*)dtable);
+  if (a.chunks > 1) {
+    const int64_t items = (a.chunks - 1) * ceil_div(a.H, kJoinColumns * 4);  // at most
+    launch_overlapped(join_kernel<W>, dim3((unsigned)std::min<int64_t>(items, 8 * 148)), dim3(kThreads), s, a, (W*)dtable);
+  }
 }
 
 template <typename F>
@@ -674,8 +701,9 @@ void lookup(const Ids& ids, const void* table, DType table_type, int64_t rows, i
           while ((1 << shift) < kThreads && (1 << shift) < H / 8) ++shift;
           const int64_t slices = ceil_div(H / 8, 1 << shift);
           BAGUA_CHECK(slices < 65536, Tensor, "embedding: " << H << " columns");
-          const dim3 grid((unsigned)ceil_div(ids.n, kThreads >> shift), (unsigned)slices);
-          launch_overlapped(lookup_kernel<Id, W, O>, grid, dim3(kThreads), s, (const Id*)ids.data, (const W*)table, rows, row_stride, (O*)out, ids.n,
+          const bool many = ids.n * H >= kManyElements;
+          const dim3 grid((unsigned)ceil_div(ids.n, (int64_t)(kThreads >> shift) * (many ? kRowsAhead : 1)), (unsigned)slices);
+          launch_overlapped(many ? lookup_kernel<Id, W, O, kRowsAhead> : lookup_kernel<Id, W, O, 1>, grid, dim3(kThreads), s, (const Id*)ids.data, (const W*)table, rows, row_stride, (O*)out, ids.n,
                             H, shift, scale, encoder_ops::index_report());
         } else {
           launch_overlapped(fits(2) ? lookup_any_kernel<Id, W, O, 2> : lookup_any_kernel<Id, W, O, 1>, dim3((unsigned)ceil_div(ids.n, kThreads / 32)),
@@ -688,29 +716,32 @@ void lookup(const Ids& ids, const void* table, DType table_type, int64_t rows, i
   });
 }
 
-size_t backward_scratch_bytes(int64_t n, int64_t rows, int64_t H) { return plan(n, rows, H).bytes; }
+size_t backward_scratch_bytes(int64_t n, int64_t H) { return plan(n, H).bytes; }
 
 int backward(const Ids& ids, const void* dout, DType dout_type, int64_t rows, int64_t H, float scale, int64_t padding, void* dtable,
              DType table_type, bool accumulate, void* scratch, cudaStream_t s) {
   BAGUA_CHECK(ids.n > 0 && ids.n <= kMaxTokens && rows > 0 && rows <= kMaxRows && H > 0, Tensor,
               "embedding backward: " << ids.n << " tokens, " << rows << " rows of " << H << " columns");
   BAGUA_CHECK(!accumulate || table_type == DType::F32, Tensor, "embedding gradients are added to in float32");
-  const Plan p = plan(ids.n, rows, H);
-  BAGUA_CHECK(ceil_div(H, kJoinColumns * 4) < 65536 && p.sum_blocks + ceil_div(ceil_div(rows, 32) * p.slices, kThreads / 32) < (1ll << 31), Tensor,
-              "embedding backward: " << rows << " rows of " << H << " columns");
+  const Plan p = plan(ids.n, H);
   auto at = [&](size_t offset) { return (uint32_t*)((char*)scratch + offset); };
-  uint32_t* present = accumulate ? nullptr : at(p.present);
+  void* clear_at = accumulate ? nullptr : dtable;
+  const int64_t clear_bytes = rows * H * (int64_t)dtype_bytes(table_type);
+  BAGUA_CHECK(p.sum_blocks < (1ll << 31) && ceil_div(clear_bytes, kClearBytes) < (1ll << 31), Tensor,
+              "embedding backward: " << rows << " rows of " << H << " columns");
+  BAGUA_CHECK((uintptr_t)dtable % 16 == 0 || accumulate, Tensor, "embedding backward: the gradient does not start on 16 bytes");
   SumArgs a{};
   const Keys key{rows, padding};
-  int launches = ids.wide ? sort<int64_t>(ids, key, p, at(p.keys), at(p.counts), present, &a.keys, &a.places, s)
-                          : sort<int32_t>(ids, key, p, at(p.keys), at(p.counts), present, &a.keys, &a.places, s);
-  a.present = present;
+  int launches = ids.wide ? sort<int64_t>(ids, key, p, at(p.keys), at(p.counts), at(p.runs), clear_at, clear_bytes, &a.keys, &a.places, s)
+                          : sort<int32_t>(ids, key, p, at(p.keys), at(p.counts), at(p.runs), clear_at, clear_bytes, &a.keys, &a.places, s);
+  a.accumulate = accumulate;
+  a.run_count = at(p.runs);
+  a.runs = a.run_count + 1;
   a.partial = (float*)at(p.partial);
   a.n = ids.n;
   a.rows = rows;
   a.H = H;
   a.chunks = p.chunks;
-  a.sum_blocks = p.sum_blocks;
   a.length = p.length;
   a.slices = p.slices;
   a.scale = scale;

@@ -31,8 +31,8 @@ void lookup(const Ids& ids, const void* table, DType table_type, int64_t rows, i
 
 // dtable [rows, H] from dout [n, H], both contiguous: all of its rows are written, or, with `accumulate` (dtable in F32), those that occur are
 // added to.  Ids outside the table and `padding` (-1: none) have no part in it.  Scratch: backward_scratch_bytes() of it, 16-byte aligned.
-// Returns the number of kernels launched.
-size_t backward_scratch_bytes(int64_t n, int64_t rows, int64_t H);
+// dtable starts on 16 bytes unless it is added to.  Returns the number of kernels launched.
+size_t backward_scratch_bytes(int64_t n, int64_t H);
 int backward(const Ids& ids, const void* dout, DType dout_type, int64_t rows, int64_t H, float scale, int64_t padding, void* dtable,
              DType table_type, bool accumulate, void* scratch, cudaStream_t s);
 

@@ -735,7 +735,7 @@ struct LookupNode : public EncoderNode {
       const at::Tensor d = grads[0].contiguous();
       if (!add) out[0] = fresh(table.sizes(), table.scalar_type(), table);
       // the framework's memory, not this package's pool: a graph that is being captured keeps it
-      const at::Tensor scratch = fresh({(int64_t)embedding::backward_scratch_bytes(n, rows, H)}, at::kByte, table);
+      const at::Tensor scratch = fresh({(int64_t)embedding::backward_scratch_bytes(n, H)}, at::kByte, table);
       count_launches(embedding::backward({id.data_ptr(), id.scalar_type() == at::kLong, n}, d.data_ptr(), kernel_dtype(d.scalar_type()), rows, H,
                                          (float)scale, padding, add ? table.grad().data_ptr() : out[0].data_ptr(),
                                          kernel_dtype(table.scalar_type()), add, scratch.data_ptr(), stream_of(table)));
