@@ -4,18 +4,27 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "adamw.h"
 #include "adamw_math.h"
 #include "launch.cuh"
+#include "typed_vec.cuh"
 
 namespace bagua {
 namespace adamw {
 
 namespace {
 
+using kernels::fma;
+using kernels::from_float;
+using kernels::halves;
 using kernels::launch_overlapped;
+using kernels::mul;
+using kernels::Pair;
+using kernels::pair;
+using kernels::to_float;
 using kernels::wait_for_predecessor;
 
 constexpr int kThreads = 256;
@@ -46,18 +55,6 @@ __device__ __forceinline__ int find_segment(const First& first_tile, int n, uint
   }
   return lo;
 }
-
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T>
-__device__ __forceinline__ T from_float(float x);
-template <>
-__device__ __forceinline__ float from_float<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
 // Four neighbouring elements, as one access where their address is a multiple of their size.
 template <typename T>
@@ -125,62 +122,116 @@ __global__ void __launch_bounds__(kThreads) step32_kernel(const __grid_constant_
 // A warp takes a block of elements that share their scales, eight to a lane: the largest value of a block is a reduction over the
 // warp's registers, and each element is read and written once.  Lanes hold two runs of four, so that the 32 loads of a run are one
 // piece of memory; elements of an address that no vector fits are taken one by one, lane by lane.
-constexpr int kTile8 = kThreads / 32 * kMoment8Block;
-template <typename P, typename G, int N>
-__global__ void __launch_bounds__(kThreads) step8_kernel(const __grid_constant__ Table<N> table) {
-  wait_for_predecessor();
-  const int k = find_segment(table.first_tile, table.n, blockIdx.x);
-  const Segment& a = table.seg[k];
+//
+// With 16 bytes an element instead of 28, instructions count as much as bytes (at 89 an element 67 M elements took 234 us).
+// So a warp takes several blocks one after the other, and what is asked once a tensor is asked once; two elements are computed by
+// one instruction where there is one; the square root and the reciprocal are the hardware's (within 2^-22 each: a
+// parameter is off by that part of its update); the moments' betas go into the factor that decodes them, and both directions of coding take
+// one factor.  A block with a scale beyond kPlainScale, or an eps so small that a subnormal square root counts next to
+// it, goes the longer way.
+constexpr int kBlocks8 = 4;  // of a warp
+// Blocks on an SM: so many leave 40 registers a thread and a few spilled ones.  131 M elements take 372 us, with five (48 registers)
+// 387, four (64) 421, three (80) 461: the loads of waiting warps are worth more than the spills cost.
+constexpr int kResident8 = 6;
+constexpr int kTile8 = kThreads / 32 * kMoment8Block * kBlocks8;
+constexpr float kPlainEps = 1e-10f;
+template <bool kPlain>
+__device__ __forceinline__ float root_of(float x) {
+  float y;
+  if constexpr (kPlain)
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  else
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool kPlain>
+__device__ __forceinline__ float reciprocal_of(float x) {
+  float y;
+  if constexpr (kPlain)
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  else
+    asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Byte e of a word of codes as a code's bits (code1_bits, code2_bits).
+__device__ __forceinline__ float word1_bits(uint32_t w, int e) { return __uint_as_float((uint32_t)((int)(w << (24 - 8 * e)) >> 4) & 0x87f00000u); }
+__device__ __forceinline__ float word2_bits(uint32_t w, int e) {
+  return __uint_as_float((e < 3 ? w << (19 - 8 * e) : w >> 5) & 0x07f80000u);
+}
+__device__ __forceinline__ Pair both(float x) { return pair(x, x); }
+
+template <typename P, typename G, bool kVec>
+__device__ __forceinline__ void step8_block(const Segment& a, const Hyper& h, uint32_t key, int64_t block) {
   const int lane = (int)threadIdx.x & 31;
-  const int64_t block = (int64_t)(blockIdx.x - table.first_tile[k]) * (kThreads / 32) + (threadIdx.x >> 5);
   const int64_t base = block * kMoment8Block;
-  if (base >= a.n) return;
-  const Hyper h = table.on_device ? table.on_device[a.group] : table.hyper[a.group];
-  P* p = (P*)a.p;
-  const G* g = (const G*)a.g;
-  uint8_t *m = (uint8_t*)a.m, *v = (uint8_t*)a.v;
+  P* p = (P*)a.p + base;
+  const G* g = (const G*)a.g + base;
+  uint8_t *m = (uint8_t*)a.m + base, *v = (uint8_t*)a.v + base;
   auto* copy = (__nv_bfloat16*)a.copy;
   const float ms = a.m_scale[block], vs = a.v_scale[block];
-  const bool vec = base + kMoment8Block <= a.n && fours(p) && fours(g) && fours(m) && fours(v) && fours(copy);
-  // element e of run r: base + at(r, e)
-  const int run = vec ? lane * 4 : lane, run_step = 128, step = vec ? 1 : 32;
-  const int n = (int)min((int64_t)kMoment8Block, a.n - base);
+  const int n = kVec ? kMoment8Block : (int)min((int64_t)kMoment8Block, a.n - base);
+  auto at = [&](int r, int e) { return r * 128 + (kVec ? lane * 4 + e : e * 32 + lane); };  // element e of run r
   float pv[2][4], gv[2][4], mv[2][4], vv[2][4];
   uint32_t mc[2], vc[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const int64_t i = base + r * run_step + run;
-    if (vec) {
-      load4(p + i, pv[r]);
-      load4(g + i, gv[r]);
-      mc[r] = *reinterpret_cast<const uint32_t*>(m + i);
-      vc[r] = *reinterpret_cast<const uint32_t*>(v + i);
+    if constexpr (kVec) {
+      load4(p + at(r, 0), pv[r]);
+      load4(g + at(r, 0), gv[r]);
+      mc[r] = *reinterpret_cast<const uint32_t*>(m + at(r, 0));
+      vc[r] = *reinterpret_cast<const uint32_t*>(v + at(r, 0));
     } else {
       mc[r] = vc[r] = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const bool in = r * run_step + run + e * 32 < n;
-        pv[r][e] = in ? to_float(p[i + e * 32]) : 0.f;
-        gv[r][e] = in ? to_float(g[i + e * 32]) : 0.f;
-        mc[r] |= (in ? (uint32_t)m[i + e * 32] : 0u) << (8 * e);
-        vc[r] |= (in ? (uint32_t)v[i + e * 32] : 0u) << (8 * e);
+        const int i = at(r, e);
+        pv[r][e] = i < n ? to_float(p[i]) : 0.f;
+        gv[r][e] = i < n ? to_float(g[i]) : 0.f;
+        mc[r] |= (i < n ? (uint32_t)m[i] : 0u) << (8 * e);
+        vc[r] |= (i < n ? (uint32_t)v[i] : 0u) << (8 * e);
       }
     }
   }
   uint32_t top_m = 0, top_v = 0;
+  auto step = [&](auto plain) {
+    constexpr bool kPlain = decltype(plain)::value;
+    const Pair km = both(__fmul_rn(h.b1, ms) * (kPlain ? kUp : 1.f)), kv = both(__fmul_rn(h.b2, vs) * (kPlain ? kUp : 1.f));
+    const Pair c1 = both(h.c1), c2 = both(h.c2), root = both(h.root), eps = both(h.eps), rate = both(-h.rate), keep = both(h.keep);
 #pragma unroll
-  for (int r = 0; r < 2; ++r)
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      mv[r][e] = decode1((mc[r] >> (8 * e)) & 0xffu, ms);
-      vv[r][e] = decode2((vc[r] >> (8 * e)) & 0xffu, vs);
-      update(h, pv[r][e], gv[r][e], mv[r][e], vv[r][e]);
-      // an element behind the end leaves the scales alone
-      const bool in = vec || r * run_step + run + e * step < n;
-      top_m = max(top_m, in ? float_bits(mv[r][e]) & 0x7fffffffu : 0u);
-      top_v = max(top_v, in ? float_bits(vv[r][e]) & 0x7fffffffu : 0u);
-    }
-  const uint32_t key = segment_key(h.random, a.index);
+      for (int e = 0; e < 4; e += 2) {
+        Pair mb = pair(word1_bits(mc[r], e), word1_bits(mc[r], e + 1)), vb = pair(word2_bits(vc[r], e), word2_bits(vc[r], e + 1));
+        if constexpr (!kPlain) {
+          mb = mul(mb, both(kUp));
+          vb = mul(vb, both(kUp));
+        }
+        // (moments() and parameter() of two elements)
+        const Pair gg = pair(gv[r][e], gv[r][e + 1]);
+        const Pair mm = fma(c1, gg, mul(mb, km)), v2 = fma(mul(c2, gg), gg, mul(vb, kv));
+        const float2 vf = halves(v2), mf = halves(mm);
+        const float2 d = halves(fma(pair(root_of<kPlain>(vf.x), root_of<kPlain>(vf.y)), root, eps));
+        const Pair per = pair(reciprocal_of<kPlain>(d.x), reciprocal_of<kPlain>(d.y));
+        const float2 pf = halves(fma(pair(pv[r][e], pv[r][e + 1]), keep, mul(mul(rate, mm), per)));
+        pv[r][e] = pf.x;
+        pv[r][e + 1] = pf.y;
+        mv[r][e] = mf.x;
+        mv[r][e + 1] = mf.y;
+        vv[r][e] = vf.x;
+        vv[r][e + 1] = vf.y;
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          // an element behind the end leaves the scales alone
+          const bool in = kVec || at(r, e + o) < n;
+          top_m = max(top_m, in ? float_bits(mv[r][e + o]) & 0x7fffffffu : 0u);
+          top_v = max(top_v, in ? float_bits(vv[r][e + o]) & 0x7fffffffu : 0u);
+        }
+      }
+  };
+  if (ms < kPlainScale && vs < kPlainScale && h.eps >= kPlainEps)
+    step(std::true_type{});
+  else
+    step(std::false_type{});
   float per_m, per_v;
   const float new_ms = block_scale(__reduce_max_sync(0xffffffffu, top_m), kLargest1, &per_m);
   const float new_vs = block_scale(__reduce_max_sync(0xffffffffu, top_v), kLargest2, &per_v);
@@ -188,31 +239,72 @@ __global__ void __launch_bounds__(kThreads) step8_kernel(const __grid_constant__
     a.m_scale[block] = new_ms;
     a.v_scale[block] = new_vs;
   }
+  const uint32_t random = random_base(key, base) + (uint32_t)at(0, 0) * kStride;
+  auto code = [&](auto plain) {
+    constexpr bool kPlain = decltype(plain)::value;
+    const Pair fm = both(per_m * kDown), fv = both(per_v * kDown);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      uint32_t c1[4], c2[4];
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        float2 y1 = halves(mul(pair(mv[r][e], mv[r][e + 1]), fm)), y2 = halves(mul(pair(vv[r][e], vv[r][e + 1]), fv));
+        if constexpr (!kPlain) {  // each by its own scale
+          y1 = make_float2(scaled(mv[r][e], per_m, new_ms < kPlainScale), scaled(mv[r][e + 1], per_m, new_ms < kPlainScale));
+          y2 = make_float2(scaled(vv[r][e], per_v, new_vs < kPlainScale), scaled(vv[r][e + 1], per_v, new_vs < kPlainScale));
+        }
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          const uint32_t bits = mix(random + (uint32_t)(at(r, e + o) - at(0, 0)) * kStride);
+          c1[e + o] = encode1(o ? y1.y : y1.x, bits);
+          c2[e + o] = encode2(o ? y2.y : y2.x, vv[r][e + o], bits);
+        }
+      }
+      mc[r] = c1[0] | c1[1] << 8 | c1[2] << 16 | c1[3] << 24;
+      vc[r] = c2[0] | c2[1] << 8 | c2[2] << 16 | c2[3] << 24;
+    }
+  };
+  if (new_ms < kPlainScale && new_vs < kPlainScale)
+    code(std::true_type{});
+  else
+    code(std::false_type{});
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const int64_t i = base + r * run_step + run;
-    mc[r] = vc[r] = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t random = random_bits(key, i + e * step);
-      mc[r] |= encode1(mv[r][e], per_m, random) << (8 * e);
-      vc[r] |= encode2(vv[r][e], per_v, random) << (8 * e);
-    }
-    if (vec) {
-      store4(p + i, pv[r]);
-      *reinterpret_cast<uint32_t*>(m + i) = mc[r];
-      *reinterpret_cast<uint32_t*>(v + i) = vc[r];
-      if (copy) store4(copy + i, pv[r]);
+    if constexpr (kVec) {
+      store4(p + at(r, 0), pv[r]);
+      *reinterpret_cast<uint32_t*>(m + at(r, 0)) = mc[r];
+      *reinterpret_cast<uint32_t*>(v + at(r, 0)) = vc[r];
+      if (copy) store4(copy + base + at(r, 0), pv[r]);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (r * run_step + run + e * 32 >= n) continue;
-        p[i + e * 32] = from_float<P>(pv[r][e]);
-        m[i + e * 32] = (uint8_t)(mc[r] >> (8 * e));
-        v[i + e * 32] = (uint8_t)(vc[r] >> (8 * e));
-        if (copy) copy[i + e * 32] = __float2bfloat16_rn(pv[r][e]);
+        const int i = at(r, e);
+        if (i >= n) continue;
+        p[i] = from_float<P>(pv[r][e]);
+        m[i] = (uint8_t)(mc[r] >> (8 * e));
+        v[i] = (uint8_t)(vc[r] >> (8 * e));
+        if (copy) copy[base + i] = __float2bfloat16_rn(pv[r][e]);
       }
     }
+  }
+}
+template <typename P, typename G, int N>
+__global__ void __launch_bounds__(kThreads, kResident8) step8_kernel(const __grid_constant__ Table<N> table) {
+  wait_for_predecessor();
+  const int k = find_segment(table.first_tile, table.n, blockIdx.x);
+  const Segment& a = table.seg[k];
+  const Hyper h = table.on_device ? table.on_device[a.group] : table.hyper[a.group];
+  const uint32_t key = segment_key(h.random, a.index);
+  const bool vec = fours((P*)a.p) && fours((const G*)a.g) && fours((uint8_t*)a.m) && fours((uint8_t*)a.v) && fours((__nv_bfloat16*)a.copy);
+  // a tile's blocks in turn, so that its warps read neighbours at a time
+  int64_t block = (int64_t)(blockIdx.x - table.first_tile[k]) * (kTile8 / kMoment8Block) + (threadIdx.x >> 5);
+#pragma unroll 1
+  for (int turn = 0; turn < kBlocks8; ++turn, block += kThreads / 32) {
+    if (block * kMoment8Block >= a.n) return;
+    if (vec && (block + 1) * kMoment8Block <= a.n)
+      step8_block<P, G, true>(a, h, key, block);
+    else
+      step8_block<P, G, false>(a, h, key, block);
   }
 }
 
@@ -283,7 +375,7 @@ struct ReadTable {
   int n;
 };
 static_assert(sizeof(ReadTable) <= 32764, "launch parameters");
-constexpr int kReadTile = kThreads * 4 * 4;
+constexpr int kReadVecs = 2, kReadTile = kThreads * 8 * kReadVecs;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__ ReadTable table) {
   wait_for_predecessor();
@@ -291,20 +383,28 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__
   const cuda::Read8& a = table.seg[k];
   T *m = (T*)a.m_out, *v = (T*)a.v_out;
   const int64_t base = (int64_t)(blockIdx.x - table.first_tile[k]) * kReadTile;
-  if (base + kReadTile <= a.n && fours(a.m) && fours(a.v) && fours(m) && fours(v)) {
+  if (base + kReadTile <= a.n && ((uintptr_t)a.m | (uintptr_t)a.v) % 8 == 0 && ((uintptr_t)m | (uintptr_t)v) % 16 == 0) {
+    uint2 mc[kReadVecs], vc[kReadVecs];
+    float ms[kReadVecs], vs[kReadVecs];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t i = base + (r * kThreads + threadIdx.x) * 4;
-      const uint32_t mc = *reinterpret_cast<const uint32_t*>(a.m + i), vc = *reinterpret_cast<const uint32_t*>(a.v + i);
-      const float ms = a.m_scale[i / kMoment8Block], vs = a.v_scale[i / kMoment8Block];
-      float mv[4], vv[4];
+    for (int r = 0; r < kReadVecs; ++r) {
+      const int64_t i = base + (r * kThreads + threadIdx.x) * 8;
+      mc[r] = *reinterpret_cast<const uint2*>(a.m + i);
+      vc[r] = *reinterpret_cast<const uint2*>(a.v + i);
+      ms[r] = a.m_scale[i / kMoment8Block];
+      vs[r] = a.v_scale[i / kMoment8Block];
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        mv[e] = decode1((mc >> (8 * e)) & 0xffu, ms);
-        vv[e] = decode2((vc >> (8 * e)) & 0xffu, vs);
+    for (int r = 0; r < kReadVecs; ++r) {
+      const int64_t i = base + (r * kThreads + threadIdx.x) * 8;
+      float mv[8], vv[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        mv[e] = word1_bits(e < 4 ? mc[r].x : mc[r].y, e % 4) * kUp * ms[r];
+        vv[e] = word2_bits(e < 4 ? vc[r].x : vc[r].y, e % 4) * kUp * vs[r];
       }
-      store4(m + i, mv);
-      store4(v + i, vv);
+      kernels::store8(m + i, kernels::narrow8<T>(mv));
+      kernels::store8(v + i, kernels::narrow8<T>(vv));
     }
   } else {
     const int64_t end = min(base + kReadTile, a.n);

@@ -30,9 +30,9 @@ void step8(const Segment& a, const Hyper& h, int64_t block) {
   uint32_t top_m = 0, top_v = 0;
   for (int64_t i = lo; i < hi; ++i) {
     float pv = P::ld(p + i), &mi = mv[i - lo], &vi = vv[i - lo];
-    mi = decode1(m[i], a.m_scale[block]);
-    vi = decode2(v[i], a.v_scale[block]);
-    update(h, pv, G::ld(g + i), mi, vi);
+    moments(h, G::ld(g + i), code1_bits(m[i]) * kUp * product(h.b1, a.m_scale[block]), code2_bits(v[i]) * kUp * product(h.b2, a.v_scale[block]),
+            mi, vi);
+    pv = parameter(h, pv, mi, vi);
     P::st(p + i, pv);
     if (a.copy) kernels::Elem<DType::BF16>::st((uint16_t*)a.copy + i, pv);
     const uint32_t mb = float_bits(mi) & 0x7fffffffu, vb = float_bits(vi) & 0x7fffffffu;
@@ -40,13 +40,13 @@ void step8(const Segment& a, const Hyper& h, int64_t block) {
     top_v = vb > top_v ? vb : top_v;
   }
   float per_m, per_v;
-  a.m_scale[block] = block_scale(top_m, kLargest1, &per_m);
-  a.v_scale[block] = block_scale(top_v, kLargest2, &per_v);
+  const float ms = a.m_scale[block] = block_scale(top_m, kLargest1, &per_m);
+  const float vs = a.v_scale[block] = block_scale(top_v, kLargest2, &per_v);
   const uint32_t key = segment_key(h.random, a.index);
   for (int64_t i = lo; i < hi; ++i) {
     const uint32_t random = random_bits(key, i);
-    m[i] = (uint8_t)encode1(mv[i - lo], per_m, random);
-    v[i] = (uint8_t)encode2(vv[i - lo], per_v, random);
+    m[i] = (uint8_t)encode1(scaled(mv[i - lo], per_m, ms < kPlainScale), random);
+    v[i] = (uint8_t)encode2(scaled(vv[i - lo], per_v, vs < kPlainScale), vv[i - lo], random);
   }
 }
 

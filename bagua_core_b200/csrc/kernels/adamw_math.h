@@ -51,19 +51,23 @@ BAGUA_HD uint32_t step_random(uint64_t seed, int64_t step) {
 }
 BAGUA_HD uint32_t segment_key(uint32_t random, uint32_t k) { return mix(random + k); }
 // 32 random bits of element i of a tensor: the low half rounds the first moment, the high half the second.
-BAGUA_HD uint32_t random_bits(uint32_t key, int64_t i) {
-  return mix((uint32_t)i * 0x9e3779b9u + key + (uint32_t)((uint64_t)i >> 32) * 0x85ebca77u);
-}
+constexpr uint32_t kStride = 0x9e3779b9u;  // between the numbers that neighbouring elements' bits are made from
+BAGUA_HD uint32_t random_base(uint32_t key, int64_t i) { return (uint32_t)i * kStride + key + (uint32_t)((uint64_t)i >> 32) * 0x85ebca77u; }
+BAGUA_HD uint32_t random_bits(uint32_t key, int64_t i) { return mix(random_base(key, i)); }
 
 // A code's 7 or 8 bits, moved to where fp32 has its fraction and the low end of its exponent, are the code's value times 2^-120:
 // codes with exponent 0 become fp32's own subnormal numbers.  The way back is a shift too, and adding random bits below the cut
 // before it is the stochastic rounding, for codes of every exponent alike.
 constexpr float kUp = 0x1p120f, kDown = 0x1p-120f, kLargest1 = 480.f, kLargest2 = 496.f, kSmallestScale = 0x1p-126f;
+// Scales below this can be multiplied by 2^120, their reciprocals by 2^-120, without leaving fp32's range: the products with a block's
+// elements then take one factor instead of two.
+constexpr float kPlainScale = 64.f;
 
-BAGUA_HD float decode1(uint32_t code, float scale) {  // scale: the block's
-  return bits_float(((code & 0x7fu) << 20) | ((code & 0x80u) << 24)) * kUp * scale;
-}
-BAGUA_HD float decode2(uint32_t code, float scale) { return bits_float(code << 19) * kUp * scale; }
+// A code's bits, to be multiplied by 2^120 and its block's scale.
+BAGUA_HD float code1_bits(uint32_t code) { return bits_float(((code & 0x7fu) << 20) | ((code & 0x80u) << 24)); }
+BAGUA_HD float code2_bits(uint32_t code) { return bits_float(code << 19); }
+BAGUA_HD float decode1(uint32_t code, float scale) { return code1_bits(code) * kUp * scale; }
+BAGUA_HD float decode2(uint32_t code, float scale) { return code2_bits(code) * kUp * scale; }
 
 // The scale of a block whose largest value is `top`, as bits of a number that is not negative; its reciprocal in `per`.
 BAGUA_HD float block_scale(uint32_t top, float largest, float* per) {
@@ -71,22 +75,24 @@ BAGUA_HD float block_scale(uint32_t top, float largest, float* per) {
     *per = 0.f;
     return bits_float(0x7fc00000u);
   }
-  float s = bits_float(top) / largest;
+  float s = bits_float(top) * (1.f / largest);
   s = s < kSmallestScale ? kSmallestScale : s;
   *per = 1.f / s;
   return top ? s : 0.f;
 }
-// y = x / scale, at most the largest value but for a rounding.
-BAGUA_HD uint32_t encode1(float x, float per, uint32_t random) {
-  const uint32_t b = float_bits(x * per * kDown);
-  uint32_t c = ((b & 0x7fffffffu) + ((random & 0xffffu) << 4) + 8u) >> 20;
-  c = c > 0x7fu ? 0x7fu : c;
-  return c | (b >> 31 << 7);
+// y = x / scale times 2^-120, at most the largest value but for a rounding.
+BAGUA_HD float scaled(float x, float per, bool plain) { return plain ? x * (per * kDown) : x * per * kDown; }
+BAGUA_HD uint32_t encode1(float y, uint32_t random) {
+  const uint32_t b = float_bits(y);
+  uint32_t c = ((b & 0x7fffffffu) + ((random << 4 & 0xffff0u) | 8u)) >> 20;
+  c = c < 0x7fu ? c : 0x7fu;
+  return c | (b >> 24 & 0x80u);
 }
-BAGUA_HD uint32_t encode2(float x, float per, uint32_t random) {
-  uint32_t c = (float_bits(x * per * kDown) + ((random >> 16) << 3) + 4u) >> 19;
-  c = c > 0xffu ? 0xffu : c;
-  return c == 0u && x > 0.f ? 1u : c;
+BAGUA_HD uint32_t encode2(float y, float x, uint32_t random) {
+  uint32_t c = (float_bits(y) + ((random >> 13 & 0x7fff8u) | 4u)) >> 19;
+  c = c < 0xffu ? c : 0xffu;
+  const uint32_t least = float_bits(x) < 1u ? float_bits(x) : 1u;  // 1 unless x is 0
+  return c > least ? c : least;
 }
 
 BAGUA_HD Hyper make_hyper(const GroupValues& g, int64_t step, uint64_t seed) {
@@ -103,20 +109,39 @@ BAGUA_HD Hyper make_hyper(const GroupValues& g, int64_t step, uint64_t seed) {
   return h;
 }
 
-// Both moments' new values and the parameter's.
-BAGUA_HD void update(const Hyper& h, float& p, float g, float& m, float& v) {
+// Products and multiply-adds spelled out: which of two products is rounded is not left to the compiler.
+BAGUA_HD float product(float a, float b) {
 #ifdef __CUDA_ARCH__
-  // multiply-adds spelled out: which of two products is rounded is not left to the compiler
-  m = __fmaf_rn(h.c1, g, __fmul_rn(h.b1, m));
-  v = __fmaf_rn(__fmul_rn(h.c2, g), g, __fmul_rn(h.b2, v));
-  const float d = __fmaf_rn(__fsqrt_rn(v), h.root, h.eps);
-  p = __fmaf_rn(p, h.keep, -__fmul_rn(h.rate, __fdiv_rn(m, d)));
+  return __fmul_rn(a, b);
 #else
-  m = __builtin_fmaf(h.c1, g, h.b1 * m);
-  v = __builtin_fmaf(h.c2 * g, g, h.b2 * v);
-  const float d = __builtin_fmaf(__builtin_sqrtf(v), h.root, h.eps);
-  p = __builtin_fmaf(p, h.keep, -(h.rate * (m / d)));
+  return a * b;
 #endif
+}
+BAGUA_HD float multiply_add(float a, float b, float c) {
+#ifdef __CUDA_ARCH__
+  return __fmaf_rn(a, b, c);
+#else
+  return __builtin_fmaf(a, b, c);
+#endif
+}
+// The new moments, from the old ones times their betas.
+BAGUA_HD void moments(const Hyper& h, float g, float b1_m, float b2_v, float& m, float& v) {
+  m = multiply_add(h.c1, g, b1_m);
+  v = multiply_add(product(h.c2, g), g, b2_v);
+}
+// The new parameter.
+BAGUA_HD float parameter(const Hyper& h, float p, float m, float v) {
+#ifdef __CUDA_ARCH__
+  const float d = __fmaf_rn(__fsqrt_rn(v), h.root, h.eps);
+  return __fmaf_rn(p, h.keep, -__fmul_rn(h.rate, __fdiv_rn(m, d)));
+#else
+  const float d = __builtin_fmaf(__builtin_sqrtf(v), h.root, h.eps);
+  return __builtin_fmaf(p, h.keep, -(h.rate * (m / d)));
+#endif
+}
+BAGUA_HD void update(const Hyper& h, float& p, float g, float& m, float& v) {
+  moments(h, g, product(h.b1, m), product(h.b2, v), m, v);
+  p = parameter(h, p, m, v);
 }
 
 }  // namespace adamw

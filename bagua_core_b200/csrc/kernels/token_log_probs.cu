@@ -35,33 +35,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   return y;
 }
 
-// Two fp32 values that are added or multiplied by one instruction.
-using Pair = unsigned long long;
-__device__ __forceinline__ Pair pair(float x, float y) {
-  Pair p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
-  return p;
-}
-__device__ __forceinline__ float2 halves(Pair p) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
-  return f;
-}
-__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
-  Pair d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ Pair add(Pair a, Pair b) {
-  Pair d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ Pair mul(Pair a, Pair b) {
-  Pair d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 __device__ __forceinline__ Pair exp2_fast(Pair p) {
   const float2 f = halves(p);
   return pair(exp2_fast(f.x), exp2_fast(f.y));

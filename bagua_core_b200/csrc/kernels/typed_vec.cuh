@@ -1,4 +1,4 @@
-// Eight neighbouring elements of a floating-point type in registers as fp32, loaded and stored 16 bytes at a time.
+// Floating-point elements in registers as fp32: eight neighbours loaded and stored 16 bytes at a time, pairs computed together.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -19,6 +19,34 @@ template <>
 __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Two fp32 values that are added or multiplied by one instruction, each rounded as alone.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float x, float y) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ float2 halves(Pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ Pair add(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Pair mul(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 
 // The elements as they lie in memory.
 template <typename T>
