@@ -1056,8 +1056,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         p->keep = true;
         return p;
       }))
-      .def("add", &trainer::AdamWPlan::add, py::arg("param"), py::arg("grad"), py::arg("exp_avg"), py::arg("exp_avg_sq"), py::arg("scales"),
-           py::arg("bf16_shadow"), py::arg("group"))
+      .def("add",
+           [](trainer::AdamWPlan& p, const at::Tensor& param, const at::Tensor& g, const at::Tensor& ms, const at::Tensor& vs,
+              const std::optional<at::Tensor>& scales, const std::optional<at::Tensor>& shadow, int group) {
+             p.add(param, g, ms, vs, scales ? &*scales : nullptr, shadow ? &*shadow : nullptr, group);
+           },
+           py::arg("param"), py::arg("grad"), py::arg("exp_avg"), py::arg("exp_avg_sq"), py::arg("scales"), py::arg("bf16_shadow"),
+           py::arg("group"))
       .def("step",
            [](trainer::AdamWPlan& p, const std::vector<std::tuple<double, double, double, double, double>>& groups, const py::object& step,
               uint64_t seed) {

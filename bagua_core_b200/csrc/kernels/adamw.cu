@@ -30,7 +30,7 @@ using kernels::wait_for_predecessor;
 constexpr int kThreads = 256;
 
 // Segments are cut into tiles, a block each; the table of them travels with the launch.  A launch's parameters may take 32,764
-// bytes; a step of few tensors takes the small table, whose 4 KB reach the GPU sooner.
+// bytes; steps of fewer tensors take smaller tables, which reach the GPU sooner.
 constexpr int kGroups = 8;
 template <int N>
 struct Table {
@@ -40,7 +40,7 @@ struct Table {
   uint32_t first_tile[N + 1];
   int n;
 };
-constexpr int kFew = 44, kMany = 400;
+constexpr int kFew = 44, kSome = 128, kMany = 400;
 static_assert(sizeof(Table<kFew>) <= 4096 && sizeof(Table<kMany>) <= 32764, "launch parameters");
 
 template <typename First>
@@ -129,11 +129,11 @@ __global__ void __launch_bounds__(kThreads) step32_kernel(const __grid_constant_
 // parameter is off by that part of its update); the moments' betas go into the factor that decodes them, and both directions of coding take
 // one factor.  A block with a scale beyond kPlainScale, or an eps so small that a subnormal square root counts next to
 // it, goes the longer way.
-constexpr int kBlocks8 = 4;  // of a warp
+constexpr int kTurns8 = 2;  // blocks of a warp; us with 1, 2, 4: 131 M elements in fp32 353, 363, 363, in bf16 356, 333, 328; 10 M 32.4, 31.6, 34.1
 // Blocks on an SM: so many leave 40 registers a thread and a few spilled ones.  131 M elements take 372 us, with five (48 registers)
 // 387, four (64) 421, three (80) 461: the loads of waiting warps are worth more than the spills cost.
 constexpr int kResident8 = 6;
-constexpr int kTile8 = kThreads / 32 * kMoment8Block * kBlocks8;
+constexpr int kTile8 = kThreads / 32 * kMoment8Block * kTurns8;
 constexpr float kPlainEps = 1e-10f;
 template <bool kPlain>
 __device__ __forceinline__ float root_of(float x) {
@@ -157,6 +157,12 @@ __device__ __forceinline__ float reciprocal_of(float x) {
 __device__ __forceinline__ float word1_bits(uint32_t w, int e) { return __uint_as_float((uint32_t)((int)(w << (24 - 8 * e)) >> 4) & 0x87f00000u); }
 __device__ __forceinline__ float word2_bits(uint32_t w, int e) {
   return __uint_as_float((e < 3 ? w << (19 - 8 * e) : w >> 5) & 0x07f80000u);
+}
+// The largest magnitude, or NaN.
+__device__ __forceinline__ float largest(float a, float b, float c) {
+  float y;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
 }
 __device__ __forceinline__ Pair both(float x) { return pair(x, x); }
 
@@ -192,7 +198,7 @@ __device__ __forceinline__ void step8_block(const Segment& a, const Hyper& h, ui
       }
     }
   }
-  uint32_t top_m = 0, top_v = 0;
+  float top_m = 0.f, top_v = 0.f;
   auto step = [&](auto plain) {
     constexpr bool kPlain = decltype(plain)::value;
     const Pair km = both(__fmul_rn(h.b1, ms) * (kPlain ? kUp : 1.f)), kv = both(__fmul_rn(h.b2, vs) * (kPlain ? kUp : 1.f));
@@ -219,12 +225,13 @@ __device__ __forceinline__ void step8_block(const Segment& a, const Hyper& h, ui
         mv[r][e + 1] = mf.y;
         vv[r][e] = vf.x;
         vv[r][e + 1] = vf.y;
-#pragma unroll
-        for (int o = 0; o < 2; ++o) {
-          // an element behind the end leaves the scales alone
-          const bool in = kVec || at(r, e + o) < n;
-          top_m = max(top_m, in ? float_bits(mv[r][e + o]) & 0x7fffffffu : 0u);
-          top_v = max(top_v, in ? float_bits(vv[r][e + o]) & 0x7fffffffu : 0u);
+        // (an element behind the end leaves the scales alone)
+        if (kVec || at(r, e + 1) < n) {
+          top_m = largest(top_m, mf.x, mf.y);
+          top_v = largest(top_v, vf.x, vf.y);
+        } else if (at(r, e) < n) {
+          top_m = largest(top_m, mf.x, mf.x);
+          top_v = largest(top_v, vf.x, vf.x);
         }
       }
   };
@@ -233,8 +240,8 @@ __device__ __forceinline__ void step8_block(const Segment& a, const Hyper& h, ui
   else
     step(std::false_type{});
   float per_m, per_v;
-  const float new_ms = block_scale(__reduce_max_sync(0xffffffffu, top_m), kLargest1, &per_m);
-  const float new_vs = block_scale(__reduce_max_sync(0xffffffffu, top_v), kLargest2, &per_v);
+  const float new_ms = block_scale(__reduce_max_sync(0xffffffffu, float_bits(top_m)), kLargest1, &per_m);
+  const float new_vs = block_scale(__reduce_max_sync(0xffffffffu, float_bits(top_v)), kLargest2, &per_v);
   if (lane == 0) {
     a.m_scale[block] = new_ms;
     a.v_scale[block] = new_vs;
@@ -248,15 +255,15 @@ __device__ __forceinline__ void step8_block(const Segment& a, const Hyper& h, ui
       uint32_t c1[4], c2[4];
 #pragma unroll
       for (int e = 0; e < 4; e += 2) {
-        float2 y1 = halves(mul(pair(mv[r][e], mv[r][e + 1]), fm)), y2 = halves(mul(pair(vv[r][e], vv[r][e + 1]), fv));
+        float2 y1 = halves(mul(pair(fabsf(mv[r][e]), fabsf(mv[r][e + 1])), fm)), y2 = halves(mul(pair(vv[r][e], vv[r][e + 1]), fv));
         if constexpr (!kPlain) {  // each by its own scale
-          y1 = make_float2(scaled(mv[r][e], per_m, new_ms < kPlainScale), scaled(mv[r][e + 1], per_m, new_ms < kPlainScale));
+          y1 = make_float2(scaled(fabsf(mv[r][e]), per_m, new_ms < kPlainScale), scaled(fabsf(mv[r][e + 1]), per_m, new_ms < kPlainScale));
           y2 = make_float2(scaled(vv[r][e], per_v, new_vs < kPlainScale), scaled(vv[r][e + 1], per_v, new_vs < kPlainScale));
         }
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
           const uint32_t bits = mix(random + (uint32_t)(at(r, e + o) - at(0, 0)) * kStride);
-          c1[e + o] = encode1(o ? y1.y : y1.x, bits);
+          c1[e + o] = encode1(o ? y1.y : y1.x, mv[r][e + o], bits);
           c2[e + o] = encode2(o ? y2.y : y2.x, vv[r][e + o], bits);
         }
       }
@@ -299,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, kResident8) step8_kernel(const __gri
   // a tile's blocks in turn, so that its warps read neighbours at a time
   int64_t block = (int64_t)(blockIdx.x - table.first_tile[k]) * (kTile8 / kMoment8Block) + (threadIdx.x >> 5);
 #pragma unroll 1
-  for (int turn = 0; turn < kBlocks8; ++turn, block += kThreads / 32) {
+  for (int turn = 0; turn < kTurns8; ++turn, block += kThreads / 32) {
     if (block * kMoment8Block >= a.n) return;
     if (vec && (block + 1) * kMoment8Block <= a.n)
       step8_block<P, G, true>(a, h, key, block);
@@ -338,6 +345,8 @@ int steps(const Segment* segs, int n, const Hyper* hypers, int groups, bool on_d
     if (part.empty()) return;
     if ((int)part.size() <= kFew)
       launch<P, G, kMoments8, kFew>(part.data(), (int)part.size(), h.data(), (int)h.size(), on_device ? hypers : nullptr, s);
+    else if ((int)part.size() <= kSome)
+      launch<P, G, kMoments8, kSome>(part.data(), (int)part.size(), h.data(), (int)h.size(), on_device ? hypers : nullptr, s);
     else
       launch<P, G, kMoments8, kMany>(part.data(), (int)part.size(), h.data(), (int)h.size(), on_device ? hypers : nullptr, s);
     ++launches;
@@ -369,15 +378,16 @@ int steps(bool moments8, const Segment* segs, int n, const Hyper* hypers, int gr
 }
 
 // ---- moments read back --------------------------------------------------------------------------
+template <int N>
 struct ReadTable {
-  cuda::Read8 seg[kMany];
-  uint32_t first_tile[kMany + 1];
+  cuda::Read8 seg[N];
+  uint32_t first_tile[N + 1];
   int n;
 };
-static_assert(sizeof(ReadTable) <= 32764, "launch parameters");
+static_assert(sizeof(ReadTable<kMany>) <= 32764, "launch parameters");
 constexpr int kReadVecs = 2, kReadTile = kThreads * 8 * kReadVecs;
-template <typename T>
-__global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__ ReadTable table) {
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__ ReadTable<N> table) {
   wait_for_predecessor();
   const int k = find_segment(table.first_tile, table.n, blockIdx.x);
   const cuda::Read8& a = table.seg[k];
@@ -458,26 +468,39 @@ int step(const Types& t, const Segment* segs, int n, const Hyper* hypers, int gr
 
 int read8(const Read8* segs, int n, DType out, cudaStream_t s) {
   int launches = 0;
-  for (int at = 0; at < n;) {
-    ReadTable t;
+  auto read = [&](auto size, int from, int count) {
+    ReadTable<decltype(size)::value> t;
     t.n = 0;
     t.first_tile[0] = 0;
-    for (; at < n && t.n < kMany; ++at) {
-      if (segs[at].n == 0) continue;
-      const int64_t tiles = t.first_tile[t.n] + (segs[at].n + kReadTile - 1) / kReadTile;
-      if (tiles >= (int64_t)1 << 31) break;  // never the first: a tensor has fewer
-      t.seg[t.n] = segs[at];
-      t.first_tile[++t.n] = (uint32_t)tiles;
+    for (int k = from; k < from + count; ++k) {
+      if (segs[k].n == 0) continue;
+      t.seg[t.n] = segs[k];
+      t.first_tile[t.n + 1] = t.first_tile[t.n] + (uint32_t)((segs[k].n + kReadTile - 1) / kReadTile);
+      ++t.n;
     }
-    if (t.n == 0) continue;
+    if (t.n == 0) return;
     const dim3 grid(t.first_tile[t.n]);
+    constexpr int N = decltype(size)::value;
     switch (out) {
-      case DType::F32: launch_overlapped(read8_kernel<float>, grid, dim3(kThreads), s, t); break;
-      case DType::F16: launch_overlapped(read8_kernel<__half>, grid, dim3(kThreads), s, t); break;
-      case DType::BF16: launch_overlapped(read8_kernel<__nv_bfloat16>, grid, dim3(kThreads), s, t); break;
+      case DType::F32: launch_overlapped(read8_kernel<float, N>, grid, dim3(kThreads), s, t); break;
+      case DType::F16: launch_overlapped(read8_kernel<__half, N>, grid, dim3(kThreads), s, t); break;
+      case DType::BF16: launch_overlapped(read8_kernel<__nv_bfloat16, N>, grid, dim3(kThreads), s, t); break;
       default: throw BaguaError(ErrorKind::Tensor, std::string("moments are not read into ") + dtype_name(out));
     }
     ++launches;
+  };
+  constexpr int64_t most = (int64_t)1 << 40;  // elements of a launch: its tiles are counted in 31 bits
+  for (int at = 0; at < n;) {
+    int count = 0;
+    int64_t elements = 0;
+    for (; at + count < n && count < kMany && (count == 0 || elements + segs[at + count].n <= most); ++count) elements += segs[at + count].n;
+    if (count <= kFew)
+      read(std::integral_constant<int, kFew>{}, at, count);
+    else if (count <= kSome)
+      read(std::integral_constant<int, kSome>{}, at, count);
+    else
+      read(std::integral_constant<int, kMany>{}, at, count);
+    at += count;
   }
   return launches;
 }

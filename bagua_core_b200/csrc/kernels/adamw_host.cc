@@ -45,7 +45,7 @@ void step8(const Segment& a, const Hyper& h, int64_t block) {
   const uint32_t key = segment_key(h.random, a.index);
   for (int64_t i = lo; i < hi; ++i) {
     const uint32_t random = random_bits(key, i);
-    m[i] = (uint8_t)encode1(scaled(mv[i - lo], per_m, ms < kPlainScale), random);
+    m[i] = (uint8_t)encode1(scaled(std::fabs(mv[i - lo]), per_m, ms < kPlainScale), mv[i - lo], random);
     v[i] = (uint8_t)encode2(scaled(vv[i - lo], per_v, vs < kPlainScale), vv[i - lo], random);
   }
 }

@@ -1,6 +1,10 @@
 // The arithmetic of an AdamW step on one element, and the 8-bit form of its moments, for host and device.
 #pragma once
 
+#ifdef __CUDACC__
+#include <cuda_runtime.h>
+#endif
+
 #include <cmath>
 #include <cstdint>
 #include <cstring>
@@ -82,15 +86,20 @@ BAGUA_HD float block_scale(uint32_t top, float largest, float* per) {
 }
 // y = x / scale times 2^-120, at most the largest value but for a rounding.
 BAGUA_HD float scaled(float x, float per, bool plain) { return plain ? x * (per * kDown) : x * per * kDown; }
-BAGUA_HD uint32_t encode1(float y, uint32_t random) {
-  const uint32_t b = float_bits(y);
-  uint32_t c = ((b & 0x7fffffffu) + ((random << 4 & 0xffff0u) | 8u)) >> 20;
-  c = c < 0x7fu ? c : 0x7fu;
-  return c | (b >> 24 & 0x80u);
+BAGUA_HD uint32_t sum_up_to(uint32_t a, uint32_t b, uint32_t most) {
+#ifdef __CUDA_ARCH__
+  return __viaddmin_u32(a, b, most);
+#else
+  return a + b < most ? a + b : most;
+#endif
+}
+// Codes of y, at least 0, and of a moment x with the sign (first) or above 0 (second).  Neither sum leaves 32 bits, for a y that is not finite either.
+constexpr uint32_t kLastBits = 0x07ffffffu;  // those of both largest codes, and of what is cut off
+BAGUA_HD uint32_t encode1(float y, float x, uint32_t random) {
+  return sum_up_to(float_bits(y), (random << 4 & 0xffff0u) | 8u, kLastBits) >> 20 | (float_bits(x) >> 24 & 0x80u);
 }
 BAGUA_HD uint32_t encode2(float y, float x, uint32_t random) {
-  uint32_t c = (float_bits(y) + ((random >> 13 & 0x7fff8u) | 4u)) >> 19;
-  c = c < 0xffu ? c : 0xffu;
+  const uint32_t c = sum_up_to(float_bits(y), (random >> 13 & 0x7fff8u) | 4u, kLastBits) >> 19;
   const uint32_t least = float_bits(x) < 1u ? float_bits(x) : 1u;  // 1 unless x is 0
   return c > least ? c : least;
 }

@@ -279,6 +279,8 @@ __global__ void __launch_bounds__(kThreads)
 // times as long to get there.)
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortRounds = 8, kSortBlocks = 8;
 constexpr int64_t kSortTokens = (int64_t)kSortBlocks * kSortThreads * kSortRounds;
+// A block of it clears so many bytes itself, in about a microsecond; a launch of its own for that would cost two.
+constexpr int64_t kSmallClear = 128 << 10;
 constexpr int kSortBits = 9, kSortDigits = 1 << kSortBits;  // of a pass at most: two for up to 2^18 - 1 rows
 struct SortShared {
   uint32_t seen[kSortWarps][kSortDigits];
@@ -290,7 +292,7 @@ size_t sort_shared_bytes(int rounds) { return sizeof(SortShared) + (size_t)round
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads)
     sort_kernel(const Id* __restrict__ ids, Keys key, int n, int bits, int digit_bits, int rounds, uint32_t* __restrict__ keys_out,
-                uint32_t* __restrict__ places_out, uint32_t* __restrict__ zero) {
+                uint32_t* __restrict__ places_out, uint32_t* __restrict__ zero, uint4* __restrict__ clear_at, int64_t clear_bytes) {
   extern __shared__ __align__(16) char s_memory[];
   SortShared& s = *reinterpret_cast<SortShared*>(s_memory);
   const int room = rounds * kSortThreads;  // tokens of a block
@@ -303,6 +305,10 @@ __global__ void __launch_bounds__(kSortThreads)
   wait_for_predecessor();
   let_successor_start();
   if (rank == 0 && tid == 0) *zero = 0;
+  if (clear_at) {
+    for (int64_t i = rank * kSortThreads + tid; i < clear_bytes / 16; i += blocks * kSortThreads) clear_at[i] = make_uint4(0, 0, 0, 0);
+    if (rank == 0 && tid < clear_bytes % 16) reinterpret_cast<char*>(clear_at)[clear_bytes / 16 * 16 + tid] = 0;
+  }
   const int digits = 1 << digit_bits;
   for (int shift = 0, from = 0; shift < bits; shift += digit_bits, from ^= 1) {
     uint2* in = s_tokens + from * room;
@@ -629,12 +635,13 @@ int sort(const Ids& ids, Keys key, const Plan& p, uint32_t* buffers, uint32_t* c
       if (device < 64) allowed[device].store(true, std::memory_order_release);
     }
     const int passes = (bits + kSortBits - 1) / kSortBits, digit_bits = std::max(5, (bits + passes - 1) / passes);  // whole warps of digits
+    const bool small = clear_bytes <= kSmallClear * blocks;
     launch_clusters_shared(sort_kernel<Id>, 1, blocks, dim3(kSortThreads), shared, s, (const Id*)ids.data, key, (int)n, bits,
-                           digit_bits, rounds, buffers, buffers + n, zero);
-    if (clear_at) clear(clear_at, clear_bytes, s);
+                           digit_bits, rounds, buffers, buffers + n, zero, (uint4*)(small ? clear_at : nullptr), clear_bytes);
+    if (clear_at && !small) clear(clear_at, clear_bytes, s);
     *keys = buffers;
     *places = buffers + n;
-    return clear_at ? 2 : 1;
+    return clear_at && !small ? 2 : 1;
   }
   uint32_t* k[2] = {buffers, buffers + 2 * n};
   const uint32_t *in_k = nullptr, *in_p = nullptr;

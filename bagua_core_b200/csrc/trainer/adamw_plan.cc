@@ -38,27 +38,50 @@ void check_values(const adamw::GroupValues& g) {
 
 cudaStream_t stream_on(int device) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream(); }
 
+// A tensor's memory.  Those of a kind (all parameters, all gradients, ...) are a list.
 struct Piece {
   uintptr_t from, to;
-  bool written;
 };
-void check_pieces(std::vector<Piece>& pieces) {
-  std::sort(pieces.begin(), pieces.end(), [](const Piece& a, const Piece& b) { return a.from < b.from; });
+struct Pieces {
+  std::vector<Piece> list;
+  bool written = true;
+  void add(const void* p, int64_t bytes) {
+    if (p && bytes > 0) list.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes});
+  }
+};
+// Throws if a piece that is written overlaps another one.
+void check_apart(std::vector<Pieces>& kinds) {
+  constexpr const char* what = "a buffer that is written overlaps another one of the same call";
+  auto before = [](const Piece& a, const Piece& b) { return a.from < b.from; };
+  // Lists whose pieces follow each other, in a part of memory that no other list has: slices of flat buffers.  Seen without sorting them all.
+  std::vector<Piece> whole;
+  bool apart = true;
+  for (const Pieces& k : kinds) {
+    if (k.list.empty()) continue;
+    for (size_t i = 1; i < k.list.size() && apart; ++i) apart = k.list[i].from >= k.list[i - 1].to;
+    whole.push_back({k.list.front().from, k.list.back().to});
+  }
+  std::sort(whole.begin(), whole.end(), before);
+  for (size_t i = 1; i < whole.size() && apart; ++i) apart = whole[i].from >= whole[i - 1].to;
+  if (apart) return;
+  struct Mixed : Piece {
+    bool written;
+  };
+  std::vector<Mixed> all;
+  for (const Pieces& k : kinds)
+    for (const Piece& p : k.list) all.push_back({{p.from, p.to}, k.written});
+  std::sort(all.begin(), all.end(), before);
   uintptr_t read = 0, written = 0;  // the furthest ends so far
-  for (const Piece& x : pieces) {
-    BAGUA_CHECK(x.from >= written && (!x.written || x.from >= read), Tensor,
-                "a buffer that AdamW writes overlaps another one of the same call");
+  for (const Mixed& x : all) {
+    BAGUA_CHECK(x.from >= written && (!x.written || x.from >= read), Tensor, what);
     (x.written ? written : read) = std::max(x.written ? written : read, x.to);
   }
-}
-void piece(std::vector<Piece>& to, const void* p, int64_t bytes, bool written) {
-  if (p && bytes > 0) to.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, written});
 }
 
 }  // namespace
 
 void AdamWPlan::add(const at::Tensor& p, const at::Tensor& g, const at::Tensor& m, const at::Tensor& v,
-                    const std::optional<at::Tensor>& scales, const std::optional<at::Tensor>& copy, int group) {
+                    const at::Tensor* scales, const at::Tensor* copy, int group) {
   BAGUA_CHECK((p.is_cuda() || p.is_cpu()) && real(p.scalar_type()) && real(g.scalar_type()) && p.layout() == at::kStrided, Tensor,
               "AdamW works on float32, float16 and bfloat16 tensors on a GPU or the host");
   const int device = p.is_cuda() ? (int)p.device().index() : -1;
@@ -73,7 +96,7 @@ void AdamWPlan::add(const at::Tensor& p, const at::Tensor& g, const at::Tensor& 
   for (const at::Tensor* t : {&g, &m, &v})
     BAGUA_CHECK(t->layout() == at::kStrided && t->device() == p.device() && same_layout(*t, p), Tensor,
                 "AdamW needs gradients and moments of the parameter's sizes and strides, on its device");
-  BAGUA_CHECK(moments8 == scales.has_value(), Tensor, "moments of 8 bits need scales, others have none");
+  BAGUA_CHECK(moments8 == (scales != nullptr), Tensor, "moments of 8 bits need scales, others have none");
   if (scales) check_scales(*scales, p.numel(), p.device());
   if (copy)
     BAGUA_CHECK(copy->scalar_type() == at::kBFloat16 && copy->device() == p.device() && same_layout(*copy, p), Tensor,
@@ -111,19 +134,21 @@ void AdamWPlan::add_grad_buffer(const at::Tensor& g) {
 }
 
 void AdamWPlan::check_apart() const {
-  std::vector<Piece> pieces;
-  pieces.reserve(segs_.size() * 4);
+  std::vector<Pieces> kinds(7);
+  for (auto& k : kinds) k.list.reserve(segs_.size());
+  kinds[1].written = false;
   const int64_t p = (int64_t)dtype_bytes(types_.p), g = (int64_t)dtype_bytes(types_.g), held = types_.moments8 ? 1 : 4;
   for (const auto& a : segs_) {
-    piece(pieces, a.p, a.n * p, true);
-    piece(pieces, a.g, a.n * g, false);
-    piece(pieces, a.m, a.n * held, true);
-    piece(pieces, a.v, a.n * held, true);
-    piece(pieces, a.copy, a.n * 2, true);
-    piece(pieces, a.m_scale, adamw::moment8_blocks(a.n) * 4, true);
-    piece(pieces, a.v_scale, adamw::moment8_blocks(a.n) * 4, true);
+    const int64_t blocks = adamw::moment8_blocks(a.n) * 4;
+    kinds[0].add(a.p, a.n * p);
+    kinds[1].add(a.g, a.n * g);
+    kinds[2].add(a.m, a.n * held);
+    kinds[3].add(a.v, a.n * held);
+    kinds[4].add(a.copy, a.n * 2);
+    kinds[5].add(a.m_scale, blocks);
+    kinds[6].add(a.v_scale, blocks);
   }
-  check_pieces(pieces);
+  trainer::check_apart(kinds);
 }
 
 int AdamWPlan::step(const std::vector<adamw::GroupValues>& groups, const StepNumbers& numbers, uint64_t seed) {
@@ -175,9 +200,9 @@ int adamw_step(const TensorList& p, const TensorList& g, const TensorList& m, co
               "AdamW needs lists of one length");
   AdamWPlan plan;
   plan.first_index = first_index;
+  plan.reserve(n);
   for (size_t k = 0; k < n; ++k)
-    plan.add(p[k], g[k], m[k], v[k], scales ? std::optional<at::Tensor>((*scales)[k]) : std::nullopt,
-             copies ? std::optional<at::Tensor>((*copies)[k]) : std::nullopt, 0);
+    plan.add(p[k], g[k], m[k], v[k], scales ? &(*scales)[k] : nullptr, copies ? &(*copies)[k] : nullptr, 0);
   plan.check_apart();
   return plan.step({values}, numbers, seed);
 }
@@ -191,8 +216,10 @@ int adamw_read8(const TensorList& m, const TensorList& v, const TensorList& scal
   BAGUA_CHECK((m[0].is_cuda() || m[0].is_cpu()) && real(type), Tensor,
               "moments on a GPU or the host are read into float32, float16 or bfloat16 tensors");
   std::vector<adamw::cuda::Read8> segs;
-  std::vector<Piece> pieces;
-  pieces.reserve(4 * n);
+  std::vector<Pieces> kinds(6);
+  for (auto& k : kinds) k.list.reserve(n);
+  for (int k = 0; k < 4; ++k) kinds[k].written = false;
+  segs.reserve(n);
   for (size_t k = 0; k < n; ++k) {
     BAGUA_CHECK(m[k].scalar_type() == at::kByte && v[k].scalar_type() == at::kByte && m_out[k].scalar_type() == type &&
                     v_out[k].scalar_type() == type,
@@ -206,14 +233,14 @@ int adamw_read8(const TensorList& m, const TensorList& v, const TensorList& scal
     segs.push_back({m[k].data_ptr<uint8_t>(), v[k].data_ptr<uint8_t>(), s, s + scales[k].stride(0), m_out[k].data_ptr(), v_out[k].data_ptr(),
                     m[k].numel()});
     const int64_t bytes = m[k].numel() * (int64_t)m_out[k].element_size(), blocks = adamw::moment8_blocks(m[k].numel()) * 4;
-    piece(pieces, segs.back().m, m[k].numel(), false);
-    piece(pieces, segs.back().v, m[k].numel(), false);
-    piece(pieces, segs.back().m_scale, blocks, false);
-    piece(pieces, segs.back().v_scale, blocks, false);
-    piece(pieces, segs.back().m_out, bytes, true);
-    piece(pieces, segs.back().v_out, bytes, true);
+    kinds[0].add(segs.back().m, m[k].numel());
+    kinds[1].add(segs.back().v, m[k].numel());
+    kinds[2].add(segs.back().m_scale, blocks);
+    kinds[3].add(segs.back().v_scale, blocks);
+    kinds[4].add(segs.back().m_out, bytes);
+    kinds[5].add(segs.back().v_out, bytes);
   }
-  check_pieces(pieces);
+  check_apart(kinds);
   if (!m[0].is_cuda()) {
     adamw::host::read8(segs.data(), (int)n, dtype_of(type));
     return 1;

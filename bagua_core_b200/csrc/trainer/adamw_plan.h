@@ -20,11 +20,12 @@ struct StepNumbers {
   std::optional<at::Tensor> device;
 };
 
-// A tensor with its gradient, moments and, for moments in 8 bits, their scales [2, blocks]; `copy`: where it goes in bf16.
+// Tensors with their gradients, moments and, for moments in 8 bits, their scales [2, blocks]; `copy`: where they go in bf16.
 class AdamWPlan {
  public:
-  void add(const at::Tensor& p, const at::Tensor& g, const at::Tensor& m, const at::Tensor& v, const std::optional<at::Tensor>& scales,
-           const std::optional<at::Tensor>& copy, int group);
+  void add(const at::Tensor& p, const at::Tensor& g, const at::Tensor& m, const at::Tensor& v, const at::Tensor* scales, const at::Tensor* copy,
+           int group);
+  void reserve(size_t n) { segs_.reserve(n); }
   // Throws if a buffer that is written overlaps another one of the plan.
   void check_apart() const;
   // On the current stream of the tensors' device; returns the number of kernels launched.
