@@ -11,7 +11,8 @@ they skip the per-forward weight casts and the cast-and-add of every weight grad
 Under bf16 autocast on a GPU what lies between the projections runs as this package's kernels
 (`csrc/kernels/encoder_ops.h`) and the library's LayerNorm in native autograd functions: the embedding
 sum and the gradients of its tables, GELU with the projection in front of it, the packing of the attention
-gradients, the span loss.  The roundings are those of the plain composition below, which runs elsewhere."""
+gradients, the span loss.  Batches of more tokens than that embedding takes look their tokens up with
+`ops.embedding`.  The roundings are those of the plain composition below, which runs elsewhere."""
 from __future__ import annotations
 
 from dataclasses import dataclass
@@ -24,9 +25,10 @@ from .._native import C as _C
 from ..ops import wgrad
 from ..ops.fused_linear import ShadowLinear
 from ..ops.modules import drops_nothing, plain_embedding, untouched
+from ..ops.token_embedding import embedding
 
 
-_EMBED_TOKENS = _C.max_embedding_tokens  # more tokens per batch take the framework's embedding
+_EMBED_TOKENS = _C.max_embedding_tokens  # more tokens per batch take `ops.embedding`
 
 
 @dataclass
@@ -156,7 +158,11 @@ class BertForQuestionAnswering(nn.Module):
                                     self.ln.bias, self.ln.eps, wgrad.active())
         else:
             pos = torch.arange(s, device=input_ids.device)
-            x = self.ln(self.tok(input_ids) + self.pos(pos)[None] + self.typ.weight[0][None, None])
+            # more tokens than that kernel's gradient is made for: this one's is sorted by token
+            many = (plain_embedding(m.get("tok")) and _fused(self.tok.weight, m.get("ln")) and input_ids.is_cuda
+                    and input_ids.dtype == torch.int64 and b * s > _EMBED_TOKENS)
+            tok = embedding(input_ids, self.tok.weight) if many else self.tok(input_ids)
+            x = self.ln(tok + self.pos(pos)[None] + self.typ.weight[0][None, None])
         x = self.drop(x)
         for layer in self.layers:
             x = layer(x)
