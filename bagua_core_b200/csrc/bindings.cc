@@ -1050,6 +1050,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       n.host = steps.cast<std::vector<int64_t>>();
     return n;
   };
+  // The tensors of a list or tuple, which holds them for the time of the call.
+  static auto refs = [](const py::handle& list) {
+    const py::object fast = py::reinterpret_steal<py::object>(PySequence_Fast(list.ptr(), "a list of tensors is needed"));
+    if (!fast) throw py::error_already_set();
+    TORCH_CHECK_TYPE(fast.ptr() == list.ptr(), "a list or tuple of tensors is needed");
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast.ptr());
+    PyObject** items = PySequence_Fast_ITEMS(fast.ptr());
+    trainer::TensorRefs r((size_t)n);
+    for (Py_ssize_t k = 0; k < n; ++k) {
+      TORCH_CHECK_TYPE(THPVariable_Check(items[k]), "a list of tensors holds something else");
+      r[(size_t)k] = &THPVariable_Unpack(items[k]);
+    }
+    return r;
+  };
+  static auto maybe_refs = [](const py::object& list) { return list.is_none() ? std::nullopt : std::optional<trainer::TensorRefs>(refs(list)); };
   py::class_<trainer::AdamWPlan>(m, "AdamWPlan")
       .def(py::init([]() {
         auto p = std::make_unique<trainer::AdamWPlan>();
@@ -1075,14 +1090,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("zero_grad", &trainer::AdamWPlan::zero_grad, py::arg("stream"));
   m.def(
       "adamw_step",
-      [](const trainer::TensorList& p, const trainer::TensorList& g, const trainer::TensorList& ms, const trainer::TensorList& vs,
-         const std::optional<trainer::TensorList>& scales, const std::optional<trainer::TensorList>& copies, double lr, double b1, double b2,
-         double eps, double wd, const py::object& step, uint64_t seed, uint32_t first_index) {
-        return trainer::adamw_step(p, g, ms, vs, scales, copies, {lr, b1, b2, eps, wd}, step_numbers(step), seed, first_index);
+      [](const py::object& p, const py::object& g, const py::object& ms, const py::object& vs, const py::object& scales, const py::object& copies,
+         double lr, double b1, double b2, double eps, double wd, const py::object& step, uint64_t seed, uint32_t first_index) {
+        return trainer::adamw_step(refs(p), refs(g), refs(ms), refs(vs), maybe_refs(scales), maybe_refs(copies), {lr, b1, b2, eps, wd},
+                                   step_numbers(step), seed, first_index);
       },
       py::arg("params"), py::arg("grads"), py::arg("exp_avgs"), py::arg("exp_avg_sqs"), py::arg("scales"), py::arg("copies"), py::arg("lr"),
       py::arg("beta1"), py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"), py::arg("step"), py::arg("seed"), py::arg("first_index"));
-  m.def("adamw_read8", &trainer::adamw_read8, py::arg("exp_avgs"), py::arg("exp_avg_sqs"), py::arg("scales"), py::arg("exp_avgs_out"),
+  m.def("adamw_read8", [](const py::object& ms, const py::object& vs, const py::object& scales, const py::object& m_out, const py::object& v_out) {
+          return trainer::adamw_read8(refs(ms), refs(vs), refs(scales), refs(m_out), refs(v_out));
+        }, py::arg("exp_avgs"), py::arg("exp_avg_sqs"), py::arg("scales"), py::arg("exp_avgs_out"),
         py::arg("exp_avg_sqs_out"));
   m.attr("moment8_block") = adamw::kMoment8Block;
   py::class_<trainer::GradHooks, std::shared_ptr<trainer::GradHooks>>(m, "GradHooks")

@@ -50,7 +50,8 @@ struct Segment {
   float *m_scale, *v_scale;  // of codes: one for each block
   int64_t n;
   uint32_t index;  // its own number among the tensors of a step
-  int32_t group;   // index of its hyperparameters
+  int16_t group;   // index of its hyperparameters
+  int16_t lead;    // set by the GPU path: elements in front of the first four that all buffers hold as one piece; -1: there are none
 };
 
 // Which types a call's parameters and gradients have, and what its moments are held in.

@@ -92,6 +92,7 @@ void AdamWPlan::add(const at::Tensor& p, const at::Tensor& g, const at::Tensor& 
                                                                                                     << g.scalar_type());
   const at::ScalarType held = moments8 ? at::kByte : at::kFloat;
   BAGUA_CHECK(m.scalar_type() == held && v.scalar_type() == held, Tensor, "AdamW's moments are both float32, or both codes of 8 bits (uint8)");
+  BAGUA_CHECK(!p.is_neg() && !g.is_neg(), Tensor, "AdamW needs tensors that hold their values as they are, not negated views");
   BAGUA_CHECK(p.is_non_overlapping_and_dense(), Tensor, "AdamW needs parameters without gaps between their elements");
   for (const at::Tensor* t : {&g, &m, &v})
     BAGUA_CHECK(t->layout() == at::kStrided && t->device() == p.device() && same_layout(*t, p), Tensor,
@@ -103,7 +104,7 @@ void AdamWPlan::add(const at::Tensor& p, const at::Tensor& g, const at::Tensor& 
                 "the copy must be a bfloat16 tensor of the parameter's sizes and strides on its device");
   BAGUA_CHECK(segs_.empty() || (device == device_ && types.p == types_.p && types.g == types_.g && types.moments8 == types_.moments8), Tensor,
               "the tensors of an AdamW step are of one kind: one device, one type of parameters, of gradients and of moments");
-  BAGUA_CHECK(group >= 0, Tensor, "negative parameter group");
+  BAGUA_CHECK(group >= 0 && group < 32768, Tensor, "parameter group " << group << " is not one of the first 32768");
   device_ = device;
   types_ = types;
   adamw::Segment a{};
@@ -118,7 +119,7 @@ void AdamWPlan::add(const at::Tensor& p, const at::Tensor& g, const at::Tensor& 
   }
   a.n = p.numel();
   a.index = first_index + (uint32_t)segs_.size();
-  a.group = group;
+  a.group = (int16_t)group;
   segs_.push_back(a);
   if (!keep) return;
   keep_.insert(keep_.end(), {p, g, m, v});
@@ -192,8 +193,8 @@ int AdamWPlan::step(const std::vector<adamw::GroupValues>& groups, const StepNum
   return adamw::cuda::step(types_, segs_.data(), (int)segs_.size(), h.data(), (int)h.size(), false, s);
 }
 
-int adamw_step(const TensorList& p, const TensorList& g, const TensorList& m, const TensorList& v, const std::optional<TensorList>& scales,
-               const std::optional<TensorList>& copies, const adamw::GroupValues& values, const StepNumbers& numbers, uint64_t seed,
+int adamw_step(const TensorRefs& p, const TensorRefs& g, const TensorRefs& m, const TensorRefs& v, const std::optional<TensorRefs>& scales,
+               const std::optional<TensorRefs>& copies, const adamw::GroupValues& values, const StepNumbers& numbers, uint64_t seed,
                uint32_t first_index) {
   const size_t n = p.size();
   BAGUA_CHECK(g.size() == n && m.size() == n && v.size() == n && (!scales || scales->size() == n) && (!copies || copies->size() == n), Tensor,
@@ -202,18 +203,23 @@ int adamw_step(const TensorList& p, const TensorList& g, const TensorList& m, co
   plan.first_index = first_index;
   plan.reserve(n);
   for (size_t k = 0; k < n; ++k)
-    plan.add(p[k], g[k], m[k], v[k], scales ? &(*scales)[k] : nullptr, copies ? &(*copies)[k] : nullptr, 0);
+    plan.add(*p[k], *g[k], *m[k], *v[k], scales ? (*scales)[k] : nullptr, copies ? (*copies)[k] : nullptr, 0);
   plan.check_apart();
-  return plan.step({values}, numbers, seed);
+  const int launches = plan.step({values}, numbers, seed);
+  // autograd notices that a graph's values have changed since
+  for (const TensorRefs* list : {&p, &m, &v})
+    for (const at::Tensor* t : *list)
+      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  return launches;
 }
 
-int adamw_read8(const TensorList& m, const TensorList& v, const TensorList& scales, const TensorList& m_out, const TensorList& v_out) {
+int adamw_read8(const TensorRefs& m, const TensorRefs& v, const TensorRefs& scales, const TensorRefs& m_out, const TensorRefs& v_out) {
   const size_t n = m.size();
   BAGUA_CHECK(v.size() == n && scales.size() == n && m_out.size() == n && v_out.size() == n, Tensor, "reading moments needs lists of one length");
   if (n == 0) return 0;
-  const at::ScalarType type = m_out[0].scalar_type();
-  const at::Device device = m[0].device();
-  BAGUA_CHECK((m[0].is_cuda() || m[0].is_cpu()) && real(type), Tensor,
+  const at::ScalarType type = m_out[0]->scalar_type();
+  const at::Device device = m[0]->device();
+  BAGUA_CHECK((m[0]->is_cuda() || m[0]->is_cpu()) && real(type), Tensor,
               "moments on a GPU or the host are read into float32, float16 or bfloat16 tensors");
   std::vector<adamw::cuda::Read8> segs;
   std::vector<Pieces> kinds(6);
@@ -221,27 +227,27 @@ int adamw_read8(const TensorList& m, const TensorList& v, const TensorList& scal
   for (int k = 0; k < 4; ++k) kinds[k].written = false;
   segs.reserve(n);
   for (size_t k = 0; k < n; ++k) {
-    BAGUA_CHECK(m[k].scalar_type() == at::kByte && v[k].scalar_type() == at::kByte && m_out[k].scalar_type() == type &&
-                    v_out[k].scalar_type() == type,
+    BAGUA_CHECK(m[k]->scalar_type() == at::kByte && v[k]->scalar_type() == at::kByte && m_out[k]->scalar_type() == type &&
+                    v_out[k]->scalar_type() == type,
                 Tensor, "moments are read from codes of 8 bits (uint8) into tensors of one type");
-    BAGUA_CHECK(m[k].is_non_overlapping_and_dense() && m[k].device() == device, Tensor,
+    BAGUA_CHECK(m[k]->is_non_overlapping_and_dense() && m[k]->device() == device, Tensor,
                 "moments are read from tensors without gaps, on one device");
-    for (const at::Tensor* t : {&v[k], &m_out[k], &v_out[k]})
-      BAGUA_CHECK(t->device() == device && same_layout(*t, m[k]), Tensor, "moments and what they are read into have one size and layout, on one device");
-    check_scales(scales[k], m[k].numel(), device);
-    const float* s = scales[k].data_ptr<float>();
-    segs.push_back({m[k].data_ptr<uint8_t>(), v[k].data_ptr<uint8_t>(), s, s + scales[k].stride(0), m_out[k].data_ptr(), v_out[k].data_ptr(),
-                    m[k].numel()});
-    const int64_t bytes = m[k].numel() * (int64_t)m_out[k].element_size(), blocks = adamw::moment8_blocks(m[k].numel()) * 4;
-    kinds[0].add(segs.back().m, m[k].numel());
-    kinds[1].add(segs.back().v, m[k].numel());
+    for (const at::Tensor* t : {v[k], m_out[k], v_out[k]})
+      BAGUA_CHECK(t->device() == device && same_layout(*t, *m[k]), Tensor, "moments and what they are read into have one size and layout, on one device");
+    check_scales(*scales[k], m[k]->numel(), device);
+    const float* s = scales[k]->data_ptr<float>();
+    segs.push_back({m[k]->data_ptr<uint8_t>(), v[k]->data_ptr<uint8_t>(), s, s + scales[k]->stride(0), m_out[k]->data_ptr(), v_out[k]->data_ptr(),
+                    m[k]->numel()});
+    const int64_t bytes = m[k]->numel() * (int64_t)m_out[k]->element_size(), blocks = adamw::moment8_blocks(m[k]->numel()) * 4;
+    kinds[0].add(segs.back().m, m[k]->numel());
+    kinds[1].add(segs.back().v, m[k]->numel());
     kinds[2].add(segs.back().m_scale, blocks);
     kinds[3].add(segs.back().v_scale, blocks);
     kinds[4].add(segs.back().m_out, bytes);
     kinds[5].add(segs.back().v_out, bytes);
   }
   check_apart(kinds);
-  if (!m[0].is_cuda()) {
+  if (!m[0]->is_cuda()) {
     adamw::host::read8(segs.data(), (int)n, dtype_of(type));
     return 1;
   }

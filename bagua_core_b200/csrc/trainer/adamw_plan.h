@@ -13,6 +13,7 @@ namespace bagua {
 namespace trainer {
 
 using TensorList = std::vector<at::Tensor>;
+using TensorRefs = std::vector<const at::Tensor*>;  // that the caller holds
 
 // The number of a step for each parameter group: known to the host, or int64 on the device that are read when the step runs.
 struct StepNumbers {
@@ -46,12 +47,12 @@ class AdamWPlan {
   TensorList keep_;
 };
 
-int adamw_step(const TensorList& p, const TensorList& g, const TensorList& m, const TensorList& v, const std::optional<TensorList>& scales,
-               const std::optional<TensorList>& copies, const adamw::GroupValues& values, const StepNumbers& numbers, uint64_t seed,
+int adamw_step(const TensorRefs& p, const TensorRefs& g, const TensorRefs& m, const TensorRefs& v, const std::optional<TensorRefs>& scales,
+               const std::optional<TensorRefs>& copies, const adamw::GroupValues& values, const StepNumbers& numbers, uint64_t seed,
                uint32_t first_index);
 
 // The values of moments held in 8 bits, into m_out and v_out.
-int adamw_read8(const TensorList& m, const TensorList& v, const TensorList& scales, const TensorList& m_out, const TensorList& v_out);
+int adamw_read8(const TensorRefs& m, const TensorRefs& v, const TensorRefs& scales, const TensorRefs& m_out, const TensorRefs& v_out);
 
 }  // namespace trainer
 }  // namespace bagua

@@ -35,7 +35,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                exp_avg_sqs: Sequence[torch.Tensor], *, step: Union[int, torch.Tensor], lr: float, betas: Tuple[float, float] = (0.9, 0.999),
                eps: float = 1e-8, weight_decay: float = 1e-2, scales: Optional[Sequence[torch.Tensor]] = None,
                copies: Optional[Sequence[torch.Tensor]] = None, seed: int = 0, first_index: int = 0, stream=None) -> int:
-    """Steps all `params` in place and returns how many kernels that took.
+    """Steps all `params` (lists or tuples of tensors) in place and returns how many kernels that took.
 
     Parameters are float32, float16 or bfloat16, gradients of their type or float32, or of any of the three where the
     parameters are float32; the arithmetic is fp32.  Each tensor has its elements without gaps, and its gradient, its moments

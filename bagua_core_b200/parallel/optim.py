@@ -379,7 +379,9 @@ class FlatAdamW(_FlatOptimizer):
 
     def moments(self, p) -> Tuple[torch.Tensor, torch.Tensor]:
         """(first, second) moment of a parameter that was stepped or laid out, in fp32."""
-        s = self.state[p]
+        s = self.state.get(p, {})
+        if "step" not in s:
+            raise KeyError("the parameter has no moments yet: it was neither stepped nor laid out")
         if self.state_bits == 32:
             return s["exp_avg"].clone(), s["exp_avg_sq"].clone()
         m, v = (torch.empty_like(s["exp_avg"], dtype=torch.float32) for _ in range(2))

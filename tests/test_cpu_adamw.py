@@ -226,6 +226,40 @@ def test_refusals():
     check_refusals("cpu")
 
 
+def check_unaligned32(device):
+    """fp32 moments in tensors that start anywhere: all alike, so that whole vectors are found further on, and each elsewhere."""
+    for offsets in ((1, 1, 1, 1, 1), (3, 3, 3, 3, 3), (2, 2, 2, 2, 0), (1, 2, 3, 0, 1)):
+        for n in (1, 2, 3, 4, 5, 1023, 1024, 1025, 1027, 5000):
+            ps, gs, ms, vs = tensors([n], (torch.float32, torch.float32), "cpu", seed=n)
+            want = [x[0].clone().to(device) for x in (ps, gs, ms, vs)]
+            got = [torch.full((n + 8,), 9.0, device=device)[o:o + n].copy_(x[0]) for o, x in zip(offsets, (ps, gs, ms, vs))]
+            copies = [torch.zeros(n + 8, dtype=torch.bfloat16, device=device)[offsets[4]:offsets[4] + n], torch.zeros(n, dtype=torch.bfloat16, device=device)]
+            for (p, g, m, v), c in ((got, copies[0]), (want, copies[1])):
+                ops.adamw_step([p], [g], [m], [v], step=3, copies=[c], **HYPER)
+            assert all(torch.equal(a, b) for a, b in zip(got + copies[:1], want + copies[1:]))
+            for t, o in zip(got, offsets):  # what lies around them is as it was
+                whole = torch.as_strided(t, (n + 8,), (1,), 0)
+                assert (whole[:o] == 9).all() and (whole[o + n:] == 9).all()
+
+
+def test_fp32_moments_that_start_anywhere():
+    check_unaligned32("cpu")
+
+
+def check_versions(device):
+    """A graph whose values a step has changed since is noticed."""
+    p = torch.ones(4, device=device, requires_grad=True)
+    y = (p * p).sum()
+    m, v = torch.zeros(4, device=device), torch.zeros(4, device=device)
+    ops.adamw_step([p], [torch.ones(4, device=device)], [m], [v], step=1, lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_graphs_notice_a_step():
+    check_versions("cpu")
+
+
 def check_step_on_device(device):
     """A step's number in a tensor gives what the same number of the host gives, to the bit."""
     for bits in (32, 8):
@@ -327,6 +361,8 @@ def test_gradients_and_parameters_of_any_layout():
 
 def test_optimizer_refusals():
     p = [torch.nn.Parameter(torch.ones(3))]
+    with pytest.raises(KeyError):
+        P.FlatAdamW(p).moments(p[0])
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(weight_decay=-0.1), dict(state_bits=16), dict(seed=-1)):
         with pytest.raises(ValueError):
             P.FlatAdamW(p, **bad)
@@ -362,6 +398,36 @@ def _wrapped(rank, world, bits, shadow):
     kinds = sorted({str(s["exp_avg"].dtype) for s in states["state"].values()})
     P.destroy_process_group()
     return flat, copies, steps, kinds
+
+
+def _decentralized(rank, world):
+    import bagua_core_b200.parallel as P
+    from bagua_core_b200.models import MLP
+
+    torch.manual_seed(7)
+    model = MLP(16, 33, 5, depth=3)
+    P.init_process_group(torch.device("cpu"))
+    opt = P.FlatAdamW(model.parameters(), lr=1e-2, state_bits=8)
+    bm = P.with_bagua(model, [opt], P.DecentralizedAlgorithm(peer_selection_mode="all"), bucket_bytes=4096)
+    xs, ys = _batches(world)
+    bs = xs.shape[1] // world
+    before = torch.cat([p.detach().reshape(-1) for p in model.parameters()])
+    for s in range(3):
+        opt.zero_grad()
+        torch.nn.functional.mse_loss(bm(xs[s, rank * bs:(rank + 1) * bs]), ys[s, rank * bs:(rank + 1) * bs]).backward()
+        opt.step()
+    after = torch.cat([p.detach().reshape(-1) for p in model.parameters()])
+    P.destroy_process_group()
+    return before, after, len(opt._flat)
+
+
+def test_flat_adamw_on_buckets_of_weights():
+    from mp_util import run_ranks
+
+    for before, after, flat in run_ranks(_decentralized, 2):
+        assert flat > 1 and torch.isfinite(after).all()
+        # three steps of about lr each, none of more than ten times that
+        assert 1e-3 < (after - before).abs().max() <= 3 * 10 * 1e-2
 
 
 def _batches(world):

@@ -32,6 +32,14 @@ def test_special_values():
     host.check_special("cuda")
 
 
+def test_fp32_moments_that_start_anywhere():
+    host.check_unaligned32("cuda")
+
+
+def test_graphs_notice_a_step():
+    host.check_versions("cuda")
+
+
 def test_refusals():
     host.check_refusals("cuda")
 

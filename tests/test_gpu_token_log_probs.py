@@ -157,7 +157,7 @@ def test_offsets_beyond_32_bits():
     # two rows are split over blocks and sum in another order: each is off by at most (check())
     off = 2 * (2.0 ** -22 + (vocab / 256 + 64 + 2 ** 8) * host.U) * 16
     assert all(((p[-2:] - q).abs() <= off).all() for p, q in zip(r[:3], want[:3])) and torch.equal(r.top_ids[-2:], want.top_ids)
-    assert abs(float(r.log_probs[0]) + math.log(vocab)) < 1e-5
+    assert abs(float(r.log_probs[0].detach()) + math.log(vocab)) < 1e-5
     (d,) = torch.autograd.grad(r.log_probs.sum(), y)
     z = x[-2:].detach().clone().requires_grad_()
     (e,) = torch.autograd.grad(ops.token_log_probs(z, t[-2:]).log_probs.sum(), z)
