@@ -1,4 +1,6 @@
 // See adamw.h.  Streams over memory: with fp32 parameters, gradients and moments 28 bytes an element, 16 with moments in 8 bits.
+// 131 M elements: 534 us with fp32 moments (6.95 TB/s, above the rate of a copy), 365 with 8 bits (5.8 TB/s; integer
+// instructions are issued in three quarters of all cycles), 120 to read those into bf16 (6.6 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
