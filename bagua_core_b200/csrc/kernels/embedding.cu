@@ -31,8 +31,10 @@ constexpr int kThreads = 256;
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---- lookup -------------------------------------------------------------------------------------
-// A thread takes eight columns of a row, or of four rows, whose loads wait for their ids together, where enough threads are left.  Rows that fit no 16 bytes a row go the other way: a warp takes a row, its lanes pairs of columns or
-// single ones, eight of them under way together (40001 rows of 333 in fp16: 73 us with a thread for each element).
+// A thread takes eight columns of a row, or of four rows, whose loads wait for their ids together, where enough threads are left (65536
+// rows of 2048 in bf16: 66 us, 84 with one row each).  Rows that do not lie on 16 bytes go the other way: a warp takes a row, its
+// lanes pairs of columns or single ones, eight of them under way together (40001 rows of 333 in fp16: 13 us, 73 with a thread for
+// each element).
 constexpr int kRowsAhead = 4;
 constexpr int64_t kManyElements = 148ll * 2048 * 8 * kRowsAhead;
 template <typename Id, typename W, typename O, int kRows>
@@ -138,9 +140,9 @@ struct Keys {
   }
 };
 
-// Number of a lane's key among the equal digits of its warp's keys so far, which `seen` counts.  All lanes of the warp come here.  (Equal digits are
-// found bit by bit: the instruction that matches values takes a turn for each different one, 15,700 cycles for 8192 keys where
-// this takes 3,000.)
+// Number of a lane's key among the equal digits of its warp's keys so far, which `seen` counts.  All lanes of the warp come here.
+// (Equal digits are found bit by bit: the instruction that matches values takes a turn for each different one, 15,700 cycles for
+// 8192 keys in 512 digits where this takes 9,600.)
 template <int kBits>
 __device__ __forceinline__ uint32_t rank_in_warp(uint32_t* seen, uint32_t digit, bool valid) {
   uint32_t peers = __ballot_sync(0xffffffffu, valid);
@@ -159,7 +161,7 @@ __device__ __forceinline__ uint32_t rank_in_warp(uint32_t* seen, uint32_t digit,
 
 // Sorting in blocks that hand tiles to each other through memory.
 constexpr int kRounds = 8, kTile = kThreads * kRounds, kWarps = kThreads / 32;
-// counts[digit][tile].
+// counts[digit][tile]: how many of a tile's keys have a digit.
 template <typename Id>
 __global__ void __launch_bounds__(kThreads)
     histogram_kernel(const Id* __restrict__ ids, const uint32_t* __restrict__ keys, Keys key, int64_t n, int shift, uint32_t* __restrict__ counts,
@@ -180,8 +182,8 @@ __global__ void __launch_bounds__(kThreads)
   counts[(int64_t)threadIdx.x * tiles + blockIdx.x] = s_count[threadIdx.x];
 }
 constexpr int kScanThreads = 1024, kScanEach = 16;
-// Exclusive sums of n counts, a multiple of 4 of them on a 16-byte border, in one block.
-// Lets its successor start at once, and sets `zero` to 0.
+// Exclusive sums of n counts, a multiple of 4 of them on a 16-byte border, in one block.  Lets its successor start at once, and sets
+// `zero` to 0.
 __global__ void __launch_bounds__(kScanThreads) scan_kernel(uint32_t* __restrict__ counts, int64_t n, uint32_t* __restrict__ zero) {
   __shared__ uint32_t s_warp[32];
   __shared__ uint32_t s_total;
@@ -278,10 +280,11 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Sorting in one launch, which lets its successor start at once: the blocks of a cluster hold all tokens in their shared memory and hand them to each other there.  A pass counts
-// its digits by warp, makes the counts into places by sums over warps, blocks and digits, puts the block's tokens in their order, and copies
-// them, now neighbours for the most part, to where they belong.  (Stored from where they were, one by one, they took five
-// times as long to get there.)
+// Sorting in one launch, which lets its successor start at once: the blocks of a cluster hold all tokens in their shared memory and hand
+// them to each other there.  A pass counts its digits by warp, makes the counts into places by sums over warps, blocks and digits, puts
+// the block's tokens in their order, and copies them, now neighbours for the most part, to where they belong.  (Stored one by one from
+// where they were, 8192 tokens a block took 20,600 cycles to get there, 3,400 so.)  12288 tokens: 13 us, 65536: 32, hidden behind the
+// clearing of a large gradient; through memory 200,000 take 52.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortRounds = 8, kSortBlocks = 8;
 constexpr int64_t kSortTokens = (int64_t)kSortBlocks * kSortThreads * kSortRounds;
 // A block of it clears so many bytes itself, in about a microsecond; a launch of its own for that would cost two.
@@ -468,7 +471,8 @@ __device__ __forceinline__ void finish_row(T* row, float (&f)[8], float scale, b
 
 constexpr int kSumBlocks = 3;  // resident on an SM
 template <typename D, typename W, bool kVec, int kWidth>
-__global__ void __launch_bounds__(kThreads, kSumBlocks) sum_kernel(const __grid_constant__ SumArgs a, const D* __restrict__ dout, W* __restrict__ dtable) {
+__global__ void __launch_bounds__(kThreads, kSumBlocks)
+    sum_kernel(const __grid_constant__ SumArgs a, const D* __restrict__ dout, W* __restrict__ dtable) {
   wait_for_predecessor();
   const int warp_lane = (int)threadIdx.x & 31;
   const int64_t unit = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kWidth;
@@ -622,8 +626,8 @@ Plan plan(int64_t n, int64_t H) {
 }
 
 template <typename Id>
-int sort(const Ids& ids, Keys key, const Plan& p, uint32_t* buffers, uint32_t* counts, uint32_t* zero, void* clear_at, int64_t clear_bytes, const uint32_t** keys,
-         const uint32_t** places, cudaStream_t s) {
+int sort(const Ids& ids, Keys key, const Plan& p, uint32_t* buffers, uint32_t* counts, uint32_t* zero, void* clear_at, int64_t clear_bytes,
+         const uint32_t** keys, const uint32_t** places, cudaStream_t s) {
   const int64_t n = ids.n;
   int bits = 1;
   while (bits < 32 && (key.rows >> bits) != 0) ++bits;
@@ -706,7 +710,8 @@ void lookup(const Ids& ids, const void* table, DType table_type, int64_t rows, i
         // whether runs of so many elements start on multiples of their size, up to 16 bytes, in every row
         auto fits = [&](int64_t e) {
           const int64_t w = std::min<int64_t>(16, e * (int64_t)sizeof(W)), o = std::min<int64_t>(16, e * (int64_t)sizeof(O));
-          return H % e == 0 && (int64_t)((uintptr_t)table % w) == 0 && row_stride * (int64_t)sizeof(W) % w == 0 && (int64_t)((uintptr_t)out % o) == 0;
+          return H % e == 0 && (int64_t)((uintptr_t)table % w) == 0 && row_stride * (int64_t)sizeof(W) % w == 0 &&
+                 (int64_t)((uintptr_t)out % o) == 0;
         };
         if (fits(8)) {
           int shift = 0;
@@ -715,8 +720,8 @@ void lookup(const Ids& ids, const void* table, DType table_type, int64_t rows, i
           BAGUA_CHECK(slices < 65536, Tensor, "embedding: " << H << " columns");
           const bool many = ids.n * H >= kManyElements;
           const dim3 grid((unsigned)ceil_div(ids.n, (int64_t)(kThreads >> shift) * (many ? kRowsAhead : 1)), (unsigned)slices);
-          launch_overlapped(many ? lookup_kernel<Id, W, O, kRowsAhead> : lookup_kernel<Id, W, O, 1>, grid, dim3(kThreads), s, (const Id*)ids.data, (const W*)table, rows, row_stride, (O*)out, ids.n,
-                            H, shift, scale, encoder_ops::index_report());
+          launch_overlapped(many ? lookup_kernel<Id, W, O, kRowsAhead> : lookup_kernel<Id, W, O, 1>, grid, dim3(kThreads), s,
+                            (const Id*)ids.data, (const W*)table, rows, row_stride, (O*)out, ids.n, H, shift, scale, encoder_ops::index_report());
         } else {
           launch_overlapped(fits(2) ? lookup_any_kernel<Id, W, O, 2> : lookup_any_kernel<Id, W, O, 1>, dim3((unsigned)ceil_div(ids.n, kThreads / 32)),
                             dim3(kThreads), s, (const Id*)ids.data, (const W*)table, rows, row_stride, (O*)out, ids.n, H, scale,

@@ -261,11 +261,12 @@ __device__ __forceinline__ int turns_of_step(const RowPart& r) {
 // ---- alternatives -------------------------------------------------------------------------------
 // The `top` largest of a group of threads' values, equal ones in the order of their ids, -inf and NaN not among them.
 //
-// A list kept along the way costs ten times the pass itself (64 rows of 131072, 20 alternatives: 90 us; now 15, without them 7).  Here the pass leaves
-// the largest value of every few vectors of a thread.  From the threads' largest ones comes a floor that at least `top` values reach, and in
-// rows that are not ordered few more: the least, over the warps, of the top / warps-th largest of a warp's lanes.  The vectors
+// A list kept along the way costs ten times the pass itself (64 rows of 131072, 20 alternatives: 90 us; now 15, without them 7).
+// Here the pass leaves the largest value of every few vectors of a thread.  From the threads' largest ones comes a floor that at least
+// `top` values reach, and in rows that are not ordered few more: the least, over the warps, of the top / warps-th largest of a warp's lanes.  The vectors
 // whose largest value reaches the floor are read again, the values that do are collected, and put in order by counting, for each, the
-// better ones.
+// better ones.  Where that collects too many, as in a row with a few hundred tokens left, all neighbours, the floor is the top-th largest of all
+// threads' values, and where that does too, values being equal, one alternative is looked for after the other.
 //
 // A candidate is one number: its value in the order of whole numbers, then its id from the last to the first.
 using Key = unsigned long long;
@@ -293,7 +294,7 @@ struct TopScratch {
   Key found[kRoom];
   int reach[kRoom];  // the first vectors of steps with a value that reaches the floor
   float step[kSteps<kGroup>][kGroup];
-  float floor[kGroup / 32];
+  float floor[kGroup / 32], largest[kGroup];
   int count, steps;
 };
 
@@ -310,28 +311,14 @@ __device__ __forceinline__ void each_value(const T* x, const RowPart& r, F&& f) 
   }
 }
 
-// The group's best into best[0 .. top), kNoKey where there are no more; `largest`: of this thread's values.  All threads of the group.
+// Collects the values of a part that reach the floor, and returns how many there are, kRoom + 1 for any number above kRoom, of which not all are in
+// s.found.  `largest`: of this thread's values.  All threads of the group; s.count and s.steps are 0.
 template <typename T, int kGroup>
-__device__ __forceinline__ void choose(const T* x, const RowPart& r, int top, float largest, TopScratch<kGroup>& s, Key* best) {
-  constexpr int kVec = 16 / sizeof(T), kGroupWarps = kGroup / 32;
-  const int tid = (int)threadIdx.x % kGroup, lane = tid & 31;
-  {
-    int before = 0;  // lanes with larger values, or equal ones in front
-#pragma unroll
-    for (int k = 0; k < 32; ++k) {
-      const float v = __shfl_sync(kFull, largest, k);
-      before += (int)(v > largest) | ((int)(v == largest) & (int)(k < lane));
-    }
-    if (before == (top - 1) / kGroupWarps) s.floor[tid >> 5] = largest;
-  }
-  if (tid == 0) s.count = s.steps = 0;
-  for (int k = tid; k < top; k += kGroup) best[k] = kNoKey;
-  sync_group<kGroup>();
-  float floor = s.floor[0];
-#pragma unroll
-  for (int k = 1; k < kGroupWarps; ++k) floor = fminf(floor, s.floor[k]);
+__device__ __forceinline__ int collect(const T* x, const RowPart& r, float floor, float largest, TopScratch<kGroup>& s) {
+  constexpr int kVec = 16 / sizeof(T);
+  const int tid = (int)threadIdx.x % kGroup;
   // the steps that reach the floor, dealt out to all threads: a thread's own would wait for one another
-  const int turns = turns_of_step<kGroup>(r), vectors = turns * kAhead;
+  const int vectors = turns_of_step<kGroup>(r) * kAhead;
   if (largest >= floor && largest > -INFINITY) {
     if (tid < r.rest) {
       const float v = to_float(x[r.outside(tid)]);
@@ -370,7 +357,44 @@ __device__ __forceinline__ void choose(const T* x, const RowPart& r, int top, fl
     }
   }
   sync_group<kGroup>();
-  const int count = steps <= kRoom ? s.count : kRoom + 1;  // each step has a value
+  return steps <= kRoom ? min(s.count, kRoom + 1) : kRoom + 1;
+}
+
+// The group's best into best[0 .. top), kNoKey where there are no more; `largest`: of this thread's values.  All threads of the group.
+template <typename T, int kGroup>
+__device__ __forceinline__ void choose(const T* x, const RowPart& r, int top, float largest, TopScratch<kGroup>& s, Key* best) {
+  constexpr int kGroupWarps = kGroup / 32;
+  const int tid = (int)threadIdx.x % kGroup, lane = tid & 31;
+  {
+    int before = 0;  // lanes with larger values, or equal ones in front
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      const float v = __shfl_sync(kFull, largest, k);
+      before += (int)(v > largest) | ((int)(v == largest) & (int)(k < lane));
+    }
+    if (before == (top - 1) / kGroupWarps) s.floor[tid >> 5] = largest;
+  }
+  if (tid == 0) s.count = s.steps = 0;
+  for (int k = tid; k < top; k += kGroup) best[k] = kNoKey;
+  if constexpr (kGroupWarps > 1) s.largest[tid] = largest;
+  sync_group<kGroup>();
+  float floor = s.floor[0];
+#pragma unroll
+  for (int k = 1; k < kGroupWarps; ++k) floor = fminf(floor, s.floor[k]);
+  int count = collect<T, kGroup>(x, r, floor, largest, s);
+  if constexpr (kGroupWarps > 1) {
+    if (count > kRoom) {
+      sync_group<kGroup>();  // everybody has read the counts
+      int before = 0;
+#pragma unroll 8
+      for (int k = 0; k < kGroup; ++k) before += (int)(s.largest[k] > largest) | ((int)(s.largest[k] == largest) & (int)(k < tid));
+      if (before == top - 1) s.floor[0] = largest;
+      if (tid == 0) s.count = s.steps = 0;
+      sync_group<kGroup>();
+      const float higher = s.floor[0];
+      if (higher > floor) count = collect<T, kGroup>(x, r, higher, largest, s);
+    }
+  }
   if (count <= kRoom) {
     // four lanes share a candidate
     for (int base = 0; base < count; base += kGroup / 4) {
@@ -386,7 +410,6 @@ __device__ __forceinline__ void choose(const T* x, const RowPart& r, int top, fl
     sync_group<kGroup>();
     return;
   }
-  // Too many of one value: one alternative after the other, each the best behind the one before.
   Key last = ~0ull;
   for (int k = 0; k < top; ++k) {
     Key mine = kNoKey;

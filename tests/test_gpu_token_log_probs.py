@@ -52,6 +52,19 @@ def test_alternatives_in_every_order(top):
             host.check(x, torch.tensor([0, 1, 2, 3, 4, 0]), top, backward=False)
 
 
+@pytest.mark.parametrize("vocab", [5000, 30522, 131072])
+@pytest.mark.parametrize("left", [1, 19, 300, 1200])
+def test_alternatives_of_few_neighbouring_tokens(vocab, left):
+    """Rows of which a mask leaves tokens that are neighbours: the threads of a few warps hold them all."""
+    g = torch.Generator().manual_seed(left)
+    for n in (1, 3, 700 if vocab < 10000 else 40):
+        x = torch.full((n, vocab), -INF)
+        first = torch.randint(0, vocab - left, (n,), generator=g)
+        for i in range(n):
+            x[i, first[i]:first[i] + left] = torch.randn(left, generator=g)
+        host.check(x.bfloat16().cuda(), first + left // 2, 20, backward=False)
+
+
 def test_special_rows():
     host.check_special("cuda")
 
