@@ -60,6 +60,13 @@ def main():
         backend.mark_communication_ready(solo.tensors()[0], 0)
         backend.wait_pending_comm_ops()
 
+    v = torch.zeros_like(x)
+    m8, v8, scales8 = ops.adamw_state8(x)
+    logits = x.view(-1, 32768) if n % 32768 == 0 else x.view(1, -1)
+    targets = torch.zeros(logits.shape[0], dtype=torch.int64, device="cuda")
+    table = x.view(-1, 1024)
+    ids = torch.randperm(table.shape[0], device="cuda")
+
     cases = {
         # name: (callable, algorithmic bytes)
         "add": (lambda: ops.add_inplace(x, y), 3 * S),
@@ -69,6 +76,10 @@ def main():
         "reduce_chunk": (lambda: ops.reduce_chunk_inplace(x, n_chunks, 0, average=True), S + S // n_chunks),
         "async_average": (lambda: ops.async_model_average(x, y, m, 8), 4 * S),
         "sgd": (lambda: ops.sgd_momentum_flat(x, y, m, 1e-6, 0.9), 5 * S),
+        "adamw": (lambda: ops.adamw_step([out], [y], [m], [v], step=1, lr=1e-6), 7 * S),
+        "adamw8": (lambda: ops.adamw_step([out], [y], [m8], [v8], step=1, lr=1e-6, scales=[scales8]), 4 * S),
+        "token_log_probs": (lambda: ops.token_log_probs(logits, targets), S),
+        "embedding": (lambda: ops.embedding(ids, table), 2 * S),
         # the input once and 1 byte per element out (a second read of what did not stay on chip is not counted)
         "compress": (lambda: bx.compress("MinMaxUInt8", n_chunks, -1), S + S // 4),
         "decompress": (lambda: bo.decompress_from("MinMaxUInt8", n_chunks, comp), S // 4 + S),
