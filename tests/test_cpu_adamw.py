@@ -400,6 +400,53 @@ def _wrapped(rank, world, bits, shadow):
     return flat, copies, steps, kinds
 
 
+def _resumed(rank, world, bits):
+    import bagua_core_b200.parallel as P
+    from bagua_core_b200.models import MLP
+
+    def make():
+        torch.manual_seed(7)
+        model = MLP(16, 33, 5, depth=3)
+        return model, P.FlatAdamW(model.parameters(), lr=1e-2, state_bits=bits, seed=3)
+
+    def wrap(model, opt):
+        return P.with_bagua(model, [opt], P.GradientAllReduceAlgorithm(), bucket_bytes=4096)
+
+    def run(bm, opt, steps):
+        for s in steps:
+            opt.zero_grad()
+            torch.nn.functional.mse_loss(bm(xs[s, rank * bs:(rank + 1) * bs]), ys[s, rank * bs:(rank + 1) * bs]).backward()
+            opt.step()
+
+    P.init_process_group(torch.device("cpu"))
+    xs, ys = _batches(world)
+    bs = xs.shape[1] // world
+    model, opt = make()
+    bm = wrap(model, opt)
+    run(bm, opt, range(3))
+    saved = copy.deepcopy(model.state_dict()), copy.deepcopy(opt.state_dict())
+    run(bm, opt, range(3, 6))
+    out = []
+    for m, o in ((model, opt), make(), make()):
+        if m is not model:
+            first = not out[1:]  # the state is loaded before the buckets are laid out, and after
+            w = None if first else wrap(m, o)
+            m.load_state_dict(saved[0])
+            o.load_state_dict(saved[1])
+            run(w or wrap(m, o), o, range(3, 6))
+        out.append([p.detach().clone() for p in m.parameters()] + [x for p in m.parameters() for x in o.moments(p)])
+    P.destroy_process_group()
+    return out
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_training_goes_on_from_a_checkpoint(bits):
+    from mp_util import run_ranks
+
+    for a, b, c in run_ranks(_resumed, 2, args=(bits,)):
+        assert all(torch.equal(x, y) for x, y in zip(a, b)) and all(torch.equal(x, y) for x, y in zip(a, c))
+
+
 def _decentralized(rank, world):
     import bagua_core_b200.parallel as P
     from bagua_core_b200.models import MLP
