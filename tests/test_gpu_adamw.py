@@ -73,6 +73,30 @@ def test_host_and_gpu_give_the_same_bits(bits, count, size):
             assert ((p - q).abs() <= 3 * (2 * host.U * q.abs() + 2.0 ** -21 * 10 * host.HYPER["lr"])).all() and torch.equal(d, q.bfloat16())
 
 
+@pytest.mark.parametrize("size,eps", [(1e6, 1e-8), (1e17, 1e-8), (1.0, 1e-12), (1e-18, 1e-30), (3e3, 0.0)])
+def test_scales_and_eps_of_any_size(size, eps):
+    """8-bit moments whose scales leave the range of the short way, or an eps that a subnormal root counts next to: the host's bits."""
+    got = []
+    for device in ("cpu", "cuda"):
+        ps, gs, _, _ = host.tensors([3000, 5], (torch.float32, torch.float32), "cpu")
+        gs = [g * size for g in gs]
+        gs[0][1000:1512] /= size  # two blocks of ordinary size among them
+        ps, gs = [p.to(device) for p in ps], [g.to(device) for g in gs]  # (the framework's division rounds by device)
+        state = [ops.adamw_state8(p) for p in ps]
+        ms, vs, ss = ([s[i] for s in state] for i in range(3))
+        for t in (1, 2, 3):
+            ops.adamw_step(ps, gs, ms, vs, step=t, lr=1e-2, eps=eps, scales=ss, seed=1)
+        got.append(([x.cpu() for x in ms + vs + ss], [p.cpu() for p in ps]))
+    # (blocks whose second moment is not finite have the scale NaN, and codes that say nothing)
+    for k, (a, b) in enumerate(zip(got[0][0], got[1][0])):
+        assert torch.equal(a.nan_to_num(-1.0), b.nan_to_num(-1.0)), k
+    for p, q in zip(got[0][1], got[1][1]):
+        assert torch.equal(p.isfinite(), q.isfinite())
+        keep = p.isfinite()
+        # three steps, each off by a rounding of the parameter and 2^-21 of an update of at most 10 lr
+        assert ((p - q).abs()[keep] <= (3 * (2 * host.U * q.abs() + 2.0 ** -21 * 10 * 1e-2))[keep]).all()
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_captured_step_counts_on(bits):
     """A captured step with its number on the device, replayed, does what as many calls do; a number of the host is refused."""
