@@ -59,6 +59,7 @@ SOURCES = [
     "kernels/conv_wgrad.cu",
     "kernels/model_ops_cpu.cc",
     "kernels/encoder_ops.cu",
+    "kernels/clusters.cc",
     "kernels/embedding.cu",
     "kernels/token_log_probs.cu",
     "kernels/adamw.cu",

@@ -1,0 +1,50 @@
+#include "clusters.h"
+
+#include <cuda_runtime.h>
+
+#include <map>
+#include <mutex>
+#include <tuple>
+
+namespace bagua {
+namespace kernels {
+
+int fitting_cluster(const void* kernel, int wanted, int threads, size_t shared, cudaStream_t s) {
+  using Key = std::tuple<const void*, int, int, size_t, unsigned long long>;
+  // (never given back: threads may outlive static objects)
+  static std::mutex& mu = *new std::mutex;
+  static std::map<Key, int>& known = *new std::map<Key, int>;
+  // a stream that is being captured is not asked for its id, which would end the capture
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const bool has_id = cudaStreamIsCapturing(s, &capturing) == cudaSuccess && capturing == cudaStreamCaptureStatusNone &&
+                      cudaStreamGetId(s, &id) == cudaSuccess;
+  if (!has_id) cudaGetLastError();
+  const Key key{kernel, wanted, threads, shared, id};
+  std::lock_guard<std::mutex> g(mu);
+  if (has_id)
+    if (const auto it = known.find(key); it != known.end()) return it->second;
+  int blocks = wanted;
+  for (; blocks > 1; blocks /= 2) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)blocks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int fit = 0;
+    if (cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) == cudaSuccess && fit > 0) break;
+    cudaGetLastError();
+  }
+  if (known.size() >= 1024) known.clear();
+  if (has_id) known[key] = blocks;
+  return blocks;
+}
+
+}  // namespace kernels
+}  // namespace bagua

@@ -11,6 +11,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "clusters.h"
 #include "embedding.h"
 #include "index_report.cuh"
 #include "launch.cuh"
@@ -285,8 +286,11 @@ __global__ void __launch_bounds__(kThreads)
 // the block's tokens in their order, and copies them, now neighbours for the most part, to where they belong.  (Stored one by one from
 // where they were, 8192 tokens a block took 20,600 cycles to get there, 3,400 so.)  12288 tokens: 13 us, 65536: 32, hidden behind the
 // clearing of a large gradient; through memory 200,000 take 52.
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortRounds = 8, kSortBlocks = 8;
-constexpr int64_t kSortTokens = (int64_t)kSortBlocks * kSortThreads * kSortRounds;
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortRounds = 8;
+// Blocks of a cluster at most: 8, or 16 where so many tokens are left for each that it pays (us of 65536 tokens' whole gradient, 1000 x 64:
+// 46.7, 53.5 with 8; but 13.3 for 256 tokens, and 16.0 by a kernel that may form clusters of 16).  More tokens than they hold go through memory.
+constexpr int kSortBlocks = 8, kSortBlocksMany = 16;
+constexpr int64_t kSortMany = 32768, kSortTokens = (int64_t)kSortBlocksMany * kSortThreads * kSortRounds;
 // A block of it clears so many bytes itself, in about a microsecond; a launch of its own for that would cost two.
 constexpr int64_t kSmallClear = 128 << 10;
 constexpr int kSortBits = 9, kSortDigits = 1 << kSortBits;  // of a pass at most: two for up to 2^18 - 1 rows
@@ -297,7 +301,7 @@ struct SortShared {
   uint32_t own[kSortDigits];
 };
 size_t sort_shared_bytes(int rounds) { return sizeof(SortShared) + (size_t)rounds * kSortThreads * 2 * sizeof(uint2); }
-template <typename Id>
+template <typename Id, int kMaxBlocks>
 __global__ void __launch_bounds__(kSortThreads)
     sort_kernel(const Id* __restrict__ ids, Keys key, int n, int bits, int digit_bits, int rounds, uint32_t* __restrict__ keys_out,
                 uint32_t* __restrict__ places_out, uint32_t* __restrict__ zero, uint4* __restrict__ clear_at, int64_t clear_bytes) {
@@ -350,7 +354,7 @@ __global__ void __launch_bounds__(kSortThreads)
     uint32_t before = 0, all = 0, mine = 0, up = 0, own_up = 0;
     if (tid < digits) {
 #pragma unroll
-      for (int b = 0; b < kSortBlocks; ++b) {
+      for (int b = 0; b < kMaxBlocks; ++b) {
         const uint32_t c = b < blocks ? cluster.map_shared_rank(s.count, b)[tid] : 0u;
         before += b < rank ? c : 0u;
         mine = b == rank ? c : mine;
@@ -625,33 +629,51 @@ Plan plan(int64_t n, int64_t H) {
   return p;
 }
 
+// Lets a kernel have more shared memory, and with `large` form larger clusters, than any may; once for each device.
+template <typename K>
+void allow_large(K kernel, size_t bytes, bool large, std::atomic<bool> (&allowed)[64]) {
+  int device = 0;
+  BAGUA_CUDA_CHECK(cudaGetDevice(&device));
+  if (device < 64 && allowed[device].load(std::memory_order_acquire)) return;
+  BAGUA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  if (large) BAGUA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  if (device < 64) allowed[device].store(true, std::memory_order_release);
+}
+
 template <typename Id>
 int sort(const Ids& ids, Keys key, const Plan& p, uint32_t* buffers, uint32_t* counts, uint32_t* zero, void* clear_at, int64_t clear_bytes,
          const uint32_t** keys, const uint32_t** places, cudaStream_t s) {
   const int64_t n = ids.n;
   int bits = 1;
   while (bits < 32 && (key.rows >> bits) != 0) ++bits;
-  if (n <= kSortTokens) {
-    int blocks = 1;
-    while (blocks < kSortBlocks && (int64_t)blocks * kSortThreads < n) blocks *= 2;
-    const int rounds = (int)ceil_div(n, (int64_t)blocks * kSortThreads);
-    const size_t shared = sort_shared_bytes(rounds);
+  const int passes = (bits + kSortBits - 1) / kSortBits;
+  const int digit_bits = std::max(5, (bits + passes - 1) / passes);  // whole warps of digits
+  // In one launch, by as many blocks as there is work for and the stream's context has room for; -1: not by this kernel.
+  auto in_cluster = [&](auto most) {
+    auto* kernel = sort_kernel<Id, decltype(most)::value>;
     static std::atomic<bool> allowed[64];
-    int device = 0;
-    BAGUA_CUDA_CHECK(cudaGetDevice(&device));
-    if (device >= 64 || !allowed[device].load(std::memory_order_acquire)) {
-      BAGUA_CUDA_CHECK(cudaFuncSetAttribute(sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sort_shared_bytes(kSortRounds)));
-      if (device < 64) allowed[device].store(true, std::memory_order_release);
+    allow_large(kernel, sort_shared_bytes(kSortRounds), most > 8, allowed);
+    int blocks = 1;
+    while (blocks < most && (int64_t)blocks * kSortThreads < n) blocks *= 2;
+    for (; blocks >= 1; blocks /= 2) {
+      const int64_t rounds = ceil_div(n, (int64_t)blocks * kSortThreads);
+      if (rounds > kSortRounds) return -1;
+      const size_t shared = sort_shared_bytes((int)rounds);
+      if (fitting_cluster((const void*)kernel, blocks, kSortThreads, shared, s) != blocks) continue;
+      const bool small = clear_bytes <= kSmallClear * blocks;
+      launch_clusters_shared(kernel, 1, blocks, dim3(kSortThreads), shared, s, (const Id*)ids.data, key, (int)n, bits, digit_bits, (int)rounds,
+                             buffers, buffers + n, zero, (uint4*)(small ? clear_at : nullptr), clear_bytes);
+      if (clear_at && !small) clear(clear_at, clear_bytes, s);
+      *keys = buffers;
+      *places = buffers + n;
+      return clear_at && !small ? 2 : 1;
     }
-    const int passes = (bits + kSortBits - 1) / kSortBits, digit_bits = std::max(5, (bits + passes - 1) / passes);  // whole warps of digits
-    const bool small = clear_bytes <= kSmallClear * blocks;
-    launch_clusters_shared(sort_kernel<Id>, 1, blocks, dim3(kSortThreads), shared, s, (const Id*)ids.data, key, (int)n, bits,
-                           digit_bits, rounds, buffers, buffers + n, zero, (uint4*)(small ? clear_at : nullptr), clear_bytes);
-    if (clear_at && !small) clear(clear_at, clear_bytes, s);
-    *keys = buffers;
-    *places = buffers + n;
-    return clear_at && !small ? 2 : 1;
-  }
+    return -1;
+  };
+  if (n > kSortMany && n <= kSortTokens)
+    if (const int launches = in_cluster(std::integral_constant<int, kSortBlocksMany>{}); launches > 0) return launches;
+  if (n <= (int64_t)kSortBlocks * kSortThreads * kSortRounds)
+    if (const int launches = in_cluster(std::integral_constant<int, kSortBlocks>{}); launches > 0) return launches;
   uint32_t* k[2] = {buffers, buffers + 2 * n};
   const uint32_t *in_k = nullptr, *in_p = nullptr;
   int launches = 0, to = 0;

@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "clusters.h"
 #include "index_report.cuh"
 #include "launch.cuh"
 #include "token_log_probs.h"
@@ -797,7 +798,9 @@ void launch_forward(const ForwardArgs<T>& a, cudaStream_t s) {
     launch_overlapped(forward_short_kernel<T, kTop>, dim3((unsigned)((a.rows + kWarps - 1) / kWarps)), dim3(kThreads), s, a);
     return;
   }
-  const int shift = forward_shift<T>(a.rows, a.vocab);
+  int shift = forward_shift<T>(a.rows, a.vocab);
+  if (shift > 0)
+    for (int fit = fitting_cluster((const void*)forward_kernel<T, kTop, kThreads>, 1 << shift, kThreads, 0, s); 1 << shift > fit;) --shift;
   if (shift > 0)
     launch_clusters(forward_kernel<T, kTop, kThreads>, (int)a.rows, 1 << shift, dim3(kThreads), s, a, shift);
   else if (a.rows >= kManyRows && (int64_t)a.vocab * (int64_t)sizeof(T) <= kSmallRow)

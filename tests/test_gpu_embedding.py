@@ -27,7 +27,7 @@ def test_types(table_type, out_type, H):
 
 # rows around the ends of a digit, tokens around those of a tile, a chunk and a block
 @pytest.mark.parametrize("n,rows", [(1, 1), (1, 300), (31, 7), (32, 255), (33, 256), (1023, 257), (1024, 65535), (1025, 65536), (2048, 65537),
-                                    (2049, 3), (8192, 1), (8193, 1000), (12288, 30522), (65536, 5000), (65537, 511), (150001, 20000)])
+                                    (2049, 3), (8192, 1), (8193, 1000), (12288, 30522), (65536, 5000), (65537, 511), (131072, 4001), (131073, 70000), (150001, 20000)])
 @pytest.mark.parametrize("how", ["any", "few", "one", "ordered"])
 def test_tokens_and_rows(n, rows, how):
     host.check("cuda", n, rows, 16, how=how)
@@ -89,7 +89,7 @@ def test_ids_outside_the_table(n):
     ops.embedding(ids, w)
 
 
-@pytest.mark.parametrize("n", [300, 20000])
+@pytest.mark.parametrize("n", [300, 20000, 140000])
 def test_added_to_the_gradient_in_place(n):
     """With `wgrad.enabled` the rows that occur are added to `.grad`; the others are not touched."""
     wgrad.enabled = True
@@ -110,6 +110,25 @@ def test_added_to_the_gradient_in_place(n):
     w.grad = None
     (ops.embedding(ids, w).sum() + ops.embedding(ids, w).sum()).backward()
     assert torch.equal(w.grad, 2 * count.float().expand(1000, 24))
+
+
+def test_contexts_of_few_sms():
+    """Green contexts run smaller clusters, or none of this size: fewer blocks sort, or the tokens go through memory."""
+    green = pytest.importorskip("torch.cuda.green_contexts")
+    torch.cuda.synchronize()
+    try:
+        contexts = [green.GreenContext.create(sms, 0) for sms in (8, 16, 32)]
+    except RuntimeError as e:
+        pytest.skip(str(e))
+    for context in contexts:
+        context.set_context()
+        try:
+            for n in (100, 5000, 40000, 70000, 131072):
+                host.check("cuda", n, 3000, 16, how="few")
+            torch.cuda.synchronize()
+        finally:
+            context.pop_context()
+    host.check("cuda", 40000, 3000, 16, how="few")
 
 
 def test_captured_and_replayed_beside_another_stream():

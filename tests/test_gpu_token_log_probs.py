@@ -115,6 +115,25 @@ def test_gradients_that_are_not_contiguous():
     assert torch.equal(c.view(64, 5000), want)
 
 
+def test_contexts_of_few_sms():
+    """Green contexts may run smaller clusters: a row is split over fewer blocks."""
+    green = pytest.importorskip("torch.cuda.green_contexts")
+    torch.cuda.synchronize()
+    try:
+        contexts = [green.GreenContext.create(sms, 0) for sms in (8, 16)]
+    except RuntimeError as e:
+        pytest.skip(str(e))
+    for context in contexts:
+        context.set_context()
+        try:
+            for n in (1, 40):
+                check(n, 30522, torch.bfloat16, top=9)
+                check(n, 131072, torch.float32, top=32)
+            torch.cuda.synchronize()
+        finally:
+            context.pop_context()
+
+
 def test_changed_logits_are_noticed():
     x = torch.randn(3, 5000, device="cuda", requires_grad=True)
     y = x * 2
