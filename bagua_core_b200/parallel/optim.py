@@ -261,11 +261,15 @@ class FlatAdamW(_FlatOptimizer):
     `seed` is that of their rounding, the same on all ranks.  `moments(p)` reads a parameter's moments.
 
     The state of a parameter (`state[p]`, `state_dict()`, `load_state_dict()`) is `step` with `exp_avg` and `exp_avg_sq`, to which
-    8 bits add `scales`; it goes along when a bucket is laid out (again).  A step cannot be captured into a CUDA graph,
-    since its number is counted on the host; `bagua_core_b200.ops.adamw_step` takes one that lies on the device."""
+    8 bits add `scales`; it goes along when a bucket is laid out (again).
+
+    `capturable=True`: the steps of the flat buffers are counted on the device, so that `step()` can be captured into a CUDA
+    graph and replayed (with the learning rates that it was captured with).  It is captured again after a new layout, and after a
+    loaded state whose parameters differ in their numbers of steps.  Otherwise, and for parameters outside any bucket, a step that
+    is being captured is refused."""
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
-                 weight_decay: float = 1e-2, bf16_shadow: bool = False, state_bits: int = 32, seed: int = 0):
+                 weight_decay: float = 1e-2, bf16_shadow: bool = False, state_bits: int = 32, seed: int = 0, capturable: bool = False):
         if lr < 0 or eps < 0 or weight_decay < 0 or not all(0 <= b < 1 for b in betas):
             raise ValueError("AdamW needs lr, eps and weight_decay of 0 or more and betas from 0 to below 1")
         if state_bits not in (8, 32):
@@ -275,6 +279,9 @@ class FlatAdamW(_FlatOptimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay), bf16_shadow)
         self.state_bits = state_bits
         self.seed = seed
+        self.capturable = capturable
+        self._device_steps = None                # of the plan's groups, where they are counted on the device
+        self._earlier_device_steps = []          # that a graph may still hold
         self._plan_groups: List[List[int]] = []  # [parameter group, steps done] of each group of the plan
         self._plan_group_of = {}                 # id(parameter in the flat buffers) -> index of its group there
         self._plan_tensors = 0
@@ -336,10 +343,21 @@ class FlatAdamW(_FlatOptimizer):
                 plan.add(*(x[lo:hi] for x in flats), scales, f["h"][lo:hi] if "h" in f else None, k)
             self._plan_tensors += len(pieces)
             plan.add_grad_buffer(f["g"])
+        if self.capturable:
+            steps = torch.tensor([done for _, done in self._plan_groups], dtype=torch.int64, device=self._flat[0]["p"].device)
+            if self._device_steps is not None and self._device_steps.shape == steps.shape and self._device_steps.device == steps.device:
+                self._device_steps.copy_(steps)  # a captured step goes on counting there
+            else:
+                if self._device_steps is not None:
+                    self._earlier_device_steps.append(self._device_steps)
+                self._device_steps = steps
         return plan
 
     def _sync_steps(self):
         """The steps that the plan has counted, into the parameters' state."""
+        if self._device_steps is not None and self._flat:
+            for group, done in zip(self._plan_groups, self._device_steps.tolist()):
+                group[1] = done
         for f in self._flat:
             for p, _, _ in f["owners"]:
                 if p in self.state:
@@ -400,9 +418,12 @@ class FlatAdamW(_FlatOptimizer):
             for gi, done in self._plan_groups:
                 g = self.param_groups[gi]
                 values.append((g["lr"], *g["betas"], g["eps"], g["weight_decay"]))
-            self.kernel_launches += self._plan.step(values, [done + 1 for _, done in self._plan_groups], self.seed)
-            for group in self._plan_groups:
-                group[1] += 1
+            if self.capturable:
+                self.kernel_launches += self._plan.step(values, self._device_steps.add_(1), self.seed)
+            else:
+                self.kernel_launches += self._plan.step(values, [done + 1 for _, done in self._plan_groups], self.seed)
+                for group in self._plan_groups:
+                    group[1] += 1
         if self._shadowed and not self.shadows_valid:
             self._validate_shadows()
         self._step_loose()

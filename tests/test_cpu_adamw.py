@@ -508,3 +508,42 @@ def test_flat_adamw_on_buckets(bits, shadow):
     else:
         # rounded moments: an update is off by less than an eighth and a thirty-second of itself at each of 6 steps of about lr
         assert ((res[0][0] - want).abs() <= 6 * 2e-2).all() and (res[0][0] - want).abs().mean() <= 6 * 1e-2 * (1 / 8 + 1 / 32)
+
+
+def _device_counted(rank, world, bits):
+    import bagua_core_b200.parallel as P
+    from bagua_core_b200.models import MLP
+
+    P.init_process_group(torch.device("cpu"))
+    xs, ys = _batches(world)
+    bs = xs.shape[1] // world
+    out = []
+    for capturable in (False, True):
+        torch.manual_seed(7)
+        model = MLP(16, 33, 5, depth=3)
+        opt = P.FlatAdamW(model.parameters(), lr=1e-2, state_bits=bits, seed=3, capturable=capturable)
+        bm = P.with_bagua(model, [opt], P.GradientAllReduceAlgorithm(), bucket_bytes=4096)
+        for s in range(5):
+            if s == 2:
+                bm._reset()
+            if s == 3:  # parameters that differ in their numbers of steps
+                state = copy.deepcopy(opt.state_dict())
+                state["state"][0]["step"] = 1
+                opt.load_state_dict(state)
+            opt.zero_grad()
+            torch.nn.functional.mse_loss(bm(xs[s, rank * bs:(rank + 1) * bs]), ys[s, rank * bs:(rank + 1) * bs]).backward()
+            opt.step()
+        steps = [s["step"] for s in opt.state_dict()["state"].values()]
+        out.append([p.detach().clone() for p in model.parameters()] + [x for p in model.parameters() for x in opt.moments(p)] + [torch.tensor(steps)])
+    P.destroy_process_group()
+    return out
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_counted_on_the_device(bits):
+    """Counting them there changes nothing, also behind a new layout and a loaded state."""
+    from mp_util import run_ranks
+
+    for a, b in run_ranks(_device_counted, 2, args=(bits,)):
+        assert a[-1].tolist() == [3] + [5] * (len(a[-1]) - 1)
+        assert all(torch.equal(x, y) for x, y in zip(a, b))

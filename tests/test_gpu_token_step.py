@@ -94,3 +94,59 @@ def test_bert_with_many_tokens_looks_them_up_by_sorting(in_place):
     want = got[1][1].double()
     assert (got[0][1].double() - want).abs().max() <= 64 * 2.0 ** -24 * want.abs().max() + 2.0 ** -24 * want.norm()
     assert (got[0][1].double() - want).norm() <= 2.0 ** -20 * want.norm()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_optimizer_steps(bits):
+    """With `capturable=True` a captured step of the flat buffers, replayed, does what as many calls do, also behind a loaded state;
+    without it, it is refused."""
+    os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
+    os.environ.setdefault("MASTER_PORT", "29563")
+    dev = torch.device("cuda", 0)
+    g = torch.Generator().manual_seed(3)
+    P.init_process_group(dev)
+
+    def make(capturable):
+        torch.manual_seed(2)
+        model = tm.Model().to(dev)
+        biases = [p for n, p in model.named_parameters() if n.endswith("bias")]
+        weights = [p for n, p in model.named_parameters() if not n.endswith("bias")]
+        opt = P.FlatAdamW([{"params": weights}, {"params": biases, "weight_decay": 0.0}], lr=1e-2, state_bits=bits, capturable=capturable)
+        return model, opt, P.with_bagua(model, [opt], P.GradientAllReduceAlgorithm(), bucket_bytes=100 << 10)
+
+    eager, captured = make(False), make(True)
+    grads = [torch.randn(p.shape, generator=g).to(dev) for p in eager[0].parameters()]
+    for model, *_ in (eager, captured):
+        for p, x in zip(model.parameters(), grads):
+            p.grad.copy_(x)
+    graph = torch.cuda.CUDAGraph()
+    eager[1].step(), captured[1].step()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured[1].step()
+    for _ in range(3):
+        eager[1].step(), graph.replay()
+
+    def same():
+        torch.cuda.synchronize()
+        a, b = (o.state_dict()["state"] for o in (eager[1], captured[1]))
+        assert all(x["step"] == y["step"] for x, y in zip(a.values(), b.values()))
+        assert all(torch.equal(p, q) for p, q in zip(eager[0].parameters(), captured[0].parameters()))
+        assert all(torch.equal(x, y) for p, q in zip(eager[0].parameters(), captured[0].parameters())
+                   for x, y in zip(eager[1].moments(p), captured[1].moments(q)))
+        return {k: {n: v.clone() if isinstance(v, torch.Tensor) else v for n, v in x.items()} for k, x in a.items()}
+
+    saved = same()
+    assert {x["step"] for x in saved.values()} == {4}
+    eager[1].step(), graph.replay()
+    for _, opt, _ in (eager, captured):
+        opt.load_state_dict({"state": saved, "param_groups": opt.state_dict()["param_groups"]})
+    eager[1].step(), graph.replay()
+    assert {x["step"] for x in same().values()} == {5}
+    refused = torch.cuda.CUDAGraph()
+    x = torch.zeros(1, device=dev)
+    with torch.cuda.graph(refused):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="captured"):
+            eager[1].step()
+    P.destroy_process_group()
