@@ -92,7 +92,8 @@ void AdamWPlan::add(const at::Tensor& p, const at::Tensor& g, const at::Tensor& 
                                                                                                     << g.scalar_type());
   const at::ScalarType held = moments8 ? at::kByte : at::kFloat;
   BAGUA_CHECK(m.scalar_type() == held && v.scalar_type() == held, Tensor, "AdamW's moments are both float32, or both codes of 8 bits (uint8)");
-  BAGUA_CHECK(!p.is_neg() && !g.is_neg(), Tensor, "AdamW needs tensors that hold their values as they are, not negated views");
+  BAGUA_CHECK(!p.is_neg() && !g.is_neg() && !m.is_neg() && !v.is_neg(), Tensor,
+              "AdamW needs tensors that hold their values as they are, not negated views");
   BAGUA_CHECK(p.is_non_overlapping_and_dense(), Tensor, "AdamW needs parameters without gaps between their elements");
   for (const at::Tensor* t : {&g, &m, &v})
     BAGUA_CHECK(t->layout() == at::kStrided && t->device() == p.device() && same_layout(*t, p), Tensor,
@@ -100,7 +101,7 @@ void AdamWPlan::add(const at::Tensor& p, const at::Tensor& g, const at::Tensor& 
   BAGUA_CHECK(moments8 == (scales != nullptr), Tensor, "moments of 8 bits need scales, others have none");
   if (scales) check_scales(*scales, p.numel(), p.device());
   if (copy)
-    BAGUA_CHECK(copy->scalar_type() == at::kBFloat16 && copy->device() == p.device() && same_layout(*copy, p), Tensor,
+    BAGUA_CHECK(copy->scalar_type() == at::kBFloat16 && copy->device() == p.device() && same_layout(*copy, p) && !copy->is_neg(), Tensor,
                 "the copy must be a bfloat16 tensor of the parameter's sizes and strides on its device");
   BAGUA_CHECK(segs_.empty() || (device == device_ && types.p == types_.p && types.g == types_.g && types.moments8 == types_.moments8), Tensor,
               "the tensors of an AdamW step are of one kind: one device, one type of parameters, of gradients and of moments");
@@ -232,6 +233,8 @@ int adamw_read8(const TensorRefs& m, const TensorRefs& v, const TensorRefs& scal
                 Tensor, "moments are read from codes of 8 bits (uint8) into tensors of one type");
     BAGUA_CHECK(m[k]->is_non_overlapping_and_dense() && m[k]->device() == device, Tensor,
                 "moments are read from tensors without gaps, on one device");
+    BAGUA_CHECK(!m[k]->is_neg() && !v[k]->is_neg() && !m_out[k]->is_neg() && !v_out[k]->is_neg(), Tensor,
+                "moments are read from and into tensors that hold their values as they are, not negated views");
     for (const at::Tensor* t : {v[k], m_out[k], v_out[k]})
       BAGUA_CHECK(t->device() == device && same_layout(*t, *m[k]), Tensor, "moments and what they are read into have one size and layout, on one device");
     check_scales(*scales[k], m[k]->numel(), device);

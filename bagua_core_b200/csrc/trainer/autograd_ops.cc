@@ -698,6 +698,9 @@ struct EmbedNode : public EncoderNode {
 bool kernel_type(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
 DType kernel_dtype(at::ScalarType t) { return t == at::kFloat ? DType::F32 : t == at::kHalf ? DType::F16 : DType::BF16; }
 
+// Memory that holds the values as they are: a lazily negated view holds their opposites.
+at::Tensor as_held(const at::Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 at::Tensor lookup_composition(const at::Tensor& ids, const at::Tensor& table, double scale, int64_t padding, at::ScalarType type) {
   // ids outside the table: rows of NaN without a gradient
   const at::Tensor known = ids.ge(0).logical_and(ids.lt(table.size(0)));
@@ -732,7 +735,7 @@ struct LookupNode : public EncoderNode {
     if (!add && (n == 0 || table.numel() == 0)) {
       out[0] = at::zeros(table.sizes(), table.options());
     } else if (n > 0 && table.numel() > 0) {
-      const at::Tensor d = grads[0].contiguous();
+      const at::Tensor d = as_held(grads[0]).contiguous();
       if (!add) out[0] = fresh(table.sizes(), table.scalar_type(), table);
       // the framework's memory, not this package's pool: a graph that is being captured keeps it
       const at::Tensor scratch = fresh({(int64_t)embedding::backward_scratch_bytes(n, H)}, at::kByte, table);
@@ -809,7 +812,7 @@ std::vector<at::Tensor> top_composition(const at::Tensor& logits, const at::Tens
 
 // Logits as rows: [rows, vocab] with neighbouring columns, a view where there is one.
 at::Tensor logit_rows(const at::Tensor& logits) {
-  const at::Tensor x = logits.reshape({-1, logits.size(-1)});
+  const at::Tensor x = as_held(logits).reshape({-1, logits.size(-1)});
   return x.size(1) <= 1 || x.stride(1) == 1 ? x : x.contiguous();
 }
 
@@ -857,7 +860,7 @@ struct LogProbNode : public Node {
     }
     at::Tensor g[2];
     for (int k = 0; k < 2; ++k)
-      if (grads[k].defined()) g[k] = grads[k].reshape({-1});
+      if (grads[k].defined()) g[k] = as_held(grads[k]).reshape({-1});
     token_log_probs::backward({x.data_ptr(), kernel_dtype(x.scalar_type()), rows, vocab, x.stride(0)}, t.data_ptr<int64_t>(),
                               (const token_log_probs::RowStats*)st.data_ptr(), g[0].defined() ? g[0].data_ptr<float>() : nullptr,
                               g[0].defined() ? g[0].stride(0) : 0, g[1].defined() ? g[1].data_ptr<float>() : nullptr,
@@ -1158,8 +1161,8 @@ at::Tensor embedding(const at::Tensor& ids, const at::Tensor& table, double scal
   at::Tensor idc, y;
   {
     PlainDispatch plain;
-    idc = ids.contiguous();
-    const at::Tensor w = H <= 1 || table.stride(1) == 1 ? table : table.contiguous();
+    idc = as_held(ids).contiguous();
+    const at::Tensor held = as_held(table), w = H <= 1 || held.stride(1) == 1 ? held : held.contiguous();
     std::vector<int64_t> sizes = ids.sizes().vec();
     sizes.push_back(H);
     y = fresh(sizes, to, table);
@@ -1261,7 +1264,7 @@ std::vector<at::Tensor> token_log_probs(const at::Tensor& logits, const at::Tens
   {
     PlainDispatch plain;
     const at::Tensor x = logit_rows(logits);
-    t = targets.contiguous();
+    t = as_held(targets).contiguous();
     for (int k = 0; k < 2; ++k) out[k] = fresh(targets.sizes(), at::kFloat, x);
     if (top) {
       std::vector<int64_t> sizes = targets.sizes().vec();

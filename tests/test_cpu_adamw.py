@@ -547,3 +547,12 @@ def test_steps_counted_on_the_device(bits):
     for a, b in run_ranks(_device_counted, 2, args=(bits,)):
         assert a[-1].tolist() == [3] + [5] * (len(a[-1]) - 1)
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_negated_views_are_refused(which):
+    """The memory of a lazily negated view holds the opposites of its values."""
+    parts = [[torch._neg_view(torch.ones(8)) if k == which else torch.ones(8)] for k in range(4)]
+    assert parts[which][0].is_neg()
+    with pytest.raises(RuntimeError, match="negated views"):
+        ops.adamw_step(*parts, step=1, lr=0.1)

@@ -181,3 +181,17 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(y[-300:], w.detach()[ids[-300:]])
     (g,) = torch.autograd.grad(y, w, torch.ones_like(y))
     assert torch.equal(g, torch.bincount(ids, minlength=100)[:, None].float().expand(100, H).bfloat16())
+
+
+def test_negated_views():
+    """Lazily negated views, as the imaginary part of a conjugate is one: the table, and the gradient that comes back."""
+    g = torch.Generator().manual_seed(0)
+    z = torch.randn(9, 40, dtype=torch.complex64, generator=g).cuda()
+    table, ids = z.conj().imag, torch.tensor([3, 0, 3, 8], device="cuda")
+    assert table.is_neg()
+    assert torch.equal(ops.embedding(ids, table), -z.imag[ids])
+    w = torch.randn(9, 40, generator=g).cuda().requires_grad_()
+    d = torch.randn(4, 40, dtype=torch.complex64, generator=g).cuda()
+    ops.embedding(ids, w).backward(d.conj().imag)
+    want = torch.zeros(9, 40, device="cuda", dtype=torch.float64).index_add_(0, ids, -d.imag.double())
+    assert torch.equal(w.grad, want.float())  # sums of two values at most, rounded once

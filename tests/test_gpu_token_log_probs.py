@@ -194,3 +194,20 @@ def test_offsets_beyond_32_bits():
     z = x[-2:].detach().clone().requires_grad_()
     (e,) = torch.autograd.grad(ops.token_log_probs(z, t[-2:]).log_probs.sum(), z)
     assert ((d[-2:].double() - e.double()).abs() <= off + 2.0 ** -7 * e.double().abs()).all() and not d[1:-2].any() and d[0, 9] > 0.9
+
+
+def test_negated_views():
+    """Lazily negated views, as the imaginary part of a conjugate is one, are the values that they stand for."""
+    g = torch.Generator().manual_seed(0)
+    z = torch.randn(5, 333, dtype=torch.complex64, generator=g).cuda()
+    d = torch.randn(5, dtype=torch.complex64, generator=g).cuda()
+    t = torch.randint(0, 333, (5,), generator=g).cuda()
+    x, d = z.conj().imag, d.conj().imag
+    assert x.is_neg() and d.is_neg()
+    got = []
+    for logits, dy in ((x, d), (x.resolve_neg(), d.resolve_neg())):
+        logits = logits.detach().requires_grad_()
+        r = ops.token_log_probs(logits, t, top=3)
+        r[0].backward(dy)
+        got.append([*r, logits.grad])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
