@@ -1,5 +1,5 @@
 // See adamw.h.  Streams over memory: with fp32 parameters, gradients and moments 28 bytes an element, 16 with moments in 8 bits.
-// 131 M elements: 534 us with fp32 moments (6.95 TB/s, above the rate of a copy), 365 with 8 bits (5.8 TB/s; integer
+// 131 M elements: 534 us with fp32 moments (6.95 TB/s, above the rate of a copy), 358 with 8 bits (5.9 TB/s; integer
 // instructions are issued in three quarters of all cycles), 120 to read those into bf16 (6.6 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -130,16 +130,16 @@ __global__ void __launch_bounds__(kThreads) step32_kernel(const __grid_constant_
 // piece of memory; elements of an address that no vector fits are taken one by one, lane by lane.
 //
 // With 16 bytes an element instead of 28, instructions count as much as bytes (at 89 an element 67 M elements took 234 us).
-// So a warp takes several blocks one after the other, and what is asked once a tensor is asked once; two elements are computed by
-// one instruction where there is one; the square root and the reciprocal are the hardware's (within 2^-22 each: a
+// So two elements are computed by one instruction where there is one; the square root and the reciprocal are the hardware's (within 2^-22 each: a
 // parameter is off by that part of its update); the moments' betas go into the factor that decodes them, and both directions of coding take
 // one factor.  A block with a scale beyond kPlainScale, or an eps so small that a subnormal square root counts next to
-// it, goes the longer way.
-constexpr int kTurns8 = 2;  // blocks of a warp; us with 1, 2, 4: 131 M elements in fp32 353, 363, 363, in bf16 356, 333, 328; 10 M 32.4, 31.6, 34.1
-// Blocks on an SM: so many leave 40 registers a thread and a few spilled ones.  131 M elements take 372 us, with five (48 registers)
-// 387, four (64) 421, three (80) 461: the loads of waiting warps are worth more than the spills cost.
+// it, goes the longer way.  To know which codes fp32 leaves open costs three instructions an element, and 2 % of the blocks, whose
+// codes are settled in 64 bits (with bf16 parameters and gradients 131 M elements take 364 us, without it 312; in fp32 358 and 353).
+// Blocks on an SM: so many leave 40 registers a thread and a few spilled ones.  131 M elements take 362 us, with five (48 registers)
+// 378, seven (32) 388: the loads of waiting warps are worth more than the spills cost.  A warp that took two blocks in turn held
+// more registers over the turn than it had: 434 us.
 constexpr int kResident8 = 6;
-constexpr int kTile8 = kThreads / 32 * kMoment8Block * kTurns8;
+constexpr int kTile8 = kThreads / 32 * kMoment8Block;
 constexpr float kPlainEps = 1e-10f;
 template <bool kPlain>
 __device__ __forceinline__ float root_of(float x) {
@@ -172,8 +172,41 @@ __device__ __forceinline__ float largest(float a, float b, float c) {
 }
 __device__ __forceinline__ Pair both(float x) { return pair(x, x); }
 
+// A block's codes and scales in 64 bits, by the whole warp: one block in forty.  (131 M elements: 358 us with two elements at a time,
+// 362 with one, 364 with four.)
+template <typename G>
+__device__ __forceinline__ void code_in_64_bits(const Segment& a, const Hyper& h, uint32_t key, int64_t block) {
+  const int lane = (int)threadIdx.x & 31;
+  const int64_t base = block * kMoment8Block;
+  const int n = (int)min((int64_t)kMoment8Block, a.n - base);
+  const G* g = (const G*)a.g + base;
+  uint8_t *m = (uint8_t*)a.m + base, *v = (uint8_t*)a.v + base;
+  const float ms = a.m_scale[block], vs = a.v_scale[block];
+  float top1 = 0.f, top2 = 0.f;
+#pragma unroll 2
+  for (int i = lane; i < n; i += 32) {
+    top1 = fmaxf(top1, (float)fabs(first64(h, to_float(g[i]), m[i], ms)));
+    top2 = fmaxf(top2, (float)second64(h, to_float(g[i]), v[i], vs));
+  }
+  double per1, per2;
+  const float new_ms = scale64(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top1))), kLargest1, &per1);
+  const float new_vs = scale64(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top2))), kLargest2, &per2);
+  if (lane == 0) {  // (all lanes have read the old ones)
+    a.m_scale[block] = new_ms;
+    a.v_scale[block] = new_vs;
+  }
+#pragma unroll 2
+  for (int i = lane; i < n; i += 32) {
+    const uint32_t random = random_bits(key, base + i);
+    const float gi = to_float(g[i]);
+    m[i] = (uint8_t)first_code64(first64(h, gi, m[i], ms), per1, random);
+    v[i] = (uint8_t)second_code64(second64(h, gi, v[i], vs), per2, random);
+  }
+}
+
+// Whether the block's codes and scales are settled, and written, too.
 template <typename P, typename G, bool kVec>
-__device__ __forceinline__ void step8_block(const Segment& a, const Hyper& h, uint32_t key, int64_t block) {
+__device__ __forceinline__ bool step8_block(const Segment& a, const Hyper& h, uint32_t key, int64_t block) {
   const int lane = (int)threadIdx.x & 31;
   const int64_t base = block * kMoment8Block;
   P* p = (P*)a.p + base;
@@ -245,13 +278,25 @@ __device__ __forceinline__ void step8_block(const Segment& a, const Hyper& h, ui
     step(std::true_type{});
   else
     step(std::false_type{});
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    if constexpr (kVec) {
+      store4(p + at(r, 0), pv[r]);
+      if (copy) store4(copy + base + at(r, 0), pv[r]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = at(r, e);
+        if (i >= n) continue;
+        p[i] = from_float<P>(pv[r][e]);
+        if (copy) copy[base + i] = __float2bfloat16_rn(pv[r][e]);
+      }
+    }
+  }
   float per_m, per_v;
   const float new_ms = block_scale(__reduce_max_sync(0xffffffffu, float_bits(top_m)), kLargest1, &per_m);
   const float new_vs = block_scale(__reduce_max_sync(0xffffffffu, float_bits(top_v)), kLargest2, &per_v);
-  if (lane == 0) {
-    a.m_scale[block] = new_ms;
-    a.v_scale[block] = new_vs;
-  }
+  uint32_t near1 = ~0u, near2 = ~0u;
   const uint32_t random = random_base(key, base) + (uint32_t)at(0, 0) * kStride;
   auto code = [&](auto plain) {
     constexpr bool kPlain = decltype(plain)::value;
@@ -269,8 +314,13 @@ __device__ __forceinline__ void step8_block(const Segment& a, const Hyper& h, ui
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
           const uint32_t bits = mix(random + (uint32_t)(at(r, e + o) - at(0, 0)) * kStride);
-          c1[e + o] = encode1(o ? y1.y : y1.x, mv[r][e + o], bits);
-          c2[e + o] = encode2(o ? y2.y : y2.x, vv[r][e + o], bits);
+          const uint32_t s1 = sum1(o ? y1.y : y1.x, bits), s2 = sum2(o ? y2.y : y2.x, bits);
+          c1[e + o] = cut1(s1, mv[r][e + o]);
+          c2[e + o] = cut2(s2, vv[r][e + o]);
+          if (kVec || at(r, e + o) < n) {
+            near1 = min(near1, above1(s1));
+            near2 = min(near2, above2(s2));
+          }
         }
       }
       mc[r] = c1[0] | c1[1] << 8 | c1[2] << 16 | c1[3] << 24;
@@ -281,25 +331,29 @@ __device__ __forceinline__ void step8_block(const Segment& a, const Hyper& h, ui
     code(std::true_type{});
   else
     code(std::false_type{});
+  if (__any_sync(0xffffffffu, near1 < kNear1 || near2 < kNear2) && new_ms < INFINITY && new_vs < INFINITY) {
+    return false;
+  }
+  if (lane == 0) {
+    a.m_scale[block] = new_ms;
+    a.v_scale[block] = new_vs;
+  }
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     if constexpr (kVec) {
-      store4(p + at(r, 0), pv[r]);
       *reinterpret_cast<uint32_t*>(m + at(r, 0)) = mc[r];
       *reinterpret_cast<uint32_t*>(v + at(r, 0)) = vc[r];
-      if (copy) store4(copy + base + at(r, 0), pv[r]);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = at(r, e);
         if (i >= n) continue;
-        p[i] = from_float<P>(pv[r][e]);
         m[i] = (uint8_t)(mc[r] >> (8 * e));
         v[i] = (uint8_t)(vc[r] >> (8 * e));
-        if (copy) copy[base + i] = __float2bfloat16_rn(pv[r][e]);
       }
     }
   }
+  return true;
 }
 template <typename P, typename G, int N>
 __global__ void __launch_bounds__(kThreads, kResident8) step8_kernel(const __grid_constant__ Table<N> table) {
@@ -309,16 +363,10 @@ __global__ void __launch_bounds__(kThreads, kResident8) step8_kernel(const __gri
   const Hyper h = table.on_device ? table.on_device[a.group] : table.hyper[a.group];
   const uint32_t key = segment_key(h.random, a.index);
   const bool vec = fours((P*)a.p) && fours((const G*)a.g) && fours((uint8_t*)a.m) && fours((uint8_t*)a.v) && fours((__nv_bfloat16*)a.copy);
-  // a tile's blocks in turn, so that its warps read neighbours at a time
-  int64_t block = (int64_t)(blockIdx.x - table.first_tile[k]) * (kTile8 / kMoment8Block) + (threadIdx.x >> 5);
-#pragma unroll 1
-  for (int turn = 0; turn < kTurns8; ++turn, block += kThreads / 32) {
-    if (block * kMoment8Block >= a.n) return;
-    if (vec && (block + 1) * kMoment8Block <= a.n)
-      step8_block<P, G, true>(a, h, key, block);
-    else
-      step8_block<P, G, false>(a, h, key, block);
-  }
+  const int64_t block = (int64_t)(blockIdx.x - table.first_tile[k]) * (kTile8 / kMoment8Block) + (threadIdx.x >> 5);
+  if (block * kMoment8Block >= a.n) return;
+  const bool settled = vec && (block + 1) * kMoment8Block <= a.n ? step8_block<P, G, true>(a, h, key, block) : step8_block<P, G, false>(a, h, key, block);
+  if (!settled) code_in_64_bits<G>(a, table.on_device ? table.on_device[a.group] : table.hyper[a.group], key, block);
 }
 
 // Buffers that start anywhere, slices of flat ones, for instance: how many elements further all of them hold four as one piece.  (60 M elements

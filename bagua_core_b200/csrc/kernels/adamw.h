@@ -14,6 +14,9 @@
 // away.  The random bits are a hash of (seed, step, tensor, element): a step can be repeated.  A second moment that is not zero
 // does not become zero, since the step divides by it: it is held at the smallest code, 2^-19 of its block's largest, or 2^-9.5 of the
 // largest root.  The step itself uses both moments before they are rounded.
+// Codes are those that the definition in 64 bits gives: a value that fp32 cannot tell from the border between two codes, given its
+// random bits, is computed again, with its block, in 64 bits.  (Where a first moment is a small difference of large terms, fp32 may
+// be further off than that.)  A code that went the other way would show for as long as moments are remembered, in the scales above all.
 // A block in which a moment is not finite has the scale NaN and reads as NaN.
 #pragma once
 
@@ -36,6 +39,7 @@ struct Hyper {
   float root;          // 1 / sqrt(1 - b2^t)
   float eps, b1, c1, b2, c2;  // c: 1 - b
   uint32_t random;     // 8 bits: what the tensors' keys come from
+  double beta1, beta2; // 8 bits: b1 and b2 for what is computed in 64
 };
 struct GroupValues {
   double lr, b1, b2, eps, weight_decay;

@@ -1,4 +1,5 @@
 // AdamW on host memory, and what host and device share: hyperparameters, which types there are.
+#include <algorithm>
 #include <cmath>
 #include <vector>
 
@@ -27,6 +28,7 @@ void step8(const Segment& a, const Hyper& h, int64_t block) {
   auto* g = (const typename G::T*)a.g;
   auto *m = (uint8_t*)a.m, *v = (uint8_t*)a.v;
   float mv[kMoment8Block], vv[kMoment8Block];
+  uint8_t mc[kMoment8Block], vc[kMoment8Block];
   uint32_t top_m = 0, top_v = 0;
   for (int64_t i = lo; i < hi; ++i) {
     float pv = P::ld(p + i), &mi = mv[i - lo], &vi = vv[i - lo];
@@ -40,14 +42,36 @@ void step8(const Segment& a, const Hyper& h, int64_t block) {
     top_v = vb > top_v ? vb : top_v;
   }
   float per_m, per_v;
-  const float ms = a.m_scale[block] = block_scale(top_m, kLargest1, &per_m);
-  const float vs = a.v_scale[block] = block_scale(top_v, kLargest2, &per_v);
+  float ms = block_scale(top_m, kLargest1, &per_m), vs = block_scale(top_v, kLargest2, &per_v);
   const uint32_t key = segment_key(h.random, a.index);
+  bool near = false;
   for (int64_t i = lo; i < hi; ++i) {
     const uint32_t random = random_bits(key, i);
-    m[i] = (uint8_t)encode1(scaled(std::fabs(mv[i - lo]), per_m, ms < kPlainScale), mv[i - lo], random);
-    v[i] = (uint8_t)encode2(scaled(vv[i - lo], per_v, vs < kPlainScale), vv[i - lo], random);
+    const uint32_t s1 = sum1(scaled(std::fabs(mv[i - lo]), per_m, ms < kPlainScale), random);
+    const uint32_t s2 = sum2(scaled(vv[i - lo], per_v, vs < kPlainScale), random);
+    mc[i - lo] = (uint8_t)cut1(s1, mv[i - lo]);
+    vc[i - lo] = (uint8_t)cut2(s2, vv[i - lo]);
+    near |= above1(s1) < kNear1 || above2(s2) < kNear2;
   }
+  if (near && ms < INFINITY && vs < INFINITY) {
+    double per1, per2;
+    float top1 = 0, top2 = 0;
+    for (int64_t i = lo; i < hi; ++i) {
+      top1 = std::max(top1, (float)std::fabs(first64(h, G::ld(g + i), m[i], a.m_scale[block])));
+      top2 = std::max(top2, (float)second64(h, G::ld(g + i), v[i], a.v_scale[block]));
+    }
+    ms = scale64(top1, kLargest1, &per1);
+    vs = scale64(top2, kLargest2, &per2);
+    for (int64_t i = lo; i < hi; ++i) {
+      const uint32_t random = random_bits(key, i);
+      mc[i - lo] = (uint8_t)first_code64(first64(h, G::ld(g + i), m[i], a.m_scale[block]), per1, random);
+      vc[i - lo] = (uint8_t)second_code64(second64(h, G::ld(g + i), v[i], a.v_scale[block]), per2, random);
+    }
+  }
+  std::copy(mc, mc + (hi - lo), m + lo);
+  std::copy(vc, vc + (hi - lo), v + lo);
+  a.m_scale[block] = ms;
+  a.v_scale[block] = vs;
 }
 
 template <typename P, typename G>

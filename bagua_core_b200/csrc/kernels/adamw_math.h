@@ -93,16 +93,22 @@ BAGUA_HD uint32_t sum_up_to(uint32_t a, uint32_t b, uint32_t most) {
   return a + b < most ? a + b : most;
 #endif
 }
-// Codes of y, at least 0, and of a moment x with the sign (first) or above 0 (second).  Neither sum leaves 32 bits, for a y that is not finite either.
+// y, at least 0, with random bits added.  Neither sum leaves 32 bits, for a y that is not finite either.
 constexpr uint32_t kLastBits = 0x07ffffffu;  // those of both largest codes, and of what is cut off
-BAGUA_HD uint32_t encode1(float y, float x, uint32_t random) {
-  return sum_up_to(float_bits(y), (random << 4 & 0xffff0u) | 8u, kLastBits) >> 20 | (float_bits(x) >> 24 & 0x80u);
-}
-BAGUA_HD uint32_t encode2(float y, float x, uint32_t random) {
-  const uint32_t c = sum_up_to(float_bits(y), (random >> 13 & 0x7fff8u) | 4u, kLastBits) >> 19;
-  const uint32_t least = float_bits(x) < 1u ? float_bits(x) : 1u;  // 1 unless x is 0
+BAGUA_HD uint32_t sum1(float y, uint32_t random) { return sum_up_to(float_bits(y), (random << 4 & 0xffff0u) | 8u, kLastBits); }
+BAGUA_HD uint32_t sum2(float y, uint32_t random) { return sum_up_to(float_bits(y), (random >> 13 & 0x7fff8u) | 4u, kLastBits); }
+// The codes, of a moment x with the sign (first) or above 0 (second).
+BAGUA_HD uint32_t cut1(uint32_t sum, float x) { return sum >> 20 | (float_bits(x) >> 24 & 0x80u); }
+BAGUA_HD uint32_t cut2(uint32_t sum, float x) {
+  const uint32_t c = sum >> 19, least = float_bits(x) < 1u ? float_bits(x) : 1u;  // 1 unless x is 0
   return c > least ? c : least;
 }
+// How far a sum lies above the last border but kSlack, all bits of what is cut off at the top: less than kNear1 or kNear2 if the border
+// is nearer than kSlack steps of fp32.  y is off by 15 half steps at most: the moments' 5 (a first moment without cancellation), the
+// scale's 6 (their largest's 4, the factor, the product) with its own two in the definition, its reciprocal and the product with it.
+constexpr uint32_t kSlack = 16, kNear1 = 2 * kSlack << 12, kNear2 = 2 * kSlack << 13;
+BAGUA_HD uint32_t above1(uint32_t sum) { return (sum << 12) + (kSlack << 12); }
+BAGUA_HD uint32_t above2(uint32_t sum) { return (sum << 13) + (kSlack << 13); }
 
 BAGUA_HD Hyper make_hyper(const GroupValues& g, int64_t step, uint64_t seed) {
   Hyper h;
@@ -115,6 +121,8 @@ BAGUA_HD Hyper make_hyper(const GroupValues& g, int64_t step, uint64_t seed) {
   h.b2 = (float)g.b2;
   h.c2 = (float)(1.0 - g.b2);
   h.random = step_random(seed, step);
+  h.beta1 = g.b1;
+  h.beta2 = g.b2;
   return h;
 }
 
@@ -137,6 +145,60 @@ BAGUA_HD float multiply_add(float a, float b, float c) {
 BAGUA_HD void moments(const Hyper& h, float g, float b1_m, float b2_v, float& m, float& v) {
   m = multiply_add(h.c1, g, b1_m);
   v = multiply_add(product(h.c2, g), g, b2_v);
+}
+// The same of codes in 64 bits, the scale of a block's largest, and a code (of `fraction` bits behind the exponent) with 16 random bits.
+BAGUA_HD double product64(double a, double b) {
+#ifdef __CUDA_ARCH__
+  return __dmul_rn(a, b);
+#else
+  return a * b;
+#endif
+}
+BAGUA_HD double multiply_add64(double a, double b, double c) {
+#ifdef __CUDA_ARCH__
+  return __fma_rn(a, b, c);
+#else
+  return __builtin_fma(a, b, c);
+#endif
+}
+BAGUA_HD double first64(const Hyper& h, float g, uint32_t code, float scale) {
+  return multiply_add64(1.0 - h.beta1, g, product64(product64(code1_bits(code) * kUp, scale), h.beta1));
+}
+BAGUA_HD double second64(const Hyper& h, float g, uint32_t code, float scale) {
+  return multiply_add64(1.0 - h.beta2, product64(g, g), product64(product64(code2_bits(code) * kUp, scale), h.beta2));
+}
+BAGUA_HD float scale64(float top, float largest, double* per) {
+  float s = top / largest;
+  s = s < kSmallestScale ? kSmallestScale : s;
+  *per = 1.0 / s;
+  return top > 0 ? s : 0.f;
+}
+BAGUA_HD double power_of_two(int e) {
+#ifdef __CUDA_ARCH__
+  return __hiloint2double((1023 + e) << 20, 0);
+#else
+  return std::ldexp(1.0, e);
+#endif
+}
+BAGUA_HD uint32_t code64(double y, int fraction, uint32_t random) {
+  uint64_t bits;
+#ifdef __CUDA_ARCH__
+  bits = (uint64_t)__double_as_longlong(y);
+#else
+  std::memcpy(&bits, &y, 8);
+#endif
+  int e = (int)(bits >> 52) - 1023;
+  e = e < -6 ? -6 : e;
+  const uint32_t q = (uint32_t)multiply_add64(y, power_of_two(fraction - e), (random + 0.5) * 0x1p-16);
+  const uint32_t code = ((uint32_t)(e + 6) << fraction) + q, last = (16u << fraction) - 1;
+  return code < last ? code : last;
+}
+BAGUA_HD uint32_t first_code64(double m, double per, uint32_t random) {
+  return code64(m < 0 ? -m * per : m * per, 3, random & 0xffffu) | (m < 0 ? 0x80u : 0u);
+}
+BAGUA_HD uint32_t second_code64(double v, double per, uint32_t random) {
+  const uint32_t c = code64(v * per, 4, random >> 16);
+  return c == 0 && (float)v > 0 ? 1 : c;
 }
 // The new parameter.
 BAGUA_HD float parameter(const Hyper& h, float p, float m, float v) {

@@ -154,3 +154,8 @@ def test_more_elements_than_32_bits_count():
     m2, v2, s2 = ops.adamw_state8(q)
     ops.adamw_step([q], [h], [m2], [v2], step=1, scales=[s2], **host.HYPER)
     assert torch.equal(p[-1512:], q) and torch.equal(s[:, -6:], s2) and not p[:-1512].any()
+
+
+@pytest.mark.parametrize("dtypes", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16)])
+def test_codes_are_those_of_64_bits(dtypes):
+    host.check_codes("cuda", dtypes, 6_000_001)
