@@ -5,8 +5,8 @@
 //
 // in fp32 whatever p and g are held in; p is rounded once.  No counterpart in the reference, which has no optimizer.
 //
-// Moments in 8 bits.  kMoment8Block neighbouring elements of a tensor share a scale for each moment, fp32, chosen so that the block's
-// largest value has the largest code.  A code is a small floating point number: for m a sign, 4 bits of exponent and 3 of fraction
+// Moments in 8 bits.  kMoment8Block neighbouring elements of a tensor share a scale for each moment, fp32: the block's largest value
+// times fp32's 1/480 or 1/496, so that it has the largest code.  A code is a small floating point number: for m a sign, 4 bits of exponent and 3 of fraction
 // (up to 480, down to 2^-9), for v, which has no sign, 4 and 4 (up to 496, down to 2^-10).
 //
 // Rounding is stochastic: of the two neighbouring values the upper one is taken with the probability that keeps the mean.  To the

@@ -146,7 +146,8 @@ BAGUA_HD void moments(const Hyper& h, float g, float b1_m, float b2_v, float& m,
   m = multiply_add(h.c1, g, b1_m);
   v = multiply_add(product(h.c2, g), g, b2_v);
 }
-// The same of codes in 64 bits, the scale of a block's largest, and a code (of `fraction` bits behind the exponent) with 16 random bits.
+// The same of codes in 64 bits, the scale of a block's largest (rounded to fp32 before the product, as the definition has it), and a
+// code (of `fraction` bits behind the exponent) with 16 random bits.
 BAGUA_HD double product64(double a, double b) {
 #ifdef __CUDA_ARCH__
   return __dmul_rn(a, b);
@@ -168,7 +169,7 @@ BAGUA_HD double second64(const Hyper& h, float g, uint32_t code, float scale) {
   return multiply_add64(1.0 - h.beta2, product64(g, g), product64(product64(code2_bits(code) * kUp, scale), h.beta2));
 }
 BAGUA_HD float scale64(float top, float largest, double* per) {
-  float s = top / largest;
+  float s = top * (1.f / largest);
   s = s < kSmallestScale ? kSmallestScale : s;
   *per = 1.0 / s;
   return top > 0 ? s : 0.f;

@@ -572,7 +572,7 @@ def check_codes(device, dtypes, n):
         ops.adamw_step([p], [g], [m], [v], step=t, scales=[s], seed=9, **HYPER)
         random = plain.random_bits(9, t, 0, n)
         for x, row, largest, table, u, code in ((first, 0, 480, plain.FIRST, random & 0xFFFF, m), (second, 1, 496, plain.SECOND, random >> 16, v)):
-            scale = plain.tops(x).float() / largest  # (of normal size here)
+            scale = plain.tops(x).float() * torch.tensor(1 / largest)  # in fp32 (and of normal size here)
             assert ((s[row].cpu() - scale).abs() <= 6 * U * scale).all()
             want, same = plain.codes(x, plain.spread(scale, n), table, (u.double() + 0.5) / 65536, 0)
             assert torch.equal(want, same)
