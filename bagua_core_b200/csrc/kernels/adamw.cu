@@ -1,5 +1,5 @@
 // See adamw.h.  Streams over memory: with fp32 parameters, gradients and moments 28 bytes an element, 16 with moments in 8 bits.
-// 131 M elements: 534 us with fp32 moments (6.95 TB/s, above the rate of a copy), 358 with 8 bits (5.9 TB/s; integer
+// 131 M elements: 534 us with fp32 moments (6.95 TB/s, above the rate of a copy), 319 with 8 bits (6.6 TB/s; integer
 // instructions are issued in three quarters of all cycles), 120 to read those into bf16 (6.6 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -133,9 +133,9 @@ __global__ void __launch_bounds__(kThreads) step32_kernel(const __grid_constant_
 // So two elements are computed by one instruction where there is one; the square root and the reciprocal are the hardware's (within 2^-22 each: a
 // parameter is off by that part of its update); the moments' betas go into the factor that decodes them, and both directions of coding take
 // one factor.  A block with a scale beyond kPlainScale, or an eps so small that a subnormal square root counts next to
-// it, goes the longer way.  To know which codes fp32 leaves open costs three instructions an element, and 2 % of the blocks, whose
-// codes are settled in 64 bits (with bf16 parameters and gradients 131 M elements take 364 us, without it 312; in fp32 358 and 353).
-// Blocks on an SM: so many leave 40 registers a thread and a few spilled ones.  131 M elements take 362 us, with five (48 registers)
+// it, goes the longer way.  2 % of the blocks hold codes that fp32 leaves open.  Coding takes byte permutations where it can:
+// with shifts and masks 131 M elements took 358 us, now 319 (bf16 parameters and gradients: 364, 304).
+// Blocks on an SM: so many leave 40 registers a thread and a few spilled ones.  131 M elements took 362 us, with five (48 registers)
 // 378, seven (32) 388: the loads of waiting warps are worth more than the spills cost.  A warp that took two blocks in turn held
 // more registers over the turn than it had: 434 us.
 constexpr int kResident8 = 6;
@@ -171,9 +171,13 @@ __device__ __forceinline__ float largest(float a, float b, float c) {
   return y;
 }
 __device__ __forceinline__ Pair both(float x) { return pair(x, x); }
+__device__ __forceinline__ uint32_t top_bytes(const uint32_t (&x)[4]) {
+  return __byte_perm(__byte_perm(x[0], x[1], 0x0073), __byte_perm(x[2], x[3], 0x0073), 0x5410);
+}
+static_assert(kSlack == 16, "whole numbers of the random bits' steps, which the short way counts");
 
-// A block's codes and scales in 64 bits, by the whole warp: one block in forty.  (131 M elements: 358 us with two elements at a time,
-// 362 with one, 364 with four.)
+// A block's codes and scales in 64 bits, by the whole warp: one block in forty.  (131 M elements took 358 us with two elements at a
+// time, 362 with one, 364 with four.)
 template <typename G>
 __device__ __forceinline__ void code_in_64_bits(const Segment& a, const Hyper& h, uint32_t key, int64_t block) {
   const int lane = (int)threadIdx.x & 31;
@@ -296,42 +300,57 @@ __device__ __forceinline__ bool step8_block(const Segment& a, const Hyper& h, ui
   float per_m, per_v;
   const float new_ms = block_scale(__reduce_max_sync(0xffffffffu, float_bits(top_m)), kLargest1, &per_m);
   const float new_vs = block_scale(__reduce_max_sync(0xffffffffu, float_bits(top_v)), kLargest2, &per_v);
-  uint32_t near1 = ~0u, near2 = ~0u;
+  bool near = false;
   const uint32_t random = random_base(key, base) + (uint32_t)at(0, 0) * kStride;
-  auto code = [&](auto plain) {
-    constexpr bool kPlain = decltype(plain)::value;
+  auto bits_of = [&](int r, int e) { return mix(random + (uint32_t)(at(r, e) - at(0, 0)) * kStride); };
+  if (new_ms < kPlainScale && new_vs < kPlainScale) {
+    // sum1(), sum2(), cut1() and cut2() with all bits moved up, so that codes are bytes 3 and the bits that are cut off begin with bytes
+    // 2 and 1: bytes are put together by one instruction.  No sum overflows: y is at most three steps of fp32 above the largest code.
     const Pair fm = both(per_m * kDown), fv = both(per_v * kDown);
+    uint32_t near1 = ~0u, near2 = ~0u;  // of two codes each: above1() and above2() in units of the random bits
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      uint32_t t1[4], t2[4];
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        const float2 y1 = halves(mul(pair(mv[r][e], mv[r][e + 1]), fm)), y2 = halves(mul(pair(vv[r][e], vv[r][e + 1]), fv));
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          const uint32_t bits = bits_of(r, e + o);
+          t1[e + o] = (float_bits(o ? y1.y : y1.x) << 4) + __byte_perm(bits, 0x80u, 0x5104);
+          t2[e + o] = (float_bits(o ? y2.y : y2.x) << 5) + __byte_perm(bits, 0x80u, 0x5324);
+          if (!kVec && at(r, e + o) >= n) t1[e + o] = t2[e + o] = 0x800000u;
+          t1[e + o] |= float_bits(mv[r][e + o]) & 0x80000000u;
+        }
+        near1 = __viaddmin_u16x2(__byte_perm(t1[e], t1[e + 1], 0x6521), kSlack / 16 * 0x10001u, near1);
+        near2 = __viaddmin_u16x2(__byte_perm(t2[e], t2[e + 1], 0x6521), kSlack / 8 * 0x10001u, near2);
+      }
+      mc[r] = top_bytes(t1);
+      vc[r] = top_bytes(t2);
+      if ((vc[r] - 0x01010101u) & ~vc[r] & 0x80808080u)  // seldom: a code 0, which stands for nothing but 0
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (vv[r][e] > 0 && !(vc[r] >> (8 * e) & 0xffu)) vc[r] |= 1u << (8 * e);
+    }
+    near = (near1 & 0xffffu) < kSlack / 8 || near1 >> 16 < kSlack / 8 || (near2 & 0xffffu) < kSlack / 4 || near2 >> 16 < kSlack / 4;
+  } else {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       uint32_t c1[4], c2[4];
 #pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        float2 y1 = halves(mul(pair(fabsf(mv[r][e]), fabsf(mv[r][e + 1])), fm)), y2 = halves(mul(pair(vv[r][e], vv[r][e + 1]), fv));
-        if constexpr (!kPlain) {  // each by its own scale
-          y1 = make_float2(scaled(fabsf(mv[r][e]), per_m, new_ms < kPlainScale), scaled(fabsf(mv[r][e + 1]), per_m, new_ms < kPlainScale));
-          y2 = make_float2(scaled(vv[r][e], per_v, new_vs < kPlainScale), scaled(vv[r][e + 1], per_v, new_vs < kPlainScale));
-        }
-#pragma unroll
-        for (int o = 0; o < 2; ++o) {
-          const uint32_t bits = mix(random + (uint32_t)(at(r, e + o) - at(0, 0)) * kStride);
-          const uint32_t s1 = sum1(o ? y1.y : y1.x, bits), s2 = sum2(o ? y2.y : y2.x, bits);
-          c1[e + o] = cut1(s1, mv[r][e + o]);
-          c2[e + o] = cut2(s2, vv[r][e + o]);
-          if (kVec || at(r, e + o) < n) {
-            near1 = min(near1, above1(s1));
-            near2 = min(near2, above2(s2));
-          }
-        }
+      for (int e = 0; e < 4; ++e) {  // each by its own scale
+        const uint32_t bits = bits_of(r, e);
+        const uint32_t s1 = sum1(scaled(fabsf(mv[r][e]), per_m, new_ms < kPlainScale), bits);
+        const uint32_t s2 = sum2(scaled(vv[r][e], per_v, new_vs < kPlainScale), bits);
+        c1[e] = cut1(s1, mv[r][e]) << 24;
+        c2[e] = cut2(s2, vv[r][e]) << 24;
+        near |= (kVec || at(r, e) < n) && (above1(s1) < kNear1 || above2(s2) < kNear2);
       }
-      mc[r] = c1[0] | c1[1] << 8 | c1[2] << 16 | c1[3] << 24;
-      vc[r] = c2[0] | c2[1] << 8 | c2[2] << 16 | c2[3] << 24;
+      mc[r] = top_bytes(c1);
+      vc[r] = top_bytes(c2);
     }
-  };
-  if (new_ms < kPlainScale && new_vs < kPlainScale)
-    code(std::true_type{});
-  else
-    code(std::false_type{});
-  if (__any_sync(0xffffffffu, near1 < kNear1 || near2 < kNear2) && new_ms < INFINITY && new_vs < INFINITY) {
+  }
+  if (__any_sync(0xffffffffu, near) && new_ms < INFINITY && new_vs < INFINITY) {
     return false;
   }
   if (lane == 0) {
