@@ -135,9 +135,9 @@ __global__ void __launch_bounds__(kThreads) step32_kernel(const __grid_constant_
 // one factor.  A block with a scale beyond kPlainScale, or an eps so small that a subnormal square root counts next to
 // it, goes the longer way.  2 % of the blocks hold codes that fp32 leaves open.  Coding takes byte permutations where it can:
 // with shifts and masks 131 M elements took 358 us, now 319 (bf16 parameters and gradients: 364, 304).
-// Blocks on an SM: so many leave 40 registers a thread and a few spilled ones.  131 M elements took 362 us, with five (48 registers)
-// 378, seven (32) 388: the loads of waiting warps are worth more than the spills cost.  A warp that took two blocks in turn held
-// more registers over the turn than it had: 434 us.
+// Blocks on an SM: so many leave 40 registers a thread and a few spilled ones.  131 M elements take 317 us, with five (48 registers)
+// 337, seven (32) 355: the loads of waiting warps are worth more than the spills cost.  A warp that took two blocks in turn held
+// more registers over the turn than it had (434 us where one took 362).
 constexpr int kResident8 = 6;
 constexpr int kTile8 = kThreads / 32 * kMoment8Block;
 constexpr float kPlainEps = 1e-10f;
@@ -176,8 +176,8 @@ __device__ __forceinline__ uint32_t top_bytes(const uint32_t (&x)[4]) {
 }
 static_assert(kSlack == 16, "whole numbers of the random bits' steps, which the short way counts");
 
-// A block's codes and scales in 64 bits, by the whole warp: one block in forty.  (131 M elements took 358 us with two elements at a
-// time, 362 with one, 364 with four.)
+// A block's codes and scales in 64 bits, by the whole warp: one block in forty.  (131 M elements take 317 us with two elements at a
+// time, 320 with one; before the codes took byte permutations 358, 362, and 364 with four.)
 template <typename G>
 __device__ __forceinline__ void code_in_64_bits(const Segment& a, const Hyper& h, uint32_t key, int64_t block) {
   const int lane = (int)threadIdx.x & 31;
