@@ -560,7 +560,7 @@ def test_negated_views_are_refused(which):
 
 def check_codes(device, dtypes, n):
     """Two steps give, to the bit, the codes and scales that the definition in 64 bits gives.  fp32 alone would round one code in some
-    400,000 the other way.  Left out are first moments that are the difference of larger terms: what fp32 leaves of those is not bounded."""
+    800,000 the other way (100 of 80 million, counted).  Left out are first moments that are the difference of larger terms: what fp32 leaves of those is not bounded."""
     (p,), (g,), _, _ = tensors([n], dtypes, "cpu", seed=1)
     b1, b2 = HYPER["betas"]
     p, g = p.to(device), g.to(device)
