@@ -474,6 +474,8 @@ struct ReadTable {
   int n;
 };
 static_assert(sizeof(ReadTable<kMany>) <= 32764, "launch parameters");
+// (Vectors up to the last whole one: 79 tensors of 9.9 M elements that end anywhere take 11.5 us; tiles that end early element by
+// element 22.6.)
 constexpr int kReadVecs = 2, kReadTile = kThreads * 8 * kReadVecs;
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__ ReadTable<N> table) {
@@ -482,12 +484,17 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__
   const cuda::Read8& a = table.seg[k];
   T *m = (T*)a.m_out, *v = (T*)a.v_out;
   const int64_t base = (int64_t)(blockIdx.x - table.first_tile[k]) * kReadTile;
-  if (base + kReadTile <= a.n && ((uintptr_t)a.m | (uintptr_t)a.v) % 8 == 0 && ((uintptr_t)m | (uintptr_t)v) % 16 == 0) {
+  auto one = [&](int64_t i) {
+    m[i] = from_float<T>(decode1(a.m[i], a.m_scale[i / kMoment8Block]));
+    v[i] = from_float<T>(decode2(a.v[i], a.v_scale[i / kMoment8Block]));
+  };
+  if ((((uintptr_t)a.m | (uintptr_t)a.v) % 8 | ((uintptr_t)m | (uintptr_t)v) % 16) == 0) {
     uint2 mc[kReadVecs], vc[kReadVecs];
     float ms[kReadVecs], vs[kReadVecs];
 #pragma unroll
     for (int r = 0; r < kReadVecs; ++r) {
       const int64_t i = base + (r * kThreads + threadIdx.x) * 8;
+      if (i + 8 > a.n) continue;
       mc[r] = *reinterpret_cast<const uint2*>(a.m + i);
       vc[r] = *reinterpret_cast<const uint2*>(a.v + i);
       ms[r] = a.m_scale[i / kMoment8Block];
@@ -496,6 +503,10 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__
 #pragma unroll
     for (int r = 0; r < kReadVecs; ++r) {
       const int64_t i = base + (r * kThreads + threadIdx.x) * 8;
+      if (i + 8 > a.n) {  // the last elements, those of one vector that is not whole
+        for (int64_t k = i; k < a.n; ++k) one(k);
+        continue;
+      }
       float mv[8], vv[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -507,10 +518,7 @@ __global__ void __launch_bounds__(kThreads) read8_kernel(const __grid_constant__
     }
   } else {
     const int64_t end = min(base + kReadTile, a.n);
-    for (int64_t i = base + threadIdx.x; i < end; i += kThreads) {
-      m[i] = from_float<T>(decode1(a.m[i], a.m_scale[i / kMoment8Block]));
-      v[i] = from_float<T>(decode2(a.v[i], a.v_scale[i / kMoment8Block]));
-    }
+    for (int64_t i = base + threadIdx.x; i < end; i += kThreads) one(i);
   }
 }
 
