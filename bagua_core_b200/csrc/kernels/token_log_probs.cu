@@ -664,7 +664,8 @@ struct BackwardArgs {
   int64_t a_stride, b_stride;
   int vocab;
 };
-// d x_j = -p_j (a + b (log p_j + entropy)) = 2^d (A + B d), with the sum and what d leaves of log p_j in A and B.
+// d x_j = -p_j (a + b (log p_j + entropy)) = 2^d A + 2^d d B, with the sum and what d leaves of log p_j in A and B.  2^d d comes first: d is
+// -1.4e38 at masked tokens, where its product with B would be infinite, and NaN once it met the 2^d that is 0.
 template <typename T>
 struct Coefficients {
   float m, A, B;
@@ -676,15 +677,15 @@ struct Coefficients {
       Elements<T>::pairs(held<T>(v), g);
 #pragma unroll
       for (int k = 0; k < Elements<T>::kPairs; ++k) {
-        const Pair d = fma(g[k], log2e, less);
-        g[k] = mul(exp2_fast(d), fma(b, d, a));
+        const Pair d = fma(g[k], log2e, less), e = exp2_fast(d);
+        g[k] = fma(mul(e, d), b, mul(e, a));
       }
     } else {
       Elements<T>::pairs(v, g);
 #pragma unroll
       for (int k = 0; k < Elements<T>::kPairs; ++k) {
-        const Pair d = exponent_wide(g[k], m);
-        g[k] = mul(exp2_fast(d), fma(b, d, a));
+        const Pair d = exponent_wide(g[k], m), e = exp2_fast(d);
+        g[k] = fma(mul(e, d), b, mul(e, a));
       }
     }
   }

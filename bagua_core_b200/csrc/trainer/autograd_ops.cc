@@ -792,8 +792,8 @@ std::vector<at::Tensor> log_prob_composition(const at::Tensor& logits, const at:
   lp = at::where(none, -inf, lp);
   lp = at::where(known, lp, std::numeric_limits<double>::quiet_NaN());
   lp = at::where(scored, lp, 0.0);
-  // (the largest NaN-preserving lower bound: 0 * -inf has no place in the sum)
-  const at::Tensor entropy = at::where(scored.logical_and(none.logical_not()), (p * ls.clamp_min(-1e30)).sum(-1).neg(), 0.0);
+  // (0 * -inf has no place in the sum, nor has the product of a large gradient with the bound in the gradient: p is 0 from -104 on)
+  const at::Tensor entropy = at::where(scored.logical_and(none.logical_not()), (p * ls.clamp_min(-128.0)).sum(-1).neg(), 0.0);
   return {lp, entropy};
 }
 // {values, ids} of the likeliest tokens, detached.

@@ -246,6 +246,37 @@ def test_second_order():
     check_second_order("cpu")
 
 
+def check_scaled_entropy_gradients(device):
+    """Entropy's gradient under factors as loss scales bring them, where masks leave one token, few, or half of them."""
+    for dtype in TYPES.values():
+        half = torch.finfo(dtype).eps / 2
+        for vocab in (40, 3000):
+            for low in (-INF, torch.finfo(dtype).min):
+                x, t = logits(6, vocab, dtype, seed=vocab)
+                x[0, 1:] = low
+                x[1, :vocab - 1] = low
+                x[2, 3:] = low
+                x[3, vocab // 2:] = low
+                x[4, ::2] = low
+                t = torch.zeros_like(t)
+                for size in (1e-3, 5.0, 1e4 if dtype == torch.float16 else 1e5) + (() if dtype == torch.float16 else (1e20,)):
+                    b = size * torch.tensor([1.0, -1.0, 1.0, -1.0, 1.0, -1.0])
+                    _, entropy, _, _, want = plain(x, t, 0, -100, torch.zeros(6), b)
+                    y = x.to(device).requires_grad_()
+                    (d,) = torch.autograd.grad(ops.token_log_probs(y, t.to(device)).entropy, y, b.to(device))
+                    assert d.isfinite().all() and not d.cpu()[x == low].any()
+                    # as in check(): a probability is off by `off` relative to itself, its logarithm and the entropy by that relative to 1
+                    # and their size; what is below 2^-126 is lost
+                    off = 2.0 ** -22 + (vocab / 256 + 64 + 2 ** 8) * U
+                    lp = torch.log_softmax(x.double().clamp(min=-1e30), 1).clamp(min=-100)
+                    parts = lp.exp() * b.abs()[:, None] * (lp.abs() + entropy[:, None] + 4)
+                    close(d, want, 4 * off * parts + half * want.abs() + torch.finfo(dtype).smallest_normal * half + size * 2.0 ** -110)
+
+
+def test_scaled_entropy_gradients():
+    check_scaled_entropy_gradients("cpu")
+
+
 def check_refusals(device):
     x, t = torch.zeros(3, 5, device=device), torch.zeros(3, dtype=torch.int64, device=device)
     for args in ((x.double(), t), (x.long(), t), (x, t.int()), (x, t[:2]), (x, t.view(3, 1)), (x, t, 6), (x, t, -1), (x[:, :0], t),

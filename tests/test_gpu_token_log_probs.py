@@ -87,6 +87,10 @@ def test_gradients_and_refusals():
     host.check_refusals("cuda")
 
 
+def test_scaled_entropy_gradients():
+    host.check_scaled_entropy_gradients("cuda")
+
+
 def test_targets_outside_the_vocabulary():
     x = torch.randn(4, 3000, device="cuda", requires_grad=True)
     t = torch.tensor([5, -1, 3000, 7], device="cuda")
