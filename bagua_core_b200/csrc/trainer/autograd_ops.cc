@@ -801,9 +801,11 @@ std::vector<at::Tensor> top_composition(const at::Tensor& logits, const at::Tens
   const double inf = std::numeric_limits<double>::infinity();
   const at::Tensor all = logits.detach().to(at::kFloat).contiguous();
   const auto sorted = at::sort(all, /*stable=*/true, -1, /*descending=*/true);
-  const at::Tensor lse = at::logsumexp(all, {-1}, true), lost = lse.isnan().logical_or(lse.eq(inf)).squeeze(-1).unsqueeze(-1);
   const at::Tensor best = std::get<0>(sorted).narrow(-1, 0, top);
-  at::Tensor v = at::where(best.eq(-inf), best, best - lse), ids = std::get<1>(sorted).narrow(-1, 0, top);
+  // (differences from the largest first: the sum's logarithm would be lost beside a large one)
+  const at::Tensor first = best.narrow(-1, 0, 1), m = first.masked_fill(first.isinf(), 0.0);
+  const at::Tensor lse = at::logsumexp(all - m, {-1}, true), lost = lse.isnan().logical_or(lse.eq(inf));
+  at::Tensor v = at::where(best.eq(-inf), best, best - m - lse), ids = std::get<1>(sorted).narrow(-1, 0, top);
   v = at::where(lost, std::numeric_limits<double>::quiet_NaN(), v);
   ids = ids.masked_fill(lost, -1);
   const at::Tensor skipped = targets.eq(ignored).unsqueeze(-1);

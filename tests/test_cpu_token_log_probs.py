@@ -277,6 +277,25 @@ def test_scaled_entropy_gradients():
     check_scaled_entropy_gradients("cpu")
 
 
+def check_large_alternatives(device):
+    """Alternatives' values do not lose the row's sum beside large logits."""
+    for dtype, sizes in ((torch.float32, (1e3, 3e4, 1e10, 1e30, 3e38)), (torch.bfloat16, (1e3, 1e10, 3e38)), (torch.float16, (1e3, 3e4, 65504.0))):
+        for size in sizes:
+            for sign in (1, -1):
+                x = torch.full((3, 50), sign * size).to(dtype)
+                x[1, 7] = 0.5 * size
+                x[2, 25:] = -INF
+                r = ops.token_log_probs(x.to(device), torch.zeros(3, dtype=torch.int64, device=device), 2)
+                want = torch.tensor([[math.log(1 / 50)] * 2, [math.log(1 / 49)] * 2, [math.log(1 / 25)] * 2], dtype=torch.float64)
+                if sign < 0:
+                    want[1] = torch.tensor([0.0, float(x[1, 0].double() - x[1, 7].double())])
+                close(r.top_log_probs, want, 2.0 ** -22 + 2 ** 5 * U * 4 + 2 * U * want.abs())
+
+
+def test_large_alternatives():
+    check_large_alternatives("cpu")
+
+
 def check_refusals(device):
     x, t = torch.zeros(3, 5, device=device), torch.zeros(3, dtype=torch.int64, device=device)
     for args in ((x.double(), t), (x.long(), t), (x, t.int()), (x, t[:2]), (x, t.view(3, 1)), (x, t, 6), (x, t, -1), (x[:, :0], t),
