@@ -55,7 +55,7 @@ struct Elements;
 template <>
 struct Elements<float> {
   static constexpr int kPairs = 2;
-  static constexpr float kHeld = -1e38f, kLow = -1e37f;
+  static constexpr float kHeld = -1e38f, kNear = 0x1p20f;
   static constexpr uint32_t kMasked = 0xff800000u;  // words of -inf
   __device__ static float largest(const uint4& v) {
     return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
@@ -85,7 +85,7 @@ struct Elements16 {
 };
 template <>
 struct Elements<__half> : Elements16<__half, __half2> {
-  static constexpr float kHeld = -65504.f, kLow = -6e4f;
+  static constexpr float kHeld = -65504.f, kNear = 6e4f;
   static constexpr uint32_t kMasked = 0xfc00fc00u;
   __device__ static uint32_t held(uint32_t w) { return Elements16::held(w, 0xfbfffbffu); }
   __device__ static void pairs(const uint4& v, Pair (&p)[kPairs]) {
@@ -109,7 +109,7 @@ struct Elements<__half> : Elements16<__half, __half2> {
 };
 template <>
 struct Elements<__nv_bfloat16> : Elements16<__nv_bfloat16, __nv_bfloat162> {
-  static constexpr float kHeld = -1e38f, kLow = -1e37f;
+  static constexpr float kHeld = -1e38f, kNear = 0x1p20f;
   static constexpr uint32_t kMasked = 0xff80ff80u;
   __device__ static uint32_t held(uint32_t w) { return Elements16::held(w, 0xfe96fe96u); }  // -9.97e37
   __device__ static void pairs(const uint4& v, Pair (&p)[kPairs]) {
@@ -135,12 +135,12 @@ __device__ __forceinline__ uint4 held(const uint4& v) {
 
 // ---- exponents ----------------------------------------------------------------------------------
 // exp(x - m) is taken as 2^d, d = x log2(e) - m log2(e), one multiply-add with the same rounded m log2(e) for all of a row, so that its
-// rounding leaves the probabilities.  x is held above -inf before, so that d is finite and 2^d d is 0 where 2^d is.  For an m at the
-// ends of the type's range, where the product would be infinite or m as low as what x is held at, and for m = -inf, the difference is
-// taken first ("wide").
+// rounding, the same in every d, leaves the probabilities.  It is 2^-4 at most for |m| below kNear; at 1e10 it would be 440, and no 2^d in
+// range.  x is held above -inf before, so that d is finite and 2^d d is 0 where 2^d is.  For any other m (in fp16: next to the ends of its
+// range; NaN and infinities too) the difference x - m is taken first ("wide"): two instructions more an element.
 constexpr float kFar = -1000.f;
 template <typename T>
-__device__ __forceinline__ bool within(float m) { return m > Elements<T>::kLow && m < 1e38f; }
+__device__ __forceinline__ bool within(float m) { return fabsf(m) < Elements<T>::kNear; }
 __device__ __forceinline__ float exponent_wide(float x, float m) { return max_nan((x - (m == -INFINITY ? 0.f : m)) * kLog2e, kFar); }
 __device__ __forceinline__ Pair exponent_wide(Pair x, float m) {
   const float2 f = halves(x);
@@ -151,10 +151,13 @@ __device__ __forceinline__ Pair exponent_wide(Pair x, float m) {
 struct Sums {
   float m, s, t;
 };
-// The factor of sums of values with largest value `m`, for a larger one `to`, and by how much every d grows.
+// The factor of sums of values with largest value `m`, for a larger one `to`, and by how much every d grows: what the two take off x log2(e),
+// rounded or not, as the form of each has it.
 template <typename T>
 __device__ __forceinline__ float shift_sums(float m, float to, float* d) {
-  *d = max_nan(within<T>(m) && within<T>(to) ? __fmul_rn(m, kLog2e) - __fmul_rn(to, kLog2e) : (m - to) * kLog2e, kFar);
+  const float l = __fmul_rn(m, kLog2e), l_to = __fmul_rn(to, kLog2e);
+  const bool near = within<T>(m), near_to = within<T>(to);
+  *d = max_nan(near ? (near_to ? l - l_to : __fmaf_rn(-to, kLog2e, l)) : near_to ? __fmaf_rn(m, kLog2e, -l_to) : (m - to) * kLog2e, kFar);
   return exp2_fast(*d);
 }
 // The sums of a warp's lanes: all are moved to the largest m, then added.  (Nothing but -inf in a lane: its sums are 0, or NaN.)

@@ -296,6 +296,56 @@ def test_large_alternatives():
     check_large_alternatives("cpu")
 
 
+def large_rows(vocab, dtype, size, g):
+    """Rows whose logits are near `size` in different ways, and tokens to ask for."""
+    x = torch.randn(6, vocab, generator=g)
+    x[0] = size                                          # all equal
+    x[1] = size                                          # one that is not
+    x[1, vocab // 2] = 0.5 * size
+    x[2, vocab // 3] = size                              # one among ordinary ones
+    x[3, :vocab // 2] = size                             # a half
+    x[4, torch.rand(vocab, generator=g) < 0.5] = size    # every other one
+    # neighbours of `size`, some steps of fp32 or of the type apart
+    step = max(abs(size) * 2.0 ** -23, 2.0 ** -3 if abs(size) >= 2 ** 20 else 0, abs(size) * torch.finfo(dtype).eps)
+    x[5] = size + step * torch.randint(-40, 41, (vocab,), generator=g).double()
+    return x.clamp(torch.finfo(dtype).min, torch.finfo(dtype).max).to(dtype), torch.tensor([3, vocab // 2, vocab // 3, vocab - 1, 0, 1])
+
+
+def check_large_logits(device, vocabs, rows):
+    """Against 64 bits, with a tolerance that does not grow with the logits: a log probability is a difference of logits, each exact."""
+    g = torch.Generator().manual_seed(7)
+    for dtype in TYPES.values():
+        half = torch.finfo(dtype).eps / 2
+        sizes = [100.0, 3e4, 59968.0, 6e4, 65000.0] if dtype == torch.float16 else [
+            1e5, 2.0 ** 20 - 1, 2.0 ** 20, 2.0 ** 20 + 1, 3e6, 1e9, 6e9, 1e10, 1e12, 1e20, 1e30, 9e36, 3e37, 9.9e37, 1.1e38, 3e38]
+        for vocab in vocabs:
+            off = 2.0 ** -22 + (vocab / 256 + 64 + 2 ** 8) * U
+            for size in sizes:
+                for sign in (1, -1):
+                    x, t = large_rows(vocab, dtype, sign * size, g)
+                    for lo in range(0, len(x), rows):
+                        u, v = x[lo:lo + rows], t[lo:lo + rows]
+                        a, b = torch.randn(len(u), generator=g), torch.randn(len(u), generator=g)
+                        lp, entropy, values, ids, want = plain(u, v, 7, -100, a, b)
+                        y = u.to(device).requires_grad_()
+                        r = ops.token_log_probs(y, v.to(device), 7)
+                        (d,) = torch.autograd.grad((r.log_probs, r.entropy), y, (a.to(device), b.to(device)))
+                        # log sum: a relative error `off` of the sum, and half a step of its logarithm, below 2^5; difference and product
+                        # three half steps of the result
+                        close(r.log_probs, lp, off + 2 ** 5 * U + 4 * U * lp.abs())
+                        close(r.top_log_probs, values, off + 2 ** 5 * U + 4 * U * values.abs())
+                        assert torch.equal(r.top_ids.cpu(), ids)
+                        close(r.entropy, entropy, 2 * off * (1 + entropy.abs() + 4))
+                        w = u.double() - u.double().amax(1)[:, None]
+                        la = torch.log_softmax(w, 1).clamp(min=-100)
+                        parts = la.exp() * (a.abs()[:, None] + b.abs()[:, None] * (la.abs() + entropy.abs()[:, None] + 4))
+                        close(d, want, 4 * off * parts + (half + 2 * U) * (want.abs() + a.abs()[:, None]) + torch.finfo(dtype).smallest_normal + 2.0 ** -100)
+
+
+def test_large_logits():
+    check_large_logits("cpu", (40, 3000), 6)
+
+
 def check_refusals(device):
     x, t = torch.zeros(3, 5, device=device), torch.zeros(3, dtype=torch.int64, device=device)
     for args in ((x.double(), t), (x.long(), t), (x, t.int()), (x, t[:2]), (x, t.view(3, 1)), (x, t, 6), (x, t, -1), (x[:, :0], t),

@@ -91,6 +91,15 @@ def test_scaled_entropy_gradients():
     host.check_scaled_entropy_gradients("cuda")
 
 
+@pytest.mark.parametrize("vocab,rows", [(40, 6), (1000, 6), (3000, 6), (9001, 1), (30522, 6)])
+def test_large_logits(vocab, rows):
+    host.check_large_logits("cuda", (vocab,), rows)
+
+
+def test_large_alternatives():
+    host.check_large_alternatives("cuda")
+
+
 def test_targets_outside_the_vocabulary():
     x = torch.randn(4, 3000, device="cuda", requires_grad=True)
     t = torch.tensor([5, -1, 3000, 7], device="cuda")
