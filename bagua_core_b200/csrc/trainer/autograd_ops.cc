@@ -793,7 +793,9 @@ std::vector<at::Tensor> log_prob_composition(const at::Tensor& logits, const at:
   lp = at::where(known, lp, std::numeric_limits<double>::quiet_NaN());
   lp = at::where(scored, lp, 0.0);
   // (0 * -inf has no place in the sum, nor has the product of a large gradient with the bound in the gradient: p is 0 from -104 on)
-  const at::Tensor entropy = at::where(scored.logical_and(none.logical_not()), (p * ls.clamp_min(-128.0)).sum(-1).neg(), 0.0);
+  at::Tensor entropy = at::where(scored.logical_and(none.logical_not()), (p * ls.clamp_min(-128.0)).sum(-1).neg(), 0.0);
+  // a row whose target is unknown has an entropy, but no gradient
+  entropy = at::where(known.logical_or(scored.logical_not()), entropy, entropy.detach());
   return {lp, entropy};
 }
 // {values, ids} of the likeliest tokens, detached.
@@ -839,8 +841,8 @@ struct LogProbNode : public Node {
         at::Tensor y;
         for (int k = 0; k < 2; ++k)
           if (grads[k].defined()) {
-            // (a row whose log probability is not finite has no gradient: its factor would make one)
-            const at::Tensor part = at::where(r[k].detach().eq(-std::numeric_limits<double>::infinity()), 0.0, r[k]).mul(grads[k]).sum();
+            // (only its gradient counts, which a log probability of -inf has as any other)
+            const at::Tensor part = r[k].mul(grads[k]).sum();
             y = y.defined() ? y + part : part;
           }
         return y;

@@ -296,6 +296,57 @@ def test_large_alternatives():
     check_large_alternatives("cpu")
 
 
+def check_kept_graphs(device, unknown=False):
+    """The gradient does not depend on whether it will be differentiated, and its own is that of the formula: for targets that a mask
+    forbids, rows that it leaves nothing of, and unknown targets."""
+    x, t = logits(5, 9, torch.float32)
+    x[0, 2:5], t[0] = -INF, 3
+    x[1], t[1] = -INF, 0
+    x[2, :8], t[2] = -INF, 8
+    t[3] = -100
+    ok = t.to(device)
+    if unknown:
+        t = t.clone()
+        t[4] = 9
+    dropped = torch.tensor([False, True, False, True, unknown])
+    g = torch.Generator().manual_seed(3)
+    a, b, v = torch.randn(5, generator=g), torch.randn(5, generator=g), torch.randn(5, 9, generator=g)
+
+    def formula(y, a, b):
+        ls = torch.log_softmax(torch.where(dropped[:, None], 0.0, y), 1)
+        p = ls.exp()
+        h = -(p * ls.clamp(min=-200)).sum(1, keepdim=True)
+        hit = torch.zeros_like(p).scatter_(1, t.clamp(0, 8)[:, None], 1.0)
+        d = a[:, None] * (hit - p) - b[:, None] * p * (ls.clamp(min=-200) + h)
+        return torch.where(dropped[:, None], 0.0, d)
+
+    ins = [z.double().requires_grad_() for z in (x, a, b)]
+    want = formula(*ins)
+    seconds = torch.autograd.grad((want * v).sum(), ins)
+    for both in (0, 1, 2):  # gradients of both, of the log probabilities, of the entropies
+        got = []
+        for keep in (False, True):
+            y, c, e = (z.to(device).requires_grad_() for z in (x, a, b))
+            r = ops.token_log_probs(y, t.to(device))
+            if unknown:
+                torch.cuda.synchronize()
+                with pytest.raises(RuntimeError, match="not in the vocabulary"):
+                    ops.token_log_probs(y, ok)
+            outs, ups = ((r.log_probs, r.entropy), (c, e)) if both == 0 else ((r[both - 1],), ((c, e)[both - 1],))
+            (d,) = torch.autograd.grad(outs, y, ups, create_graph=keep)
+            got.append(d.detach().cpu().double())
+        # values of some units, sums of 9 terms, a hundred roundings at most
+        assert (got[0] - got[1]).abs().max() <= 400 * U
+        if both == 0:
+            assert (got[1] - want.detach()).abs().max() <= 400 * U
+            for z, w in zip(torch.autograd.grad((d * v.to(device)).sum(), (y, c, e)), seconds):
+                assert (z.cpu().double() - w).abs().max() <= 1000 * U
+
+
+def test_kept_graphs():
+    check_kept_graphs("cpu")
+
+
 def large_rows(vocab, dtype, size, g):
     """Rows whose logits are near `size` in different ways, and tokens to ask for."""
     x = torch.randn(6, vocab, generator=g)

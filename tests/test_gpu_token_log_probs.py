@@ -100,6 +100,11 @@ def test_large_alternatives():
     host.check_large_alternatives("cuda")
 
 
+@pytest.mark.parametrize("unknown", [False, True])
+def test_kept_graphs(unknown):
+    host.check_kept_graphs("cuda", unknown)
+
+
 def test_targets_outside_the_vocabulary():
     x = torch.randn(4, 3000, device="cuda", requires_grad=True)
     t = torch.tensor([5, -1, 3000, 7], device="cuda")
