@@ -78,6 +78,12 @@ void check_apart(std::vector<Pieces>& kinds) {
   }
 }
 
+// Lets autograd notice that a graph's values have changed since.
+void note_written(const TensorRefs& list) {
+  for (const at::Tensor* t : list)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 }  // namespace
 
 void AdamWPlan::add(const at::Tensor& p, const at::Tensor& g, const at::Tensor& m, const at::Tensor& v,
@@ -207,10 +213,9 @@ int adamw_step(const TensorRefs& p, const TensorRefs& g, const TensorRefs& m, co
     plan.add(*p[k], *g[k], *m[k], *v[k], scales ? (*scales)[k] : nullptr, copies ? (*copies)[k] : nullptr, 0);
   plan.check_apart();
   const int launches = plan.step({values}, numbers, seed);
-  // autograd notices that a graph's values have changed since
-  for (const TensorRefs* list : {&p, &m, &v})
-    for (const at::Tensor* t : *list)
-      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  for (const TensorRefs* list : {&p, &m, &v}) note_written(*list);
+  if (scales) note_written(*scales);
+  if (copies) note_written(*copies);
   return launches;
 }
 
@@ -250,12 +255,16 @@ int adamw_read8(const TensorRefs& m, const TensorRefs& v, const TensorRefs& scal
     kinds[5].add(segs.back().v_out, bytes);
   }
   check_apart(kinds);
-  if (!m[0]->is_cuda()) {
+  int launches = 1;
+  if (m[0]->is_cuda()) {
+    const c10::cuda::CUDAGuard on(device);
+    launches = adamw::cuda::read8(segs.data(), (int)n, dtype_of(type), stream_on((int)device.index()));
+  } else {
     adamw::host::read8(segs.data(), (int)n, dtype_of(type));
-    return 1;
   }
-  const c10::cuda::CUDAGuard on(device);
-  return adamw::cuda::read8(segs.data(), (int)n, dtype_of(type), stream_on((int)device.index()));
+  note_written(m_out);
+  note_written(v_out);
+  return launches;
 }
 
 }  // namespace trainer

@@ -260,6 +260,28 @@ def test_graphs_notice_a_step():
     check_versions("cpu")
 
 
+def check_versions_of_all_written(device):
+    """Copies, which forward passes read and graphs keep, scales, and moments that are read back."""
+    p = torch.randn(300, device=device).view(20, 15)
+    m, v, scales = ops.adamw_state8(p)
+    h = p.bfloat16()
+    x = torch.randn(4, 15, device=device).bfloat16().requires_grad_()
+    y = torch.nn.functional.linear(x, h)
+    z = [torch.ones(2, 2, device=device, requires_grad=True) * s for s in (scales, scales[:, :1])]  # also through a view
+    ops.adamw_step([p], [torch.ones_like(p)], [m], [v], scales=[scales], copies=[h], step=1, lr=0.1)
+    outs = [torch.zeros_like(p) for _ in range(2)]
+    w = [x.float().sum() * o for o in outs]
+    ops.adamw_read8([m], [v], [scales], *([o] for o in outs))
+    for used in (y, *z, *w):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            used.sum().backward()
+    torch.nn.functional.linear(x, h).sum().backward()  # the next forward pass
+
+
+def test_graphs_notice_all_that_is_written():
+    check_versions_of_all_written("cpu")
+
+
 def check_step_on_device(device):
     """A step's number in a tensor gives what the same number of the host gives, to the bit."""
     for bits in (32, 8):
