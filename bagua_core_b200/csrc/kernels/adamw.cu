@@ -245,7 +245,7 @@ __device__ __forceinline__ bool step8_block(const Segment& a, const Hyper& h, ui
   auto step = [&](auto plain) {
     constexpr bool kPlain = decltype(plain)::value;
     const Pair km = both(__fmul_rn(h.b1, ms) * (kPlain ? kUp : 1.f)), kv = both(__fmul_rn(h.b2, vs) * (kPlain ? kUp : 1.f));
-    const Pair c1 = both(h.c1), c2 = both(h.c2), root = both(h.root), eps = both(h.eps), rate = both(-h.rate), keep = both(h.keep);
+    const Pair c1 = both(h.c1), c2 = both(h.c2), root = both(h.root), eps = both(h.eps), rate = both(-h.rate), keep = both(h.keep), rest = both(h.rest);
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -261,7 +261,8 @@ __device__ __forceinline__ bool step8_block(const Segment& a, const Hyper& h, ui
         const float2 vf = halves(v2), mf = halves(mm);
         const float2 d = halves(fma(pair(root_of<kPlain>(vf.x), root_of<kPlain>(vf.y)), root, eps));
         const Pair per = pair(reciprocal_of<kPlain>(d.x), reciprocal_of<kPlain>(d.y));
-        const float2 pf = halves(fma(pair(pv[r][e], pv[r][e + 1]), keep, mul(mul(rate, mm), per)));
+        const Pair pp = pair(pv[r][e], pv[r][e + 1]);
+        const float2 pf = halves(fma(pp, keep, fma(pp, rest, mul(mul(rate, mm), per))));
         pv[r][e] = pf.x;
         pv[r][e + 1] = pf.y;
         mv[r][e] = mf.x;

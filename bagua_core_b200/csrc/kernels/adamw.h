@@ -3,7 +3,9 @@
 //   m = b1 m + (1 - b1) g        v = b2 v + (1 - b2) g^2
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
 //
-// in fp32 whatever p and g are held in; p is rounded once.  No counterpart in the reference, which has no optimizer.
+// in fp32 whatever p and g are held in; p is rounded once.  1 - lr wd is held in two numbers: in one it would be off by half a step of fp32
+// next to 1, a tenth of the decay for lr wd of 2e-7, in the same direction at every step.  No counterpart in the reference, which has no
+// optimizer.
 //
 // Moments in 8 bits.  kMoment8Block neighbouring elements of a tensor share a scale for each moment, fp32: the block's largest value
 // times fp32's 1/480 or 1/496, so that it has the largest code.  A code is a small floating point number: for m a sign, 4 bits of exponent and 3 of fraction
@@ -34,7 +36,7 @@ inline int64_t moment8_blocks(int64_t n) { return (n + kMoment8Block - 1) / kMom
 
 // What all elements of a parameter group have in common at a step.
 struct Hyper {
-  float keep;          // 1 - lr wd
+  float keep, rest;    // 1 - lr wd, as the sum of two numbers
   float rate;          // lr / (1 - b1^t)
   float root;          // 1 / sqrt(1 - b2^t)
   float eps, b1, c1, b2, c2;  // c: 1 - b

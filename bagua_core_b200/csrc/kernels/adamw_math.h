@@ -112,7 +112,11 @@ BAGUA_HD uint32_t above2(uint32_t sum) { return (sum << 13) + (kSlack << 13); }
 
 BAGUA_HD Hyper make_hyper(const GroupValues& g, int64_t step, uint64_t seed) {
   Hyper h;
-  h.keep = (float)(1.0 - g.lr * g.weight_decay);
+  // (the first one nearer to 0, so that both have the sign of their sum: an infinite parameter, as a mask may be, stays so)
+  const double keep = 1.0 - g.lr * g.weight_decay;
+  h.keep = (float)keep;
+  if (fabs((double)h.keep) >= fabs(keep) && h.keep != 0) h.keep = bits_float(float_bits(h.keep) - 1);
+  h.rest = (float)(keep - h.keep);
   h.rate = (float)(g.lr / (1.0 - pow(g.b1, (double)step)));
   h.root = (float)(1.0 / sqrt(1.0 - pow(g.b2, (double)step)));
   h.eps = (float)g.eps;
@@ -205,11 +209,12 @@ BAGUA_HD uint32_t second_code64(double v, double per, uint32_t random) {
 BAGUA_HD float parameter(const Hyper& h, float p, float m, float v) {
 #ifdef __CUDA_ARCH__
   const float d = __fmaf_rn(__fsqrt_rn(v), h.root, h.eps);
-  return __fmaf_rn(p, h.keep, -__fmul_rn(h.rate, __fdiv_rn(m, d)));
+  const float u = __fmul_rn(h.rate, __fdiv_rn(m, d));
 #else
   const float d = __builtin_fmaf(__builtin_sqrtf(v), h.root, h.eps);
-  return __builtin_fmaf(p, h.keep, -(h.rate * (m / d)));
+  const float u = h.rate * (m / d);
 #endif
+  return multiply_add(p, h.keep, multiply_add(p, h.rest, -u));
 }
 BAGUA_HD void update(const Hyper& h, float& p, float g, float& m, float& v) {
   moments(h, g, product(h.b1, m), product(h.b2, v), m, v);

@@ -246,6 +246,40 @@ def test_fp32_moments_that_start_anywhere():
     check_unaligned32("cpu")
 
 
+def check_weight_decay(device):
+    """A decay of a few steps of fp32 and less is taken as it is: the new parameter is off by its own rounding and the update's, no more."""
+    n = 20000
+    for lr, wd in ((1e-2, 0.1), (5e-5, 1e-2), (2e-5, 1e-2), (1e-6, 1e-2), (1e-3, 0.0)):
+        for bits in (32, 8):
+            g = torch.Generator().manual_seed(3)
+            p, grad = torch.randn(n, generator=g), torch.randn(n, generator=g)
+            if bits == 8:
+                m, v, scales = ops.adamw_state8(p)
+            else:
+                m, v, scales = torch.zeros(n), torch.zeros(n), None
+            want, _, _ = plain.step(p, grad, torch.zeros(n), torch.zeros(n), 1, lr, 0.9, 0.999, 1e-8, wd)
+            q, m, v = (x.clone().to(device) for x in (p, m, v))
+            ops.adamw_step([q], [grad.to(device)], [m], [v], step=1, lr=lr, weight_decay=wd, scales=None if scales is None else [scales.to(device)])
+            step = 2.0 ** (want.abs().log2().floor() - 23)
+            # the first step's update is lr: its factors, moments, root, division and sum, 16 roundings at most, or 2^-21 with the GPU's
+            # approximate root and reciprocal; the decay's own factor and product
+            assert ((q.cpu().double() - want).abs() <= step / 2 * (1 + 2.0 ** -10) + 2.0 ** -20 * lr + 4 * U * lr * wd * want.abs()).all()
+            # infinite ones stay, next to others that are as they were
+            inf = p.clone()
+            inf[5::300], inf[7::300], inf[-1] = -float("inf"), float("inf"), -float("inf")
+            r = inf.to(device)
+            if bits == 8:
+                m, v, scales = (x.to(device) for x in ops.adamw_state8(p))
+            else:
+                m, v = torch.zeros_like(r), torch.zeros_like(r)
+            ops.adamw_step([r], [grad.to(device)], [m], [v], step=1, lr=lr, weight_decay=wd, scales=None if scales is None else [scales])
+            assert torch.equal(r, torch.where(inf.isinf().to(device), inf.to(device), q))
+
+
+def test_weight_decay_is_taken_as_it_is():
+    check_weight_decay("cpu")
+
+
 def check_versions(device):
     """A graph whose values a step has changed since is noticed."""
     p = torch.ones(4, device=device, requires_grad=True)

@@ -40,6 +40,10 @@ def test_graphs_notice_a_step():
     host.check_versions("cuda")
 
 
+def test_weight_decay_is_taken_as_it_is():
+    host.check_weight_decay("cuda")
+
+
 def test_graphs_notice_all_that_is_written():
     host.check_versions_of_all_written("cuda")
 
