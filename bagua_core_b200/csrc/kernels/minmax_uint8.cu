@@ -26,9 +26,8 @@
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
-#include <map>
-#include <mutex>
 
+#include "clusters.h"
 #include "kernels_impl.h"
 #include "launch.cuh"
 #include "minmax_device.cuh"
@@ -590,47 +589,23 @@ uint32_t next_tag() {
   return t;
 }
 
+// Lets a kernel form clusters of more than 8 blocks.  `allowed`: its own, by device; set twice does no harm.
+template <typename K>
+void allow_large_clusters(K kernel, std::atomic<uint64_t>& allowed) {
+  int dev = 0;
+  BAGUA_CUDA_CHECK(cudaGetDevice(&dev));
+  if (allowed.load(std::memory_order_relaxed) >> (dev & 63) & 1) return;
+  BAGUA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  allowed |= 1ull << (dev & 63);
+}
+
 // The largest cluster that the stream's context can run: 16 blocks on the whole GPU, 8 in a green context of any size, fewer under other
-// limits.  Asked once per stream, by an id that no other stream of the process gets.
+// limits.
 int largest_cluster(cudaStream_t s) {
-  // (never given back: engine threads may outlive static objects)
-  static std::mutex& mu = *new std::mutex;
-  static std::map<unsigned long long, int>& known = *new std::map<unsigned long long, int>;
-  static thread_local unsigned long long last_id = 0;
-  static thread_local int last = -1;
-  unsigned long long id = 0;
-  const bool has_id = cudaStreamGetId(s, &id) == cudaSuccess;
-  if (has_id && last >= 0 && id == last_id) return last;
-  if (!has_id) cudaGetLastError();
-  std::lock_guard<std::mutex> g(mu);
-  int largest = -1;
-  if (auto it = known.find(id); has_id && it != known.end()) largest = it->second;
-  if (largest < 0) {
-    auto* kernel = compress_kernel<float, true, true>;
-    BAGUA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    for (largest = 16; largest > 1; largest /= 2) {
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = (unsigned)largest;
-      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3((unsigned)largest);
-      cfg.blockDim = dim3(kThreads);
-      cfg.stream = s;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      int fit = 0;
-      if (cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) == cudaSuccess && fit > 0) break;
-      cudaGetLastError();
-    }
-    if (known.size() >= 256) known.clear();
-    if (has_id) known[id] = largest;
-  }
-  if (has_id) {
-    last_id = id;
-    last = largest;
-  }
-  return largest;
+  static std::atomic<uint64_t> allowed{0};
+  auto* kernel = compress_kernel<float, true, true>;
+  allow_large_clusters(kernel, allowed);
+  return fitting_cluster((const void*)kernel, 16, kThreads, 0, s);
 }
 
 template <typename T>
@@ -649,13 +624,8 @@ void compress_t(const void* in, int64_t num_real, int64_t chunk, int n_chunks, u
   }
   if (blocks > 1) {
     auto* kernel = aligned ? compress_kernel<T, true, true> : compress_kernel<T, false, true>;
-    static std::atomic<uint64_t> allowed[2] = {};  // by device; set twice does no harm
-    int dev = 0;
-    BAGUA_CUDA_CHECK(cudaGetDevice(&dev));
-    if (!(allowed[aligned].load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
-      BAGUA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-      allowed[aligned] |= 1ull << (dev & 63);
-    }
+    static std::atomic<uint64_t> allowed[2] = {};
+    allow_large_clusters(kernel, allowed[aligned]);
     launch_clusters(kernel, count, blocks, dim3(kThreads), s, (const T*)in, num_real, chunk, first, count, 1, count, blocks, out, off,
                     (unsigned long long*)nullptr, 0u);
     return;
