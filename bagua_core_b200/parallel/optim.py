@@ -363,13 +363,22 @@ class FlatAdamW(_FlatOptimizer):
                 if p in self.state:
                     self.state[p]["step"] = self._plan_groups[self._plan_group_of[id(p)]][1]
 
-    def _copy_state(self, to, saved):
-        names = set(to)
-        if set(saved) != names or any(saved[k].shape != to[k].shape for k in names - {"step"}):
+    def _check_state(self, p, saved):
+        """Throws unless `saved` can be the state of `p`."""
+        held = torch.uint8 if self.state_bits == 8 else torch.float32
+        want = {"exp_avg": (p.shape, held), "exp_avg_sq": (p.shape, held)}
+        if self.state_bits == 8:
+            want["scales"] = ((2, (p.numel() + _C.moment8_block - 1) // _C.moment8_block), torch.float32)
+        if set(saved) != {"step", *want} or any(saved[k].shape != shape for k, (shape, _) in want.items()):
             raise ValueError(f"the saved state of a parameter is not that of moments in {self.state_bits} bits of its size")
-        for k in names - {"step"}:
-            if saved[k].dtype != to[k].dtype:
-                raise ValueError(f"the saved moments are {saved[k].dtype}, not {to[k].dtype}")
+        for k, (_, dtype) in want.items():
+            if saved[k].dtype != dtype:
+                raise ValueError(f"the saved moments are {saved[k].dtype}, not {dtype}")
+        if int(saved["step"]) < 0:
+            raise ValueError(f"the saved state of a parameter has taken {int(saved['step'])} steps")
+
+    def _copy_state(self, to, saved):
+        for k in set(to) - {"step"}:
             to[k].copy_(saved[k])
         to["step"] = int(saved["step"])
 
@@ -377,20 +386,36 @@ class FlatAdamW(_FlatOptimizer):
         self._sync_steps()
         return super().state_dict()
 
-    @torch.no_grad()
     def load_state_dict(self, state_dict):
-        # (torch's own would cast the codes of 8-bit moments to the parameters' type)
-        held, saved = dict(self.state), state_dict["state"]
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
-            state = held[p] if id(p) in self._attached_ids else self._new_state(p)
-            if i in saved:
-                self._copy_state(state, saved[i])
-            elif id(p) in self._attached_ids:
-                self._copy_state(state, self._new_state(p))
-            else:
+        """A state that does not fit is refused before anything has changed."""
+        # The framework's own loads everything but the moments, which it would cast to the parameters' type: they are taken out behind
+        # the hooks in front of it, and put in ahead of the hooks behind it.
+        held, saved = dict(self.state), {}
+
+        def take(_, state_dict):
+            ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+            for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+                if i in state_dict["state"]:
+                    self._check_state(p, state_dict["state"][i])
+                    saved[id(p)] = state_dict["state"][i]
+            return {**state_dict, "state": {}}
+
+        hooks = [self.register_load_state_dict_pre_hook(take),
+                 self.register_load_state_dict_post_hook(lambda _: self._put_state(held, saved), prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for h in hooks:
+                h.remove()
+
+    @torch.no_grad()
+    def _put_state(self, held, saved):
+        for p in (p for g in self.param_groups for p in g["params"]):
+            flat = id(p) in self._attached_ids
+            if id(p) not in saved and not flat:
                 continue  # made by its first step
+            state = held[p] if flat else self._new_state(p)
+            self._copy_state(state, saved[id(p)] if id(p) in saved else self._new_state(p))
             self.state[p] = state
         if self._flat:
             self._plan = self._make_plan()

@@ -503,6 +503,71 @@ def test_training_goes_on_from_a_checkpoint(bits):
         assert all(torch.equal(x, y) for x, y in zip(a, b)) and all(torch.equal(x, y) for x, y in zip(a, c))
 
 
+def _refused(rank, world):
+    import bagua_core_b200.parallel as P
+    from bagua_core_b200.models import MLP
+
+    P.init_process_group(torch.device("cpu"))
+    out = []
+    for bits in (8, 32):
+        torch.manual_seed(7)
+        model, loose = MLP(16, 33, 5, depth=2), torch.nn.Parameter(torch.randn(300))
+        opt = P.FlatAdamW([*model.parameters(), loose], lr=1e-2, state_bits=bits)
+        bm = P.with_bagua(model, [opt], P.GradientAllReduceAlgorithm(), bucket_bytes=4096)
+
+        def run(steps):
+            for s in range(steps):
+                opt.zero_grad()
+                torch.nn.functional.mse_loss(bm(torch.randn(4, 16)), torch.randn(4, 5)).backward()
+                loose.grad = torch.randn(300)
+                opt.step()
+
+        run(3)
+        good = copy.deepcopy(opt.state_dict())
+        run(2)
+        now = copy.deepcopy(opt.state_dict())
+        wrong = []
+        for _ in range(7):
+            w = copy.deepcopy(good)
+            w["param_groups"][0]["lr"] = 7.0
+            wrong.append(w)
+        last = max(good["state"])  # the loose one; the flat ones in front of it fit
+        other = {"step": 1, "exp_avg": torch.zeros(300), "exp_avg_sq": torch.zeros(300)}
+        wrong[0]["state"][last] = other if bits == 8 else {**other, "scales": torch.zeros(2, 2)}
+        wrong[1]["state"][last]["exp_avg"] = wrong[1]["state"][last]["exp_avg"][:-1]
+        wrong[2]["state"][last]["exp_avg_sq"] = wrong[2]["state"][last]["exp_avg_sq"].double()
+        wrong[3]["state"][last]["step"] = -1
+        del wrong[4]["state"][0]["exp_avg"]
+        wrong[5]["param_groups"].append(wrong[5]["param_groups"][0])
+        del wrong[6]["state"]
+        for w in wrong:
+            with pytest.raises((ValueError, KeyError)):
+                opt.load_state_dict(w)
+            got = opt.state_dict()
+            same = got["param_groups"] == now["param_groups"] and got["state"].keys() == now["state"].keys()
+            for k, st in got["state"].items():
+                same = same and all(torch.equal(torch.as_tensor(x), torch.as_tensor(now["state"][k][n])) for n, x in st.items())
+            out.append(same)
+        # hooks see, and may adapt, what is loaded
+        seen = []
+        hooks = [opt.register_load_state_dict_pre_hook(lambda o, d: {**d, "state": {k: dict(v, step=v["step"] + 10) for k, v in d["state"].items()}}),
+                 opt.register_load_state_dict_post_hook(lambda o: seen.append(sorted(s["step"] for s in o.state.values())))]
+        opt.load_state_dict(good)
+        out.append(seen[0] == [13] * len(good["state"]) and sorted(s["step"] for s in opt.state_dict()["state"].values()) == seen[0])
+        for h in hooks:
+            h.remove()
+        run(1)
+        out.append(sorted({s["step"] for s in opt.state_dict()["state"].values()}) == [14])
+    P.destroy_process_group()
+    return out
+
+
+def test_a_refused_checkpoint_changes_nothing():
+    from mp_util import run_ranks
+
+    assert all(run_ranks(_refused, 1)[0])
+
+
 def _decentralized(rank, world):
     import bagua_core_b200.parallel as P
     from bagua_core_b200.models import MLP
