@@ -15,7 +15,7 @@ from typing import List, Tuple
 import torch
 
 from .._native import C as _C
-from ..ops.adamw import adamw_read8, adamw_state8, adamw_step
+from ..ops.adamw import MOMENT8_BLOCK, adamw_read8, adamw_state8, adamw_step
 
 
 def _is_dense(t: torch.Tensor) -> bool:
@@ -29,6 +29,45 @@ def _is_dense(t: torch.Tensor) -> bool:
             return False
         expect *= sz
     return True
+
+
+def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """True if the elements of two dense tensors of one shape follow each other in memory alike."""
+    return a.numel() <= 1 or all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+
+
+@torch.no_grad()
+def _copy_moments8(to: dict, saved: dict) -> None:
+    """8-bit moments into codes and scales whose elements may follow each other in another order.
+
+    A block is 256 neighbours in memory: in another order it has other elements, whose values are read and rounded anew, each to the
+    nearest code of its new block's scale."""
+    m, v = saved["exp_avg"], saved["exp_avg_sq"]
+    if _same_order(m, to["exp_avg"]):
+        for k in ("exp_avg", "exp_avg_sq", "scales"):
+            to[k].copy_(saved[k])
+        return
+    device, n = to["exp_avg"].device, m.numel()
+    values = [torch.empty_like(m, dtype=torch.float32) for _ in range(2)]
+    adamw_read8([m], [v], [saved["scales"]], values[:1], values[1:])
+    codes = torch.arange(256, dtype=torch.uint8)
+    tables = [torch.empty(256) for _ in range(2)]
+    adamw_read8([codes], [codes], [torch.ones(2, 1)], tables[:1], tables[1:])
+    blocks = to["scales"].shape[1]
+    for row, (k, largest, last) in enumerate((("exp_avg", 480, 128), ("exp_avg_sq", 496, 256))):
+        table = tables[row][:last].to(device)
+        x = torch.empty_like(to[k], dtype=torch.float32).copy_(values[row]).as_strided((n,), (1,))
+        x = torch.nn.functional.pad(x, (0, blocks * MOMENT8_BLOCK - n)).view(blocks, MOMENT8_BLOCK)
+        top = x.abs().amax(1)
+        scale = torch.where(top > 0, (top * (1.0 / largest)).clamp(min=2.0 ** -126), top)
+        to["scales"][row].copy_(torch.where(top.isfinite(), scale, float("nan")))
+        y = x.abs().double() / torch.where(scale > 0, scale, 1.0).double()[:, None]
+        code = torch.bucketize(y, ((table[1:] + table[:-1]) / 2).double())
+        if row:
+            code = torch.where(x > 0, code.clamp(min=1), code)  # (not zero: the step divides by it)
+        else:
+            code = code + 128 * (x < 0)
+        to[k].as_strided((n,), (1,)).copy_(code.flatten()[:n])
 
 
 class _FlatOptimizer(torch.optim.Optimizer):
@@ -261,7 +300,8 @@ class FlatAdamW(_FlatOptimizer):
     `seed` is that of their rounding, the same on all ranks.  `moments(p)` reads a parameter's moments.
 
     The state of a parameter (`state[p]`, `state_dict()`, `load_state_dict()`) is `step` with `exp_avg` and `exp_avg_sq`, to which
-    8 bits add `scales`; it goes along when a bucket is laid out (again).
+    8 bits add `scales`; it goes along when a bucket is laid out (again).  Where a parameter's elements then follow each other in another
+    order in memory, 8-bit moments are rounded anew, as other elements share their scales.
 
     `capturable=True`: the steps of the flat buffers are counted on the device, so that `step()` can be captured into a CUDA
     graph and replayed (with the learning rates that it was captured with).  It is captured again after a new layout, and after a
@@ -309,7 +349,7 @@ class FlatAdamW(_FlatOptimizer):
             p, n = t.owner, t.owner.numel()
             state = {"step": 0, **{k: f[off:off + n].as_strided(tuple(p.shape), tuple(p.stride())) for k, f in flat.items()}}
             if self.state_bits == 8:
-                state["scales"] = torch.zeros(2, (n + _C.moment8_block - 1) // _C.moment8_block, device=p.device)
+                state["scales"] = torch.zeros(2, (n + MOMENT8_BLOCK - 1) // MOMENT8_BLOCK, device=p.device)
             if p in self.state and "step" in self.state[p]:  # steps taken before, here or in another layout
                 self._copy_state(state, self.state[p])
             self.state[p] = state
@@ -368,18 +408,23 @@ class FlatAdamW(_FlatOptimizer):
         held = torch.uint8 if self.state_bits == 8 else torch.float32
         want = {"exp_avg": (p.shape, held), "exp_avg_sq": (p.shape, held)}
         if self.state_bits == 8:
-            want["scales"] = ((2, (p.numel() + _C.moment8_block - 1) // _C.moment8_block), torch.float32)
+            want["scales"] = ((2, (p.numel() + MOMENT8_BLOCK - 1) // MOMENT8_BLOCK), torch.float32)
         if set(saved) != {"step", *want} or any(saved[k].shape != shape for k, (shape, _) in want.items()):
             raise ValueError(f"the saved state of a parameter is not that of moments in {self.state_bits} bits of its size")
         for k, (_, dtype) in want.items():
             if saved[k].dtype != dtype:
                 raise ValueError(f"the saved moments are {saved[k].dtype}, not {dtype}")
+        if self.state_bits == 8 and not (_is_dense(saved["exp_avg"]) and _same_order(saved["exp_avg"], saved["exp_avg_sq"])):
+            raise ValueError("the saved codes of 8-bit moments have gaps, or two orders: which of them share a scale goes by their places in memory")
         if int(saved["step"]) < 0:
             raise ValueError(f"the saved state of a parameter has taken {int(saved['step'])} steps")
 
     def _copy_state(self, to, saved):
-        for k in set(to) - {"step"}:
-            to[k].copy_(saved[k])
+        if self.state_bits == 8:
+            _copy_moments8(to, saved)
+        else:
+            for k in ("exp_avg", "exp_avg_sq"):
+                to[k].copy_(saved[k])
         to["step"] = int(saved["step"])
 
     def state_dict(self):
@@ -468,8 +513,9 @@ class FlatAdamW(_FlatOptimizer):
                 back.append((p, w))
             m = state["exp_avg"]
             if m.stride() != w.stride():  # the parameter has been laid out anew since
-                for k in ("exp_avg", "exp_avg_sq"):
-                    state[k] = torch.empty_like(w, dtype=m.dtype).copy_(state[k])
+                new = self._new_state(w)
+                self._copy_state(new, state)
+                state.update(new)
             if g.layout == torch.strided and g.stride() != w.stride():
                 g = torch.empty_like(w, dtype=g.dtype).copy_(g)
             key = (id(group), state["step"], p.device, p.dtype, g.dtype)

@@ -503,6 +503,84 @@ def test_training_goes_on_from_a_checkpoint(bits):
         assert all(torch.equal(x, y) for x, y in zip(a, b)) and all(torch.equal(x, y) for x, y in zip(a, c))
 
 
+def near_moments8(opt, p, m, v, decay=(1.0, 1.0), steps=1):
+    """The moments of `p` are m and v, each rounded to the nearest code of its block, then `steps - 1` times to a neighbouring one: a code's
+    distance is an eighth (first moment) or a sixteenth of its value, and 2^-9 or 2^-10 of the scale for the smallest."""
+    state = opt.state[p]
+    flat = lambda t: torch.empty_like(state["exp_avg"], dtype=torch.float64).copy_(t).as_strided((t.numel(),), (1,))  # noqa: E731
+    for row, (got, old, part, least) in enumerate(zip(opt.moments(p), (m, v), (2.0 ** -3, 2.0 ** -4), (2.0 ** -9, 2.0 ** -10))):
+        got, old = flat(got), flat(old)
+        scale = plain.spread(state["scales"][row].cpu(), p.numel()).to(got.device)
+        want = old * decay[row]
+        bound = (steps - 0.5) * (1 + 1e-3) * torch.maximum(torch.maximum(old.abs(), want.abs()) * part * 1.2, scale * least)
+        if row:
+            bound = torch.maximum(bound, scale * least)  # held above zero
+            assert (got > 0)[old > 0].all()
+        assert ((got - want).abs() <= bound).all(), (row, float(((got - want).abs() / bound).max()))
+
+
+def in_another_order(device):
+    """A parameter with 8-bit moments of a few steps, and its values with the channels last: blocks of other elements, of other sizes."""
+    torch.manual_seed(0)
+    p = torch.nn.Parameter(torch.randn(40, 24, 3, 3, device=device))
+    opt = P.FlatAdamW([p], state_bits=8)
+    for _ in range(3):
+        p.grad = torch.randn_like(p) * torch.rand(40, 1, 1, 1, device=device).mul(6).exp()
+        opt.step()
+    return p, opt, p.detach().clone().contiguous(memory_format=torch.channels_last)
+
+
+def check_other_orders(device):
+    p, opt, last = in_another_order(device)
+    m, v = opt.moments(p)
+    # a checkpoint of one order in a model of another, and back
+    q = torch.nn.Parameter(last)
+    other = P.FlatAdamW([q], state_bits=8)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    assert other.state[q]["exp_avg"].stride() == q.stride()
+    near_moments8(other, q, m, v)
+    m2, v2 = other.moments(q)
+    opt.load_state_dict(other.state_dict())
+    near_moments8(opt, p, m2, v2)
+    # laid out anew between two steps
+    m, v = opt.moments(p)
+    p.data = last
+    p.grad = torch.zeros_like(p)
+    opt.step()
+    near_moments8(opt, p, m, v, (0.9, 0.999), steps=2)
+    # codes that say nothing of their order
+    bad = copy.deepcopy(opt.state_dict())
+    bad["state"][0]["exp_avg"] = torch.zeros(40, 24, 3, 6, dtype=torch.uint8, device=device)[..., ::2]
+    with pytest.raises(ValueError, match="gaps"):
+        opt.load_state_dict(bad)
+
+
+def test_8_bit_moments_in_another_order():
+    check_other_orders("cpu")
+
+
+def _other_order_in_a_bucket(rank, world):
+    import bagua_core_b200.parallel as P
+
+    P.init_process_group(torch.device("cpu"))
+    p, opt, last = in_another_order("cpu")
+    m, v = opt.moments(p)
+    model = torch.nn.Conv2d(24, 40, 3, bias=False)
+    p.data, p.grad = last, None  # (a gradient has the parameter's layout)
+    model.weight = p
+    P.with_bagua(model, [opt], P.GradientAllReduceAlgorithm())
+    attached = id(p) in opt._attached_ids and p.stride() == last.stride()
+    near_moments8(opt, p, m, v)
+    P.destroy_process_group()
+    return attached
+
+
+def test_8_bit_moments_in_another_order_go_into_a_bucket():
+    from mp_util import run_ranks
+
+    assert run_ranks(_other_order_in_a_bucket, 1)[0]
+
+
 def _refused(rank, world):
     import bagua_core_b200.parallel as P
     from bagua_core_b200.models import MLP

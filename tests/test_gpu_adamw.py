@@ -40,6 +40,10 @@ def test_graphs_notice_a_step():
     host.check_versions("cuda")
 
 
+def test_8_bit_moments_in_another_order():
+    host.check_other_orders("cuda")
+
+
 def test_weight_decay_is_taken_as_it_is():
     host.check_weight_decay("cuda")
 
