@@ -46,6 +46,16 @@ class ScaledEmbedding(nn.Embedding):
         self.scale = scale
         self.dtype_out = dtype_out
 
+    @classmethod
+    def from_pretrained(cls, embeddings: torch.Tensor, freeze: bool = True, padding_idx: Optional[int] = None, scale: float = 1.0,
+                        dtype_out: Optional[torch.dtype] = None) -> "ScaledEmbedding":
+        """One whose table is `embeddings`, as `nn.Embedding.from_pretrained` makes it."""
+        if embeddings.dim() != 2:
+            raise ValueError("a table has rows and columns")
+        made = cls(*embeddings.shape, scale=scale, padding_idx=padding_idx, dtype_out=dtype_out, device="meta")
+        made.weight = nn.Parameter(embeddings, requires_grad=not freeze)
+        return made
+
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
         dtype, dev = self.dtype_out, ids.device.type
         if dtype is None and torch.is_autocast_enabled(dev):

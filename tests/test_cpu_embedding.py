@@ -127,6 +127,19 @@ def test_second_order():
     check_second_order("cpu")
 
 
+def test_module_of_a_given_table():
+    table = torch.randn(10, 8)
+    m = ops.ScaledEmbedding.from_pretrained(table, padding_idx=-1, scale=2.0)
+    ids = torch.tensor([3, 9])
+    assert m.weight.data_ptr() == table.data_ptr() and not m.weight.requires_grad and m.padding_idx == 9
+    assert (m.num_embeddings, m.embedding_dim) == (10, 8) and torch.equal(m(ids), 2.0 * table[ids])
+    m = ops.ScaledEmbedding.from_pretrained(table, freeze=False, dtype_out=torch.bfloat16)
+    m(ids).sum().backward()
+    assert m(ids).dtype == torch.bfloat16 and m.weight.grad.sum() == 16
+    with pytest.raises(ValueError):
+        ops.ScaledEmbedding.from_pretrained(table[0])
+
+
 def check_module(device):
     m = ops.ScaledEmbedding(10, 8, scale=3.0, padding_idx=2).to(device)
     ids = torch.tensor([[0, 2], [9, 9]], device=device)
