@@ -39,7 +39,8 @@ BAGUA_HD float bits_float(uint32_t u) {
 #endif
 }
 
-// A bijection of 32 bits, shifts and odd multipliers in turn, whose every output bit depends on every input bit.
+// A bijection of 32 bits, shifts and odd multipliers in turn, whose every output bit depends on every input bit: the published hash
+// lowbias32, whose constants C. Wellons found by a search for the least bias (2018, in the public domain).
 BAGUA_HD uint32_t mix(uint32_t x) {
   x ^= x >> 16;
   x *= 0x7feb352du;
