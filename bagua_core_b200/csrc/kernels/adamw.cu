@@ -1,6 +1,7 @@
 // See adamw.h.  Streams over memory: with fp32 parameters, gradients and moments 28 bytes an element, 16 with moments in 8 bits.
-// 131 M elements: 534 us with fp32 moments (6.95 TB/s, above the rate of a copy), 319 with 8 bits (6.6 TB/s; integer
-// instructions are issued in three quarters of all cycles), 120 to read those into bf16 (6.6 TB/s).
+// 131 M elements, twenty calls in a row, the best of nine such: 526 us with fp32 moments (6.97 TB/s, above the rate of a copy), 320 with
+// 8 bits (6.6 TB/s; instructions are issued in three quarters of all cycles), 120 to read those into bf16 (6.6 TB/s).  Figures below
+// are taken alike.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -133,10 +134,11 @@ __global__ void __launch_bounds__(kThreads) step32_kernel(const __grid_constant_
 // So two elements are computed by one instruction where there is one; the square root and the reciprocal are the hardware's (within 2^-22 each: a
 // parameter is off by that part of its update); the moments' betas go into the factor that decodes them, and both directions of coding take
 // one factor.  A block with a scale beyond kPlainScale, or an eps so small that a subnormal square root counts next to
-// it, goes the longer way.  2 % of the blocks hold codes that fp32 leaves open.  Coding takes byte permutations where it can:
-// with shifts and masks 131 M elements took 358 us, now 319 (bf16 parameters and gradients: 364, 304).
-// Blocks on an SM: so many leave 40 registers a thread and a few spilled ones.  131 M elements take 317 us, with five (48 registers)
-// 337, seven (32) 355: the loads of waiting warps are worth more than the spills cost.  A warp that took two blocks in turn held
+// it, goes the longer way.  2.3 % of the blocks hold codes that fp32 leaves open (256 elements, each with 2^-15 and 2^-14 of the random
+// bits near a border).  Coding takes byte permutations where it can: with shifts and masks 131 M elements took 358 us where they took 316
+// (bf16 parameters and gradients: 364, 306).  The weight decay's second factor made 320 of those, and 310.
+// Blocks on an SM: so many leave 40 registers a thread and a few spilled ones.  131 M elements take 320 us, with five (48 registers)
+// 341, seven (32) 347: the loads of waiting warps are worth more than the spills cost.  A warp that took two blocks in turn held
 // more registers over the turn than it had (434 us where one took 362).
 constexpr int kResident8 = 6;
 constexpr int kTile8 = kThreads / 32 * kMoment8Block;
@@ -176,8 +178,8 @@ __device__ __forceinline__ uint32_t top_bytes(const uint32_t (&x)[4]) {
 }
 static_assert(kSlack == 16, "whole numbers of the random bits' steps, which the short way counts");
 
-// A block's codes and scales in 64 bits, by the whole warp: one block in forty.  (131 M elements take 317 us with two elements at a
-// time, 320 with one; before the codes took byte permutations 358, 362, and 364 with four.)
+// A block's codes and scales in 64 bits, by the whole warp: 2.3 % of them.  (131 M elements take 320 us with two elements at a time, 323
+// with one.)
 template <typename G>
 __device__ __forceinline__ void code_in_64_bits(const Segment& a, const Hyper& h, uint32_t key, int64_t block) {
   const int lane = (int)threadIdx.x & 31;
