@@ -134,6 +134,45 @@ def test_special_rows():
     check_special("cpu")
 
 
+def check_ends_of_the_range(device):
+    """Rows with logits at the ends of the type's range have the values that their formula says, whatever the size of their logits."""
+    g = torch.Generator().manual_seed(11)
+    for dtype in TYPES.values():
+        low, top = torch.finfo(dtype).min, torch.finfo(dtype).max
+        for vocab in (40, 1000, 3000):
+            x = torch.zeros(8, vocab)
+            x[0] = low                                # all equal
+            x[1] = top
+            x[2] = low                                # one left
+            x[2, 9] = 0.25
+            x[3], x[3, 9] = low, low / 2              # one left among large ones
+            x[4, ::2], x[4, 1::2] = low, 0.0          # a half, all alike
+            x[5, :10], x[5, 10:] = top, low           # ten
+            x[6], x[6, :vocab // 2] = low, -INF       # half of nothing but the lowest
+            x[7], x[7, 9] = 1.0, top                  # one far above
+            n = torch.tensor([vocab, vocab, 1, 1, vocab // 2, 10, vocab - vocab // 2, 1.0])
+            t = torch.tensor([1, 1, 9, 9, 1, 0, vocab - 1, 9])
+            b = torch.randn(8, generator=g)
+            y = x.to(dtype).to(device).requires_grad_()
+            r = ops.token_log_probs(y, t.to(device), 3)
+            (d,) = torch.autograd.grad((r.log_probs, r.entropy), y, (torch.ones(8, device=device), b.to(device)))
+            # logarithms below 2^3.1 in base 2: sums of up to 3000 exact ones, log2 and its product, within 2^-20
+            close(r.log_probs, -n.double().log(), 2.0 ** -20)
+            # each p log p: p is off by half a step of its logarithm (up to 8, so 2^-22), by exp's step and a half, and by the product's half:
+            # 2^-21 of it at most, and the whole, up to 8, by that and half a step for each of the levels of its sum
+            close(r.entropy, n.double().log(), 2.0 ** -17)
+            assert torch.equal(r.top_ids[:, 0].cpu(), torch.tensor([0, 0, 9, 9, 1, 0, vocab // 2, 9]))
+            close(r.top_log_probs[:, 0], -n.double().log(), 2.0 ** -20)
+            # all that are left are alike: no gradient of the entropy, and 1 / n of the log probability's
+            left = (x.to(dtype) == x.to(dtype).amax(1, keepdim=True)).double()
+            want = torch.zeros(8, vocab, dtype=torch.float64).scatter_(1, t[:, None], 1.0) - left / n.double()[:, None]
+            close(d, want, (torch.finfo(dtype).eps / 2 + 2.0 ** -20) * want.abs() + 2.0 ** -20 * (1 + b.abs()[:, None]) * left)
+
+
+def test_ends_of_the_range():
+    check_ends_of_the_range("cpu")
+
+
 def check_layouts(device):
     x, t = logits(24, 37, torch.bfloat16)
     x, t = x.to(device), t.to(device)

@@ -69,6 +69,10 @@ def test_special_rows():
     host.check_special("cuda")
 
 
+def test_ends_of_the_range():
+    host.check_ends_of_the_range("cuda")
+
+
 def test_layouts():
     host.check_layouts("cuda")
 
