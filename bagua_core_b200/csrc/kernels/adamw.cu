@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kThreads) step32_kernel(const __grid_constant_
 // ---- moments in 8 bits --------------------------------------------------------------------------
 // A warp takes a block of elements that share their scales, eight to a lane: the largest value of a block is a reduction over the
 // warp's registers, and each element is read and written once.  Lanes hold two runs of four, so that the 32 loads of a run are one
-// piece of memory; elements of an address that no vector fits are taken one by one, lane by lane.
+// piece of memory; elements of an address that no vector fits are taken one by one, lane by lane (131 M elements: 562 us instead of 320).
 //
 // With 16 bytes an element instead of 28, instructions count as much as bytes (at 89 an element 67 M elements took 234 us).
 // So two elements are computed by one instruction where there is one; the square root and the reciprocal are the hardware's (within 2^-22 each: a

@@ -4,7 +4,7 @@
 // block's or a cluster's, by its length and the number of rows.  Bound by memory for long rows (2000 of 131072 in bf16: 86 us, 6.1
 // TB/s; 4096 of 32003 in fp32: 84 us, 6.2), for rows of some tens of KB also by what a block does once a row (4096 of 30522 in bf16:
 // 46 us, 5.4 TB/s; the exponentials alone take 28), for few rows by latency (one of 30522: 3.6 us, with 5 alternatives 7).
-// Backward: reads and writes each logit once, 4096 of 30522 in bf16 in 84 us, 6.0 TB/s.
+// Backward: reads and writes each logit once, 4096 of 30522 in bf16 in 80 us, 6.2 TB/s.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
