@@ -247,7 +247,8 @@ __device__ __forceinline__ bool step8_block(const Segment& a, const Hyper& h, ui
   auto step = [&](auto plain) {
     constexpr bool kPlain = decltype(plain)::value;
     const Pair km = both(__fmul_rn(h.b1, ms) * (kPlain ? kUp : 1.f)), kv = both(__fmul_rn(h.b2, vs) * (kPlain ? kUp : 1.f));
-    const Pair c1 = both(h.c1), c2 = both(h.c2), root = both(h.root), eps = both(h.eps), rate = both(-h.rate), keep = both(h.keep), rest = both(h.rest);
+    const Pair c1 = both(h.c1), c2 = both(h.c2), root = both(h.root), eps = both(h.eps), rate = both(-h.rate);
+    const Pair keep = both(h.keep), rest = both(h.rest);
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
